@@ -9,7 +9,11 @@ is no Triton, no torch fallback and no CPU path: without the native library, or 
 device, every entry point raises.
 
 Page kinds: the reference's "bf16", "fp16", "fp8", "fp8:row", "int8", and "fp8:page": E4M3 codes with one FP32 scale
-per (page, kv head), scales [pages][kv_heads] (scale = amax / 448 over the page's rows of that head).
+per (page, kv head), scales [pages][kv_heads] (scale = amax / 448 over the page's rows of that head); and "int4": 4-bit
+codes, pages uint8 [pages][page][kv_heads][dim / 2] (element 2 i in the low half of byte i), with one byte of scale for
+each group of 32 elements, scales uint8 [pages][page][kv_heads][dim / 32].  The byte is an unsigned float, bits 14..7 of
+an FP16 number: the one nearest to the group's max |x| / 7 (61,440 at most); a code is 8 + rint(x / scale) and stands for
+(code - 8) * scale, at most half a scale from x (scales of 2^-14 and above), exact in 16-bit types.  A group that holds a NaN reads as NaN.
 
 A row's positions are read in contiguous splits of `chunk` positions (one per cache geometry, chunk_for()); the splits'
 states are folded in split order.  This is the reference's "flash" split shape (contiguous splits, __init__.py:580-612)
@@ -25,11 +29,12 @@ import torch
 
 from . import _lib
 
-__all__ = ["KINDS", "MAX_COLUMNS", "attend", "chunk_for", "gather", "merge_shards", "move_rows", "owner", "partitions", "parts_for",
-           "engine_for", "piece_size", "plan", "prefill", "prefill_serves", "release", "slots_at", "states_for", "status", "tcgen05_serves",
+__all__ = ["KINDS", "MAX_COLUMNS", "attend", "chunk_for", "gather", "merge_shards", "move_rows", "norm_rope", "norm_rope_write", "owner",
+           "partitions", "parts_for", "rope_axes", "engine_for", "piece_size", "plan", "prefill", "prefill_serves", "release", "slots_at", "states_for", "status", "tcgen05_serves",
            "tcgen05p_serves", "tile_for", "workspace_floats", "write"]
 
-KINDS = {"bf16": 0, "fp16": 0, "fp8": 1, "fp8:row": 2, "int8": 3, "fp8:page": 4}
+KINDS = {"bf16": 0, "fp16": 0, "fp8": 1, "fp8:row": 2, "int8": 3, "fp8:page": 4, "int4": 5}
+GROUP4 = 32                 # elements of an "int4" row that share a scale
 MAX_COLUMNS = 64            # columns of one row a launch reads
 TILE = 16                   # positions a warp reads per step: chunks and pages are multiples of it
 DEFAULT_CHUNK = 1024
@@ -44,6 +49,19 @@ def _check_kind(kind, key_scales):
     if (KINDS[kind] >= 2) != (key_scales is not None):
         raise ValueError(f"{kind} pages {'take' if KINDS[kind] >= 2 else 'have no'} scales beside their codes")
     return KINDS[kind]
+
+
+def _check4(pages, scales, what):
+    """An "int4" page tensor [...][kv_heads][dim / 2] and its scales [...][kv_heads][dim / 32]: (kv_heads, dim)."""
+    hkv, dim = pages.shape[-2], 2 * pages.shape[-1]
+    if pages.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise ValueError(f"int4 pages and their scales are uint8 tensors: {what} are {pages.dtype} with scales of {scales.dtype}")
+    if dim % GROUP4 or scales.numel() * GROUP4 != pages.numel() * 2 or not scales.is_contiguous():
+        raise ValueError(f"int4 {what} of [{hkv}][{dim}] rows have contiguous scales [...][{hkv}][{dim // GROUP4}], a byte for "
+                         f"each group of {GROUP4} elements")
+    if scales.device != pages.device:
+        raise ValueError(f"int4 {what} and their scales are on one device")
+    return hkv, dim
 
 
 def _cuda(tensor, what):
@@ -251,8 +269,8 @@ def workspace_floats(tokens, heads, partitions, value_dim):
 def write(keys, values, slots, key_pages, value_pages, kind, key_scales=None, value_scales=None,
           multipliers=(1.0, 1.0)):
     """A step's keys [tokens][kv_heads][dim] and values [tokens][kv_heads][value_dim] (bf16, fp16 or fp32) into their
-    slots ([tokens] int64; a slot below 0 is skipped) of one layer's pages (any view whose storage is
-    [slots][kv_heads][dim]), encoded for the page kind, in one launch.  values and value_pages None: keys only; keys
+    slots ([tokens] int64; a slot below 0 is skipped; a slot at most once a call) of one layer's pages (any view whose
+    storage is [slots][kv_heads][dim]; "int4": two elements a byte), encoded for the page kind, in one launch.  values and value_pages None: keys only; keys
     and key_pages None: values only, at the value multiplier.  "fp8:page" takes scales [pages][kv_heads] and the page
     size from the pages' shape ([pages][page][kv_heads][dim]).  Reference: paged_kv_attention/__init__.py:289-324."""
     if keys is None:
@@ -260,11 +278,19 @@ def write(keys, values, slots, key_pages, value_pages, kind, key_scales=None, va
             raise ValueError("write takes keys, values or both")
         return write(values, None, slots, value_pages, None, kind, value_scales, None,
                      multipliers=(multipliers[1], multipliers[1]))
-    k_kind = _check_kind(kind, key_scales)
     _cuda(keys, "keys")
-    T, hkv, d = keys.shape
-    if T == 0:
+    if keys.shape[0] == 0:
+        _check_kind(kind, key_scales)
         return
+    p, _held = _append_params(keys, values, slots, key_pages, value_pages, kind, key_scales, value_scales, multipliers)
+    with torch.cuda.device(keys.device):
+        _lib.check(_lib.load().crit_b200_append(ctypes.byref(p), _stream(keys.device)), "crit_b200.write")
+
+
+def _append_params(keys, values, slots, key_pages, value_pages, kind, key_scales, value_scales, multipliers):
+    """The append's parameter block, its arguments checked, and the tensors it points at that were made here."""
+    k_kind = _check_kind(kind, key_scales)
+    T, hkv, d = keys.shape
     if keys.dtype not in _DTYPES or (values is not None and values.dtype != keys.dtype):
         raise ValueError("keys and values are bf16, fp16 or fp32 tensors of one dtype")
     if keys.stride(-1) != 1:
@@ -276,6 +302,13 @@ def write(keys, values, slots, key_pages, value_pages, kind, key_scales=None, va
     if not key_pages.is_contiguous() or (value_pages is not None and not value_pages.is_contiguous()):
         raise ValueError("pages are contiguous [slots][kv_heads][dim] storage")
     page = 1
+    if k_kind == 5:
+        for rows, pages, scales, what in ((keys, key_pages, key_scales, "keys"), (values, value_pages, value_scales, "values")):
+            if rows is not None:
+                if pages is None or scales is None:
+                    raise ValueError(f"write stores int4 {what} in pages with scales beside them")
+                if _check4(pages, scales, what) != tuple(rows.shape[1:]) or rows.shape[0] != T or pages.device != keys.device:
+                    raise ValueError(f"int4 {what} [{T}][{hkv}][{rows.shape[-1]}] go to pages [...][{hkv}][{rows.shape[-1] // 2}]")
     if k_kind == 4:
         if key_pages.dim() != 4:
             raise ValueError("fp8:page pages are given as [pages][page][kv_heads][dim]")
@@ -285,7 +318,7 @@ def write(keys, values, slots, key_pages, value_pages, kind, key_scales=None, va
     p.key_pages, p.value_pages = _ptr(key_pages), _ptr(value_pages)
     p.key_scales, p.value_scales = _ptr(key_scales), _ptr(value_scales)
     p.tokens = T
-    p.slots_total = key_pages.numel() // (hkv * d)
+    p.slots_total = key_pages.numel() // (hkv * key_pages.shape[-1])
     p.status = _ptr(_status_word(keys.device))
     p.key_stride_token, p.key_stride_head = keys.stride(0), keys.stride(1)
     if values is not None:
@@ -294,25 +327,162 @@ def write(keys, values, slots, key_pages, value_pages, kind, key_scales=None, va
     p.value_dim = values.shape[-1] if values is not None else d
     p.kind, p.in_dtype, p.page_dtype = k_kind, _DTYPES[keys.dtype], _page_dtype(kind, key_pages)
     p.key_multiplier, p.value_multiplier = float(multipliers[0]), float(multipliers[1])
-    with torch.cuda.device(keys.device):
-        _lib.check(_lib.load().crit_b200_append(ctypes.byref(p), _stream(keys.device)), "crit_b200.write")
+    return p, (keys, values)
+
+
+# -- norm and rotation ----------------------------------------------------------------------------------------------------
+def rope_axes(sections, interleaved=False, device="cuda"):
+    """The axis each pair of a head turns with, int32 [sum(sections)]: norm_rope's `axes` for positions of several axes
+    (time, height, width).  sections: the pairs each axis turns.  interleaved False: one axis' pairs after another's; True:
+    the axes take turns, pair by pair, each until its pairs are used up."""
+    sections = [int(n) for n in sections]
+    if not sections or min(sections) < 0:
+        raise ValueError("sections are the numbers of pairs each axis turns")
+    if interleaved:
+        order = sorted((turn, axis) for axis, n in enumerate(sections) for turn in range(n))
+        found = [axis for _, axis in order]
+    else:
+        found = [axis for axis, n in enumerate(sections) for _ in range(n)]
+    return torch.tensor(found, dtype=torch.int32, device=device)
+
+
+def _vectors_fit(x):
+    """Whether rows are read or written in the kernel's vectors of four elements as they lie."""
+    return x.stride(-1) == 1 and not (x.stride(0) | x.stride(1)) % 4 and not x.data_ptr() % (4 * x.element_size())
+
+
+def _vectors(x):
+    """x where the kernel's vectors fit it, else a copy."""
+    return x if _vectors_fit(x) else x.clone(memory_format=torch.contiguous_format)
+
+
+def _norm_rope_params(q, keys, positions, frequencies, q_weight, key_weight, eps, offset, axes, interleaved, magnitude, q_out, keys_out, writes):
+    """norm_rope's arguments checked: (parameter block, [q, keys] as they are read, [q, keys] outputs, outputs to copy)."""
+    given = q if q is not None else keys
+    T, d, device, dtype = given.shape[0], given.shape[-1], given.device, given.dtype
+    for x, what in ((q, "q"), (keys, "keys")):
+        if x is not None and (x.dim() != 3 or x.shape[0] != T or x.shape[-1] != d or x.dtype != dtype or x.device != device or x.dtype not in _DTYPES):
+            raise ValueError(f"q and keys are bf16, fp16 or fp32 tensors [tokens][heads][dim] of one dtype, width and device: {what} is not")
+    if frequencies.dtype != torch.float32 or frequencies.dim() != 1 or not frequencies.is_contiguous() or frequencies.device != device:
+        raise ValueError("frequencies are contiguous FP32 [rotary / 2] on the queries' device")
+    if positions.dtype != torch.int64 or positions.dim() not in (1, 2) or positions.shape[-1] != T or positions.device != device or \
+            (T and positions.stride(-1) != 1):
+        raise ValueError(f"positions are int64 [{T}], or [axes][{T}], on the queries' device")
+    n_axes = positions.shape[0] if positions.dim() == 2 else 1
+    if axes is not None and (axes.dtype != torch.int32 or axes.numel() != frequencies.numel() or not axes.is_contiguous() or axes.device != device):
+        raise ValueError("axes are contiguous int32, one for each frequency (rope_axes)")
+    if axes is None and n_axes > 1:
+        raise ValueError("positions of several axes come with the axis of each pair: axes (rope_axes)")
+    weights = [w for w in (q_weight if q is not None else None, key_weight if keys is not None else None) if w is not None]
+    for w in weights:
+        if w.dtype not in _DTYPES or w.dtype != weights[0].dtype or w.numel() != d or not w.is_contiguous() or w.device != device:
+            raise ValueError(f"q_weight and key_weight are contiguous [{d}] of one bf16, fp16 or fp32 type, on the queries' device")
+    p = _lib.NormRopeParams()
+    reads, outs, copies = [], [], []
+    for x, out, what, side in ((q, q_out, "q", "q"), (keys, keys_out, "keys", "key")):
+        if out is not None and (x is None or out.shape != x.shape or out.dtype != dtype or out.device != device):
+            raise ValueError(f"the {what} output has the shape, dtype and device of {what}")
+        if x is not None and out is None and not (writes and what == "keys"):
+            out = torch.empty(x.shape, dtype=dtype, device=device)
+        outs.append(out)
+        reads.append(None if x is None else _vectors(x))
+        if x is not None:
+            setattr(p, what, x.data_ptr() if reads[-1] is x else reads[-1].data_ptr())
+            setattr(p, side + "_stride_token", reads[-1].stride(0)), setattr(p, side + "_stride_head", reads[-1].stride(1))
+        if out is not None:
+            into = out
+            if not _vectors_fit(out):                  # made beside it and copied
+                into = torch.empty(out.shape, dtype=dtype, device=device)
+                copies.append((out, into))
+            setattr(p, what + "_out", into.data_ptr())
+            setattr(p, side + "_out_stride_token", into.stride(0)), setattr(p, side + "_out_stride_head", into.stride(1))
+    p.q_heads, p.kv_heads = (q.shape[1] if q is not None else 0), (keys.shape[1] if keys is not None else 0)
+    p.positions, p.frequencies, p.axes = _ptr(positions), _ptr(frequencies), _ptr(axes)
+    p.q_weight, p.key_weight = _ptr(q_weight), _ptr(key_weight)
+    p.status = _ptr(_status_word(device))
+    p.tokens, p.axis_stride = T, positions.stride(0) if positions.dim() == 2 else 0
+    p.head_dim, p.rotary, p.n_axes, p.interleaved = d, 2 * frequencies.numel(), n_axes, int(bool(interleaved))
+    p.dtype, p.weight_dtype = _DTYPES[dtype], _DTYPES[weights[0].dtype] if weights else 0
+    p.eps, p.offset, p.magnitude = float(eps), float(offset), float(magnitude)
+    return p, reads, outs, copies
+
+
+def norm_rope(q, keys, positions, frequencies, *, q_weight=None, key_weight=None, eps=1e-6, offset=0.0, axes=None, interleaved=False,
+              magnitude=1.0, q_out=None, keys_out=None):
+    """A step's queries [tokens][heads][dim] and keys [tokens][kv_heads][dim] (bf16, fp16 or fp32; either may be None), each
+    head normed and turned, in one launch -> (queries, keys).
+
+    y = x / sqrt(mean x^2 + eps) * (offset + weight) over each head where its weight [dim] is given; then the first rotary =
+    2 * len(frequencies) elements (a multiple of 8) in pairs, (a, b) -> magnitude * (a cos - b sin, b cos + a sin): pairs
+    (i, rotary / 2 + i), or (2 i, 2 i + 1) with interleaved.  The angle of pair i is position * frequencies[i], made in FP64;
+    positions int64 [tokens], or [axes][tokens] with axes int32 [rotary / 2] naming the axis each pair turns with
+    (rope_axes).  Sums are FP32, a result is rounded once.  q_out / keys_out: where to put them (q and keys themselves for
+    in place).  Heads of 32..256 in steps of 32."""
+    if q is None and keys is None:
+        raise ValueError("norm_rope takes q, keys or both")
+    _cuda(q if q is not None else keys, "q")
+    p, reads, outs, copies = _norm_rope_params(q, keys, positions, frequencies, q_weight, key_weight, eps, offset, axes, interleaved,
+                                               magnitude, q_out, keys_out, False)
+    _launch_norm_rope(p, None, reads, copies, "crit_b200.norm_rope")
+    return outs[0], outs[1]
+
+
+def _launch_norm_rope(p, append, reads, copies, what):
+    if p.tokens == 0:
+        return
+    device = (reads[0] if reads[0] is not None else reads[1]).device
+    with torch.cuda.device(device):
+        _lib.check(_lib.load().crit_b200_norm_rope(ctypes.byref(p), ctypes.byref(append) if append is not None else None, _stream(device)), what)
+    for out, made in copies:
+        out.copy_(made)
+
+
+def norm_rope_write(q, keys, values, positions, frequencies, slots, key_pages, value_pages, kind, key_scales=None, value_scales=None, *,
+                    multipliers=(1.0, 1.0), q_weight=None, key_weight=None, eps=1e-6, offset=0.0, axes=None, interleaved=False,
+                    magnitude=1.0, q_out=None, keys_out=None):
+    """norm_rope with write() in the same launch: the queries and keys normed and turned, the keys and the values [tokens]
+    [kv_heads][value_dim] (None: keys only) stored at their slots of one layer's pages -> the queries.  The keys go to the
+    pages from their FP32 values, with no rounding to their type on the way (16-bit pages hold what norm_rope + write
+    would put there); keys_out takes them too when given.  "fp8:page" pages, whose scales are a page's rows together, take
+    two launches.  Arguments as norm_rope's and write's."""
+    _cuda(q, "q")
+    if keys is None:
+        raise ValueError("norm_rope_write stores keys (and values): pass keys")
+    if kind == "fp8:page":
+        found, turned = norm_rope(q, keys, positions, frequencies, q_weight=q_weight, key_weight=key_weight, eps=eps, offset=offset,
+                                  axes=axes, interleaved=interleaved, magnitude=magnitude, q_out=q_out, keys_out=keys_out)
+        write(turned, values, slots, key_pages, value_pages, kind, key_scales, value_scales, multipliers)
+        return found
+    p, reads, outs, copies = _norm_rope_params(q, keys, positions, frequencies, q_weight, key_weight, eps, offset, axes, interleaved,
+                                               magnitude, q_out, keys_out, True)
+    a, _held = _append_params(reads[1], None if values is None else _vectors(values), slots, key_pages, value_pages, kind, key_scales,
+                              value_scales, multipliers)
+    _launch_norm_rope(p, a, reads, copies, "crit_b200.norm_rope_write")
+    return outs[0]
 
 
 # -- gather and slots ---------------------------------------------------------------------------------------------------
-def gather(pages, kind, page, *, table=None, slots=None, count=None, scales=None, multiplier=1.0, dtype=torch.bfloat16):
-    """Rows of one page tensor ([pages][page][kv_heads][dim] or [slots][kv_heads][dim]) dequantised to `dtype`: the
-    first `count` positions of the page table `table` (int32), or the rows at `slots` (int64, any shape).
-    -> [count][kv_heads][dim] (or slots' shape + [kv_heads][dim]).  Reference: pages.py:455-493."""
+def gather(pages, kind, page, *, table=None, slots=None, count=None, scales=None, multiplier=1.0, dtype=torch.bfloat16, out=None):
+    """Rows of one page tensor ([pages][page][kv_heads][dim] or [slots][kv_heads][dim]; "int4": two elements a byte)
+    dequantised to `dtype`: the first `count` positions of the page table `table` (int32), or the rows at `slots` (int64,
+    any shape).  -> [count][kv_heads][dim] (or slots' shape + [kv_heads][dim]); into `out` (contiguous, of that size, its
+    type in dtype's place) when given.  Reference: pages.py:455-493."""
     _cuda(pages, "pages")
     k_kind = _check_kind(kind, scales)
-    hkv, dim = pages.shape[-2], pages.shape[-1]
+    hkv, dim = _check4(pages, scales, "rows") if k_kind == 5 else pages.shape[-2:]
     shape = None
     if slots is not None:
         shape, slots = tuple(slots.shape), slots.reshape(-1).contiguous()
         count = slots.numel()
     elif table is None or count is None:
         raise ValueError("gather reads a page table's first `count` positions, or rows at `slots`")
-    out = torch.empty((count, hkv, dim), dtype=dtype, device=pages.device)
+    if out is None:
+        out = torch.empty((count, hkv, dim), dtype=dtype, device=pages.device)
+    elif out.numel() != count * hkv * dim or not out.is_contiguous() or out.dtype not in _DTYPES or out.device != pages.device:
+        raise ValueError(f"gather's out is a contiguous bf16, fp16 or fp32 tensor of [{count}][{hkv}][{dim}] on the pages' device")
+    else:
+        dtype = out.dtype
+        out = out.view(count, hkv, dim)
     if count == 0:
         return out if shape is None else out.view(*shape, hkv, dim)
     p = _lib.GatherParams()
@@ -321,7 +491,7 @@ def gather(pages, kind, page, *, table=None, slots=None, count=None, scales=None
     p.slots = _ptr(slots)
     if not pages.is_contiguous():
         raise ValueError("pages are contiguous [slots][kv_heads][dim] storage")
-    p.slots_total = pages.numel() // (hkv * dim)
+    p.slots_total = pages.numel() // (hkv * pages.shape[-1])
     p.status = _ptr(_status_word(pages.device))
     p.count, p.kv_heads, p.dim, p.page = count, hkv, dim, int(page)
     p.kind, p.page_dtype, p.out_dtype = k_kind, _page_dtype(kind, pages), _DTYPES[dtype]
@@ -364,8 +534,6 @@ def move_rows(store, source, target):
     source, target = source.contiguous(), target.contiguous()
     layers, slots = store.shape[0], store.shape[1]
     row_bytes = store[0, 0].numel() * store.element_size()
-    if row_bytes % 4:
-        raise ValueError("a store's rows are a multiple of 4 bytes")
     p = _lib.MoveParams()
     p.store, p.source, p.target = _ptr(store), _ptr(source), _ptr(target)
     p.lists, p.width, p.slots, p.row_bytes, p.layers = source.shape[0], source.shape[1], slots, row_bytes, layers
@@ -453,6 +621,14 @@ def attend(q, key_pages, value_pages, kind, tables, rows, starts, firsts, column
     _cuda(q, "q")
     T, hq, d = q.shape
     hkv, dv = key_pages.shape[-2], value_pages.shape[-1]
+    if k_kind == 5:
+        if value_scales is None:
+            raise ValueError("int4 pages take scales beside their codes, keys and values alike")
+        if _check4(key_pages, key_scales, "keys") != (hkv, d) or _check4(value_pages, value_scales, "values") != (hkv, d):
+            raise ValueError(f"int4 pages hold keys and values of q's width, [...][kv_heads][{d // 2}]")
+        if key_pages.numel() != value_pages.numel() or key_pages.device != q.device or value_pages.device != q.device:
+            raise ValueError("int4 keys and values are as many pages each, on q's device")
+        dv = d
     R = int(starts.shape[0])
     if hq % hkv or not 1 <= columns <= MAX_COLUMNS or R == 0:
         raise ValueError("query heads a multiple of the KV heads, 1..64 columns a row, one row or more")
@@ -553,7 +729,7 @@ def attend(q, key_pages, value_pages, kind, tables, rows, starts, firsts, column
     p.q_heads, p.kv_heads, p.head_dim, p.value_dim, p.page = hq, hkv, d, dv, page
     p.kind, p.page_dtype, p.q_dtype = k_kind, _page_dtype(kind, key_pages), _DTYPES[q.dtype]
     p.chunk, p.max_splits = chunk, splits
-    p.slots = key_pages.numel() // (hkv * d)
+    p.slots = key_pages.numel() // (hkv * key_pages.shape[-1])
     if staging not in (None, "tma", "cp.async"):
         raise ValueError("staging is None, tma or cp.async")
     p.flags = ({None: 0, "cp.async": 1, "tma": 2}[staging] | (4 if persistent else 0) |
@@ -609,12 +785,51 @@ def merge_shards(outs, lses, dtype=None):
 
 def prefill_serves(head_dim, value_dim, q_dtype, kind, page):
     """Whether prefill() reads a cache of this geometry (else prompt rows go through attend in pieces)."""
-    widths = (64, 128, 256) if kind in ("bf16", "fp16") else (64, 128)        # 256-wide heads: 16-bit pages (m16n8k16 tiles)
+    widths = (64, 128, 256) if kind in ("bf16", "fp16", "int4") else (64, 128)        # 256-wide heads: 16-bit pages (m16n8k16 tiles)
     return head_dim == value_dim and head_dim in widths and page % TILE == 0 and kind in KINDS and \
         q_dtype in (torch.bfloat16, torch.float16)
 
 
 # -- prompt chunks ------------------------------------------------------------------------------------------------------
+def _expanded(p, q, key_pages, value_pages, key_scales, value_scales, table, position, tokens, longest, page, workspace):
+    """4-bit pages as 16-bit ones of q's type in the workspace, one launch, in the order of the sequences' tables: (keys,
+    values, the table that reads them)."""
+    hkv, d = key_pages.shape[-2], q.shape[-1]
+    if value_scales is None or _check4(key_pages, key_scales, "keys") != (hkv, d) or _check4(value_pages, value_scales, "values") != (hkv, d) or \
+            key_pages.numel() != value_pages.numel() or key_pages.device != q.device or value_pages.device != q.device:
+        raise ValueError(f"int4 pages hold keys and values of q's width, [...][kv_heads][{d // 2}] with their scales, on q's device")
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("q is bf16 or fp16")
+    several = table.dim() == 2
+    sequences, width = table.shape if several else (1, table.shape[0])
+    if longest is not None:
+        width = min(width, -(-longest // page))
+    pages = sequences * width
+    half = pages * page * hkv * d // 2                                 # floats of the keys, or the values
+    floats = 2 * half + pages
+    # (a workspace that a launch outgrew is kept: large ones grow by powers of two)
+    space = _workspace(q.device, floats if workspace is not None or floats < 1 << 24 else 1 << (floats - 1).bit_length(), workspace)
+    e = _lib.ExpandParams()
+    e.key_pages, e.value_pages, e.key_scales, e.value_scales = _ptr(key_pages), _ptr(value_pages), _ptr(key_scales), _ptr(value_scales)
+    e.tables, e.table_stride = _ptr(table), table.stride(0) if several else 0
+    if several:
+        e.positions, e.starts = p.positions, p.starts
+    elif torch.is_tensor(position):
+        e.positions = _ptr(position)
+    else:
+        e.position = int(position)
+    keys = space[:half].view(q.dtype).view(pages, page, hkv, d)
+    values = space[half:2 * half].view(q.dtype).view(pages, page, hkv, d)
+    found = space[2 * half:2 * half + pages].view(torch.int32).view(table.shape[:-1] + (width,))
+    e.out_keys, e.out_values, e.out_tables = _ptr(keys), _ptr(values), _ptr(found)
+    e.status, e.slots_total = _ptr(_status_word(q.device)), key_pages.numel() * 2 // (hkv * d)
+    e.sequences, e.width, e.tokens, e.kv_heads, e.dim, e.page = sequences, width, tokens, hkv, d, page
+    e.out_dtype = _DTYPES[q.dtype]
+    with torch.cuda.device(q.device):
+        _lib.check(_lib.load().crit_b200_expand(ctypes.byref(e), _stream(q.device)), "crit_b200.prefill")
+    return keys, values, found
+
+
 def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scales=None, value_scales=None,
             multipliers=(1.0, 1.0), scale=None, out=None, lse=None, int8_qk=False, fresh=None, flash=False,
             sinks=None, sliding=0, splits=None, workspace=None, derive=None, engine=None, starts=None):
@@ -626,13 +841,16 @@ def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scale
     (tcgen05.mma tiles with TMEM accumulators for 16-bit pages of 128-wide heads, m16n8k16 tiles otherwise), "mma.sync"
     or "tcgen05" (refused where not served); "tcgen05:single" / "tcgen05:pair" also name the block shape (128 query rows
     two blocks an SM / 256 rows over one ring of key and value tiles, which "tcgen05" picks by the launch's size).
+    "int4" pages are first made 16-bit ones of q's type in the workspace (exact: no second rounding), positions * kv_heads *
+    dim floats a sequence and a few, the workspace of `owner` or `workspace` (FP32) when given: run a launch of that size
+    once before capturing it.
     Reference: paged_kv_attention/__init__.py:1245-1332."""
     _refuse(int8_qk=int8_qk, fresh=fresh, sinks=sinks, sliding=sliding, derive=derive)
     k_kind = _check_kind(kind, key_scales)
     _cuda(q, "q")
     T, hq, d = q.shape
     hkv = key_pages.shape[-2]
-    if value_pages.shape[-1] != d:
+    if value_pages.shape[-1] * (2 if k_kind == 5 else 1) != d:
         raise ValueError("prompt chunks read keys and values of one width")
     if not key_pages.is_contiguous() or not value_pages.is_contiguous():
         raise ValueError("pages are contiguous [slots][kv_heads][dim] storage")
@@ -644,11 +862,13 @@ def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scale
     if q.stride(-1) != 1 or out.stride(-1) != 1:
         raise ValueError("q and out have contiguous last dimensions")
     p = _lib.PrefillParams()
+    longest = None if torch.is_tensor(position) or table.dim() == 2 else int(position) + T       # positions, where the host knows them
     if table.dim() == 2:             # several sequences, one launch
         S = table.shape[0]
         if not torch.is_tensor(position):
             if len(position) != S:
                 raise ValueError("one position a sequence")
+            longest = max((int(x) for x in position), default=0)
             position = torch.tensor([int(x) for x in position], dtype=torch.int64, device=q.device)
         if position.dtype != torch.int64 or position.numel() != S or not position.is_cuda or not position.is_contiguous():
             raise ValueError("the sequences' positions are an int64 tensor [S] on the device")
@@ -664,11 +884,19 @@ def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scale
             starts = torch.tensor(starts, dtype=torch.int32, device=q.device)
             p.starts = _ptr(starts)
         p.positions, p.sequences, p.table_stride = _ptr(position), S, table.stride(0)
-        T, position = most, 0
+        T, position, held = most, 0, position
+        longest = None if longest is None else longest + most
     elif starts is not None:
         raise ValueError("starts goes with a table of several sequences")
     if torch.is_tensor(position) and (position.dtype != torch.int64 or position.numel() != 1 or not position.is_cuda):
         raise ValueError("a position read on the device is a one-element int64 tensor there")
+    if k_kind == 5:
+        key_pages, value_pages, table = _expanded(p, q, key_pages, value_pages, key_scales, value_scales, table, position, T, longest, int(page),
+                                                  workspace)
+        kind = "fp16" if q.dtype == torch.float16 else "bf16"
+        k_kind, key_scales, value_scales = 0, None, None
+        if p.sequences:
+            p.table_stride = table.stride(0)
     p.q, p.out, p.lse = _ptr(q), _ptr(out), _ptr(lse)
     p.key_pages, p.value_pages = _ptr(key_pages), _ptr(value_pages)
     p.key_scales, p.value_scales = _ptr(key_scales), _ptr(value_scales)

@@ -5,9 +5,9 @@ from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int6
 from pathlib import Path
 
 LIBRARY = Path(__file__).resolve().parent / "_native" / "libcrit_b200.so"
-ABI_VERSION = 3
+ABI_VERSION = 4
 
-KIND_16BIT, KIND_FP8, KIND_FP8_ROW, KIND_INT8, KIND_FP8_PAGE = range(5)
+KIND_16BIT, KIND_FP8, KIND_FP8_ROW, KIND_INT8, KIND_FP8_PAGE, KIND_INT4 = range(6)
 DTYPE_BF16, DTYPE_FP16, DTYPE_FP32 = range(3)
 
 
@@ -85,8 +85,27 @@ class ExchangeParams(Structure):
                 ("floats", c_int64), ("wait_ns", c_int64), ("world", c_int32), ("rank", c_int32)]
 
 
+class ExpandParams(Structure):
+    _fields_ = [("key_pages", c_void_p), ("value_pages", c_void_p), ("key_scales", c_void_p), ("value_scales", c_void_p),
+                ("tables", c_void_p), ("positions", c_void_p), ("starts", c_void_p), ("out_keys", c_void_p), ("out_values", c_void_p),
+                ("out_tables", c_void_p), ("status", c_void_p), ("position", c_int64), ("slots_total", c_int64), ("table_stride", c_int64),
+                ("sequences", c_int32), ("width", c_int32), ("tokens", c_int32), ("kv_heads", c_int32), ("dim", c_int32),
+                ("page", c_int32), ("out_dtype", c_int32)]
+
+
+class NormRopeParams(Structure):
+    _fields_ = [("q", c_void_p), ("keys", c_void_p), ("q_out", c_void_p), ("keys_out", c_void_p), ("positions", c_void_p),
+                ("frequencies", c_void_p), ("axes", c_void_p), ("q_weight", c_void_p), ("key_weight", c_void_p), ("status", c_void_p),
+                ("tokens", c_int64), ("axis_stride", c_int64), ("q_stride_token", c_int64), ("q_stride_head", c_int64),
+                ("key_stride_token", c_int64), ("key_stride_head", c_int64), ("q_out_stride_token", c_int64), ("q_out_stride_head", c_int64),
+                ("key_out_stride_token", c_int64), ("key_out_stride_head", c_int64),
+                ("q_heads", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32), ("rotary", c_int32), ("n_axes", c_int32),
+                ("interleaved", c_int32), ("dtype", c_int32), ("weight_dtype", c_int32),
+                ("eps", c_float), ("offset", c_float), ("magnitude", c_float)]
+
+
 STRUCTS = (AppendParams, GatherParams, SlotsParams, AttendParams, MergeShardsParams, PrefillParams, ExchangeParams, MoveParams,
-           CompactParams)
+           CompactParams, ExpandParams, NormRopeParams)
 
 # name -> (restype, argtypes): every symbol include/crit_b200.h declares
 SYMBOLS = {
@@ -101,6 +120,8 @@ SYMBOLS = {
     "crit_b200_merge_shards": (c_int, [POINTER(MergeShardsParams), c_void_p]),
     "crit_b200_move_rows": (c_int, [POINTER(MoveParams), c_void_p]),
     "crit_b200_compact_blocks": (c_int, [POINTER(CompactParams), c_void_p]),
+    "crit_b200_expand": (c_int, [POINTER(ExpandParams), c_void_p]),
+    "crit_b200_norm_rope": (c_int, [POINTER(NormRopeParams), POINTER(AppendParams), c_void_p]),
     "crit_b200_prefill": (c_int, [POINTER(PrefillParams), c_void_p]),
     "crit_b200_shard_push": (c_int, [POINTER(ExchangeParams), c_void_p]),
     "crit_b200_shard_wait": (c_int, [POINTER(ExchangeParams), c_void_p]),

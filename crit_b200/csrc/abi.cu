@@ -14,6 +14,8 @@ extern "C" __attribute__((visibility("default"))) int crit_b200_params_size(int3
         case 6: return (int)sizeof(crit_b200_exchange_params);
         case 7: return (int)sizeof(crit_b200_move_params);
         case 8: return (int)sizeof(crit_b200_compact_params);
+        case 9: return (int)sizeof(crit_b200_expand_params);
+        case 10: return (int)sizeof(crit_b200_norm_rope_params);
         default: return CRIT_B200_EINVAL;
     }
 }
@@ -22,7 +24,7 @@ extern "C" __attribute__((visibility("default"))) const char* crit_b200_error(in
     switch (code) {
         case 0: return "success";
         case CRIT_B200_EINVAL: return "crit_b200: a size, stride or pointer the call cannot take";
-        case CRIT_B200_EUNSUPPORTED: return "crit_b200: no kernel was built for this geometry (head widths 64, 128 or 256 with keys and values of one width, pages of a multiple of 16 positions, page kinds bf16, fp16, fp8, fp8:row, int8, fp8:page)";
+        case CRIT_B200_EUNSUPPORTED: return "crit_b200: no kernel was built for this geometry (head widths 64, 128 or 256 with keys and values of one width, pages of a multiple of 16 positions, page kinds bf16, fp16, fp8, fp8:row, int8, fp8:page, int4)";
         case CRIT_B200_EWORKSPACE: return "crit_b200: the workspace is smaller than partial_rows * q_heads * max_splits * (value_dim + 2) floats";
         case CRIT_B200_EALIGN: return "crit_b200: q and pages are read in 16-byte vectors and outputs written in 8-byte ones: a pointer or stride is not aligned for that";
         case CRIT_B200_ESTATIC: return "crit_b200: crit_b200_attend_static holds 4,194,304 floats (16 MiB) of partials; this launch needs more (partial_rows * q_heads * max_splits * (value_dim + 2)): raise chunk or attend fewer rows a call";

@@ -5,7 +5,7 @@
 // inference/attention-state/code/pages.py:420-453, :872-895.
 #include <type_traits>
 
-#include "common.cuh"
+#include "int4.cuh"
 
 namespace crit_b200 {
 
@@ -194,6 +194,84 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) append_kernel(const crit_b2
     }
 }
 
+// Eight consecutive elements from src (16-byte loads where the address allows them).
+template <typename TIN>
+__device__ __forceinline__ void load8(const TIN* src, float (&x)[8]) {
+    if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+        if constexpr (sizeof(TIN) == 2) {
+            const uint4 v = *reinterpret_cast<const uint4*>(src);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float2 f;
+                if constexpr (std::is_same<TIN, __nv_bfloat16>::value) f = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+                else f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                x[2 * i] = f.x, x[2 * i + 1] = f.y;
+            }
+        } else {
+            const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
+            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_float<TIN>(src[i]);
+}
+
+// 4-bit rows.  Four lanes serve a group of 32 elements of one (token, kv head) of the keys or the values: 8 elements a
+// lane in one 16-byte load, the group's maximum by two shuffles, 8 codes in one 4-byte store.  Every byte is read and
+// written once; bound by HBM for prompt chunks, by the launch for decode steps.
+template <typename TIN>
+__global__ void __launch_bounds__(256) append4_kernel(const crit_b200_append_params p, const int per_head, const int key_groups,
+                                                      const int per_token) {
+    const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 2;         // a group; the last quads have none
+    const int part = threadIdx.x & 3;
+    const int64_t t = item / per_token;
+    int g = (int)(item - t * per_token);
+    const bool is_v = g >= key_groups;
+    if (is_v) g -= key_groups;
+    const int groups = is_v ? p.value_dim >> 5 : per_head;
+    const int h = g / groups;
+    g -= h * groups;
+    const int64_t slot = t < p.tokens ? p.slots[t] : -1;
+    const bool outside = slot >= 0 && p.slots_total && slot >= p.slots_total;    // skipped and reported, never written
+    if (outside && part == 0 && p.status) atomicExch(p.status, CRIT_B200_STATUS_BOUNDS);
+    const bool live = slot >= 0 && !outside;
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (live) {
+        const TIN* src = is_v ? (const TIN*)p.values + t * p.value_stride_token + (int64_t)h * p.value_stride_head
+                              : (const TIN*)p.keys + t * p.key_stride_token + (int64_t)h * p.key_stride_head;
+        load8<TIN>(src + g * 32 + part * 8, x);
+    }
+    uint32_t byte;
+    const uint32_t w = int4_quantise(x, byte);
+    if (!live) return;
+    const int64_t at = (slot * p.kv_heads + h) * groups + g;
+    reinterpret_cast<uint32_t*>(is_v ? p.value_pages : p.key_pages)[at * 4 + part] = w;
+    if (part == 0) reinterpret_cast<uint8_t*>(is_v ? p.value_scales : p.key_scales)[at] = (uint8_t)byte;
+}
+
+template <typename TIN>
+static void launch_append4(const crit_b200_append_params& p, cudaStream_t s) {
+    const int per_head = p.head_dim >> 5, key_groups = p.kv_heads * per_head;
+    const int per_token = key_groups + (p.values ? p.kv_heads * (p.value_dim >> 5) : 0);
+    const int64_t quads = p.tokens * per_token;
+    append4_kernel<TIN><<<(unsigned)((quads + 63) / 64), 256, 0, s>>>(p, per_head, key_groups, per_token);
+}
+
+int check_append(const crit_b200_append_params& p) {
+    if (p.tokens < 0 || !p.keys || !p.slots || !p.key_pages || p.kv_heads < 1 || p.page < 1) return CRIT_B200_EINVAL;
+    if (p.values && !p.value_pages) return CRIT_B200_EINVAL;
+    auto width_ok = [](int d) { return d >= 32 && d <= 256 && d % 32 == 0; };
+    if (!width_ok(p.head_dim) || (p.values && !width_ok(p.value_dim))) return CRIT_B200_EUNSUPPORTED;
+    if (p.kind < 0 || p.kind > CRIT_B200_KIND_INT4) return CRIT_B200_EUNSUPPORTED;
+    if (p.kind == CRIT_B200_KIND_INT4 && (!aligned(p.key_pages, 4) || (p.values && !aligned(p.value_pages, 4)))) return CRIT_B200_EALIGN;
+    if (p.kind >= CRIT_B200_KIND_FP8_ROW && (!p.key_scales || (p.values && !p.value_scales))) return CRIT_B200_EINVAL;
+    if (p.kind == CRIT_B200_KIND_16BIT && p.page_dtype == CRIT_B200_DTYPE_FP32 && p.in_dtype != CRIT_B200_DTYPE_FP32)
+        ;   // widening into FP32 pages is served too
+    return 0;
+}
+
 }  // namespace crit_b200
 
 using namespace crit_b200;
@@ -202,14 +280,17 @@ extern "C" __attribute__((visibility("default"))) int crit_b200_append(const cri
     if (!params) return CRIT_B200_EINVAL;
     const crit_b200_append_params p = *params;
     if (p.tokens == 0) return 0;
-    if (p.tokens < 0 || !p.keys || !p.slots || !p.key_pages || p.kv_heads < 1 || p.page < 1) return CRIT_B200_EINVAL;
-    if (p.values && !p.value_pages) return CRIT_B200_EINVAL;
-    auto width_ok = [](int d) { return d >= 32 && d <= 256 && d % 32 == 0; };
-    if (!width_ok(p.head_dim) || (p.values && !width_ok(p.value_dim))) return CRIT_B200_EUNSUPPORTED;
-    if (p.kind < 0 || p.kind > CRIT_B200_KIND_FP8_PAGE) return CRIT_B200_EUNSUPPORTED;
-    if (p.kind >= CRIT_B200_KIND_FP8_ROW && (!p.key_scales || (p.values && !p.value_scales))) return CRIT_B200_EINVAL;
-    if (p.kind == CRIT_B200_KIND_16BIT && p.page_dtype == CRIT_B200_DTYPE_FP32 && p.in_dtype != CRIT_B200_DTYPE_FP32)
-        ;   // widening into FP32 pages is served too
+    if (int e = check_append(p)) return e;
+    if (p.kind == CRIT_B200_KIND_INT4) {
+        switch (p.in_dtype) {
+            case CRIT_B200_DTYPE_BF16: launch_append4<__nv_bfloat16>(p, (cudaStream_t)stream); break;
+            case CRIT_B200_DTYPE_FP16: launch_append4<__half>(p, (cudaStream_t)stream); break;
+            case CRIT_B200_DTYPE_FP32: launch_append4<float>(p, (cudaStream_t)stream); break;
+            default: return CRIT_B200_EINVAL;
+        }
+        CRIT_CHECK_LAUNCH();
+        return 0;
+    }
     const int heads_total = p.values ? 2 * p.kv_heads : p.kv_heads;
     const int64_t items = p.tokens * heads_total;
     const unsigned grid = (unsigned)((items + APPEND_WARPS - 1) / APPEND_WARPS);

@@ -15,6 +15,9 @@ namespace crit_b200 {
 
 constexpr int MERGE_WARPS = 8;
 
+int launch_decode4(const crit_b200_attend_params& p, cudaStream_t s);                                   // decode4.cu
+int plan_decode4(int q_heads, int kv_heads, int d, int columns, int32_t* out5);
+
 // States a row of L positions has in the workspace: one a split, or two (a split's head and tail; m = -inf marks one
 // that holds nothing, and the folds pass it over) after a launch that deals tiles out evenly.
 // A sink logit (natural units of the scaled scores) joins a folded state (top in base-2 units, total relative to it):
@@ -468,7 +471,7 @@ static int check(const crit_b200_attend_params& p) {
         return CRIT_B200_EINVAL;
     if (p.page < 16 || p.page % 16) return CRIT_B200_EUNSUPPORTED;
     if (p.chunk < 16 || p.chunk % 16 || p.max_splits < 1) return CRIT_B200_EINVAL;
-    if (scale_mode(p.kind) && (!p.key_scales || !p.value_scales)) return CRIT_B200_EINVAL;
+    if ((scale_mode(p.kind) || p.kind == CRIT_B200_KIND_INT4) && (!p.key_scales || !p.value_scales)) return CRIT_B200_EINVAL;
     if (p.q_dtype != CRIT_B200_DTYPE_BF16 && p.q_dtype != CRIT_B200_DTYPE_FP16) return CRIT_B200_EUNSUPPORTED;
     if (p.kind == CRIT_B200_KIND_16BIT && p.page_dtype != p.q_dtype) return CRIT_B200_EUNSUPPORTED;
     if (!aligned(p.q, 16) || p.q_stride_token % 8 || p.q_stride_head % 8 || !aligned(p.key_pages, 16) ||
@@ -592,6 +595,7 @@ static int launch_decode_ph(const crit_b200_attend_params& p, cudaStream_t s) {
 }
 
 static int launch_decode(const crit_b200_attend_params& p, cudaStream_t s) {
+    if (p.kind == CRIT_B200_KIND_INT4) return launch_decode4(p, s);
     // draft trees (parents), sliding windows, sinks and block lists are the m16n8k16 kernel's only
     if ((p.parents || p.sinks || p.sliding > 0 || p.blocks || (p.flags & CRIT_B200_ATTEND_CONTEXT)) && (p.flags & (CRIT_B200_ATTEND_TCGEN05P | CRIT_B200_ATTEND_TCGEN05T | CRIT_B200_ATTEND_TCGEN05))) return CRIT_B200_EUNSUPPORTED;
     if (p.flags & CRIT_B200_ATTEND_TCGEN05P) return ph_serves(p) ? launch_decode_ph(p, s) : CRIT_B200_EUNSUPPORTED;
@@ -772,6 +776,7 @@ extern "C" __attribute__((visibility("default"))) int crit_b200_attend_plan(int3
                                                                             int32_t page_dtype, int32_t columns, int32_t* out5) {
     if (!out5 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || columns < 1) return CRIT_B200_EINVAL;
     if (page < 16 || page % 16) return CRIT_B200_EUNSUPPORTED;
+    if (kind == CRIT_B200_KIND_INT4) return head_dim == value_dim ? plan_decode4(q_heads, kv_heads, head_dim, columns, out5) : CRIT_B200_EUNSUPPORTED;
     const int rows = columns * (q_heads / kv_heads);
     const int nt = row_tiles(rows, value_dim);
     Variant v;

@@ -1,5 +1,7 @@
 // Block-table page gather with dequantisation, slot mapping on the device, and the merge of shards' partials.
-#include "common.cuh"
+#include <type_traits>
+
+#include "int4.cuh"
 
 namespace crit_b200 {
 
@@ -37,6 +39,71 @@ __global__ void __launch_bounds__(128) gather_kernel(const crit_b200_gather_para
             v = __fmul_rn(e4m3_to_float(((const uint8_t*)p.pages)[row * p.dim + i]), scale);
         }
         dst[i] = from_float<TOUT>(v);
+    }
+}
+
+// 4-bit rows back: a thread takes 8 codes (one 4-byte load) to 8 values, (code - 8) * scale in FP32 (exact), in one 16-byte
+// store for 16-bit types.  Bound by the bytes it writes.
+template <typename TOUT>
+__global__ void __launch_bounds__(256) gather4_kernel(const crit_b200_gather_params p, const int words) {
+    const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;                // a word of 8 codes; words: those of one position
+    if (item >= p.count * words) return;
+    const int64_t n = item / words;
+    const int w = (int)(item - n * words);
+    const int64_t slot = p.slots ? p.slots[n] : (int64_t)p.table[n / p.page] * p.page + n % p.page;
+    float v[8];
+    if (p.slots_total && (slot < 0 || slot >= p.slots_total)) {      // outside the page tensor: zeros, and reported
+        if (w == 0 && p.status) atomicExch(p.status, CRIT_B200_STATUS_BOUNDS);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    } else {
+        const int64_t at = slot * words + w;
+        const uint32_t codes = reinterpret_cast<const uint32_t*>(p.pages)[at];
+        const float s = int4_scale(reinterpret_cast<const uint8_t*>(p.scales)[at >> 2]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __fmul_rn((float)((int)((codes >> (4 * i)) & 15u) - 8), s);
+    }
+    TOUT* dst = (TOUT*)p.out + item * 8;
+    if constexpr (sizeof(TOUT) == 2) {
+        constexpr bool BF16 = std::is_same<TOUT, __nv_bfloat16>::value;
+        *reinterpret_cast<uint4*>(dst) = make_uint4(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]), pack2<BF16>(v[4], v[5]), pack2<BF16>(v[6], v[7]));
+    } else {
+        *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    }
+}
+
+// The sequences' 4-bit pages as 16-bit ones, in the order of their tables: block = (page of the table, sequence, keys or
+// values).  A page past the sequence's last position is left out.  Bound by the bytes it writes.
+template <bool BF16>
+__global__ void __launch_bounds__(256) expand4_kernel(const crit_b200_expand_params p, const int words) {
+    const int j = blockIdx.x, s = blockIdx.y, is_v = blockIdx.z;
+    const int tokens = p.starts ? p.starts[s + 1] - p.starts[s] : p.tokens;
+    const int64_t length = (p.positions ? p.positions[s] : p.position) + tokens;
+    const int64_t to = (int64_t)s * p.width + j;
+    if (!is_v && threadIdx.x == 0) p.out_tables[to] = (int32_t)to;
+    if ((int64_t)j * p.page >= length) return;
+    const uint32_t pages_total = (uint32_t)(p.slots_total / p.page);
+    uint32_t pg = (uint32_t)p.tables[(int64_t)s * p.table_stride + j];
+    if (pg >= pages_total) {                       // outside the page tensor: its last page instead, and reported
+        if (threadIdx.x == 0 && p.status) atomicExch(p.status, CRIT_B200_STATUS_BOUNDS);
+        pg = pages_total - 1;
+    }
+    const uint32_t* codes = reinterpret_cast<const uint32_t*>(is_v ? p.value_pages : p.key_pages) + (int64_t)pg * words;
+    const uint8_t* scales = reinterpret_cast<const uint8_t*>(is_v ? p.value_scales : p.key_scales) + (int64_t)pg * (words >> 2);
+    uint4* out = reinterpret_cast<uint4*>(is_v ? p.out_values : p.out_keys) + to * words;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < words; i += 256) {
+        const uint32_t w = codes[i];
+        const float f = int4_scale(scales[i >> 2]);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = __fmul_rn((float)((int)((w >> (4 * e)) & 15u) - 8), f);
+        if constexpr (!BF16) {                     // (a scale above FP16's range over 7: its largest number, not infinity)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = v[e] > 65504.f ? 65504.f : (v[e] < -65504.f ? -65504.f : v[e]);
+        }
+        out[i] = make_uint4(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]), pack2<BF16>(v[4], v[5]), pack2<BF16>(v[6], v[7]));
     }
 }
 
@@ -91,6 +158,21 @@ extern "C" __attribute__((visibility("default"))) int crit_b200_gather(const cri
     if (p.count < 0 || !p.pages || !p.out || (!p.table && !p.slots) || p.kv_heads < 1 || p.dim < 1 || p.page < 1)
         return CRIT_B200_EINVAL;
     if (p.kind >= CRIT_B200_KIND_FP8_ROW && !p.scales) return CRIT_B200_EINVAL;
+    if (p.kind > CRIT_B200_KIND_INT4) return CRIT_B200_EUNSUPPORTED;
+    if (p.kind == CRIT_B200_KIND_INT4) {
+        if (p.dim % 32) return CRIT_B200_EUNSUPPORTED;
+        if (!aligned(p.pages, 4) || !aligned(p.out, 16)) return CRIT_B200_EALIGN;
+        const int words = p.kv_heads * (p.dim >> 3);
+        const unsigned blocks = (unsigned)((p.count * words + 255) / 256);
+        switch (p.out_dtype) {
+            case CRIT_B200_DTYPE_BF16: gather4_kernel<__nv_bfloat16><<<blocks, 256, 0, (cudaStream_t)stream>>>(p, words); break;
+            case CRIT_B200_DTYPE_FP16: gather4_kernel<__half><<<blocks, 256, 0, (cudaStream_t)stream>>>(p, words); break;
+            case CRIT_B200_DTYPE_FP32: gather4_kernel<float><<<blocks, 256, 0, (cudaStream_t)stream>>>(p, words); break;
+            default: return CRIT_B200_EINVAL;
+        }
+        CRIT_CHECK_LAUNCH();
+        return 0;
+    }
     const unsigned grid = (unsigned)((p.count * p.kv_heads + 3) / 4);
     cudaStream_t s = (cudaStream_t)stream;
     switch (p.out_dtype) {
@@ -118,9 +200,15 @@ __global__ void __launch_bounds__(128) move_rows_kernel(const crit_b200_move_par
             if (threadIdx.x == 0 && p.status) atomicExch(p.status, CRIT_B200_STATUS_BOUNDS);
             continue;
         }
-        const uint32_t* src = base + from * words;
-        uint32_t* dst = base + to * words;
-        for (int64_t w = threadIdx.x; w < words; w += blockDim.x) dst[w] = src[w];
+        if (p.row_bytes & 3) {
+            const char* src = (const char*)base + from * p.row_bytes;
+            char* dst = (char*)base + to * p.row_bytes;
+            for (int64_t b = threadIdx.x; b < p.row_bytes; b += blockDim.x) dst[b] = src[b];
+        } else {
+            const uint32_t* src = base + from * words;
+            uint32_t* dst = base + to * words;
+            for (int64_t w = threadIdx.x; w < words; w += blockDim.x) dst[w] = src[w];
+        }
         __syncthreads();                                     // the next move of the list may read this one's target
     }
 }
@@ -192,6 +280,26 @@ __global__ void __launch_bounds__(128) compact_blocks_kernel(const crit_b200_com
 
 }  // namespace crit_b200
 
+extern "C" __attribute__((visibility("default"))) int crit_b200_expand(const crit_b200_expand_params* params, void* stream) {
+    if (!params) return CRIT_B200_EINVAL;
+    const crit_b200_expand_params p = *params;
+    if (p.sequences == 0 || p.width == 0) return 0;
+    if (!p.key_pages || !p.value_pages || !p.key_scales || !p.value_scales || !p.tables || !p.out_keys || !p.out_values || !p.out_tables ||
+        p.sequences < 0 || p.sequences > 65535 || p.width < 0 || p.tokens < 0 || p.kv_heads < 1 || p.page < 1 || p.slots_total < p.page ||
+        (p.sequences > 1 && !p.positions) || p.position < 0 || (int64_t)p.sequences * p.width > 0x7fffffffLL)
+        return CRIT_B200_EINVAL;
+    if (p.dim < 32 || p.dim % 32 || (p.out_dtype != CRIT_B200_DTYPE_BF16 && p.out_dtype != CRIT_B200_DTYPE_FP16) ||
+        (int64_t)p.page * p.kv_heads * (p.dim >> 3) > 0x7fffffffLL)
+        return CRIT_B200_EUNSUPPORTED;
+    if (!aligned(p.key_pages, 4) || !aligned(p.value_pages, 4) || !aligned(p.out_keys, 16) || !aligned(p.out_values, 16)) return CRIT_B200_EALIGN;
+    const int words = p.page * p.kv_heads * (p.dim >> 3);
+    const dim3 grid((unsigned)p.width, (unsigned)p.sequences, 2);
+    if (p.out_dtype == CRIT_B200_DTYPE_BF16) crit_b200::expand4_kernel<true><<<grid, 256, 0, (cudaStream_t)stream>>>(p, words);
+    else crit_b200::expand4_kernel<false><<<grid, 256, 0, (cudaStream_t)stream>>>(p, words);
+    CRIT_CHECK_LAUNCH();
+    return 0;
+}
+
 extern "C" __attribute__((visibility("default"))) int crit_b200_compact_blocks(const crit_b200_compact_params* params, void* stream) {
     if (!params) return CRIT_B200_EINVAL;
     const crit_b200_compact_params p = *params;
@@ -211,8 +319,8 @@ extern "C" __attribute__((visibility("default"))) int crit_b200_move_rows(const 
     if (!params) return CRIT_B200_EINVAL;
     const crit_b200_move_params p = *params;
     if (p.lists == 0 || p.width == 0) return 0;
-    if (!p.store || !p.source || !p.target || p.lists < 0 || p.width < 0 || p.slots < 1 || p.layers < 1 || p.row_bytes < 4 ||
-        p.row_bytes % 4 || p.lists > 0x7fffffffLL || p.layers > 65535)
+    if (!p.store || !p.source || !p.target || p.lists < 0 || p.width < 0 || p.slots < 1 || p.layers < 1 || p.row_bytes < 1 ||
+        (p.row_bytes % 4 == 0 && !aligned(p.store, 4)) || p.lists > 0x7fffffffLL || p.layers > 65535)
         return CRIT_B200_EINVAL;
     dim3 grid((unsigned)p.lists, (unsigned)p.layers);
     crit_b200::move_rows_kernel<<<grid, 128, 0, (cudaStream_t)stream>>>(p);

@@ -14,7 +14,9 @@ What is built for the GPU instead of translated:
     rebuilds or re-uploads padded page tables, and host work is O(rows + new pages), not O(tokens).
   - writes, gathers and row reads go through the CUDA kernels of crit_b200 (there is no torch fallback: a pool on the
     CPU keeps page tables and slot maps only, for host-side tests).
-  - "fp8:page": E4M3 pages with one FP32 scale per (page, kv head), scales [layers][pages + 1][kv_heads].
+  - "fp8:page": E4M3 pages with one FP32 scale per (page, kv head), scales [layers][pages + 1][kv_heads];
+  - "int4": 4-bit codes, two a byte, keys [layers][pages + 1][page][kv_heads][dim / 2] uint8, with a byte of scale for each
+    32 elements, scales [layers][pages + 1][page][kv_heads][dim / 32] (crit_b200's module text has the format).
 
 Not served (the reference's other pool features): sliding rings, lending and elastic backing.
 """
@@ -22,11 +24,11 @@ import ctypes
 import heapq
 import math
 
-DTYPES = ("bf16", "fp16", "fp8", "fp8:row", "int8", "fp8:page")
+DTYPES = ("bf16", "fp16", "fp8", "fp8:row", "int8", "fp8:page", "int4")
 ROW_SCALED = ("fp8:row", "int8")
-SCALED = ROW_SCALED + ("fp8:page",)
+SCALED = ROW_SCALED + ("fp8:page", "int4")
 KERNEL_KINDS = DTYPES
-QUANTIZED = ("fp8", "fp8:row", "int8", "fp8:page")
+QUANTIZED = ("fp8", "fp8:row", "int8", "fp8:page", "int4")
 
 
 class _Tables:
@@ -131,19 +133,24 @@ class KVPool:
         self.kv_heads, self.head_dim = kv_heads, head_dim
         self.value_dim = head_dim if value_dim is None else int(value_dim)
         self.page, self.device, self.dtype = page, torch.device(device), dtype
-        self.storage = {"bf16": torch.bfloat16, "fp16": torch.float16, "int8": torch.int8}.get(dtype, torch.float8_e4m3fn)
+        self.storage = {"bf16": torch.bfloat16, "fp16": torch.float16, "int8": torch.int8, "int4": torch.uint8}.get(dtype, torch.float8_e4m3fn)
+        if dtype == "int4" and (head_dim % 32 or self.value_dim % 32):
+            raise ValueError(f"int4 pages hold heads of a multiple of 32 elements, not {head_dim} and {self.value_dim}")
+        packed = 2 if dtype == "int4" else 1                # elements a stored one holds
         self.compute = torch.float16 if dtype == "fp16" else torch.bfloat16
         self.pages = math.ceil(tokens / page)
         self.sliding, self.ring = 0, 0
         self.table_pages = max(math.ceil(int(positions) / page) if positions else self.pages, self.pages)
         n, stored = len(self.layers), self.pages + 1
         self.dump, self.stored_slots = self.pages, stored * page
-        shapes = [((n, stored, page, kv_heads, head_dim), self.storage),
-                  ((n, stored, page, kv_heads, self.value_dim), self.storage)]
+        shapes = [((n, stored, page, kv_heads, head_dim // packed), self.storage),
+                  ((n, stored, page, kv_heads, self.value_dim // packed), self.storage)]
         if dtype in ROW_SCALED:
             shapes += [((n, stored, page, kv_heads), torch.float32)] * 2
         elif dtype == "fp8:page":
             shapes += [((n, stored, kv_heads), torch.float32)] * 2
+        elif dtype == "int4":
+            shapes += [((n, stored, page, kv_heads, dim // 32), torch.uint8) for dim in (head_dim, self.value_dim)]
         offsets, sizes, end = [], [], 0
         for shape, kind in shapes:
             offsets.append(end)
@@ -413,6 +420,28 @@ class KVPool:
                            self.v[i] if self.value_dim else None, self.dtype, self.k_scales[i] if scaled else None,
                            self.v_scales[i] if scaled and self.value_dim else None, multipliers=self.scale_values[i])
 
+    def norm_rope_write(self, layer, slots, queries, keys, values, positions, frequencies, **rotation):
+        """A step's queries and keys normed and turned, and the keys and values stored at their slots, in one launch
+        (crit_b200.norm_rope_write, whose keyword arguments these are) -> the queries.  A prompt step of a pool with a
+        fresh buffer keeps the turned keys and the values there, as write() does."""
+        self._on_gpu("norm_rope_write")
+        i, tokens = self.layers[layer], keys.shape[0]
+        scaled = self.dtype in SCALED
+        fresh = self.fresh_k is not None and self._staging and tokens <= self.fresh_tokens
+        turned = None
+        if fresh:
+            turned = self.fresh_k[:tokens] if keys.dtype == self.compute else keys.new_empty(keys.shape)
+        found = self.kernels.norm_rope_write(queries, keys, values if self.value_dim else None, positions, frequencies, slots, self.k[i],
+                                             self.v[i] if self.value_dim else None, self.dtype, self.k_scales[i] if scaled else None,
+                                             self.v_scales[i] if scaled and self.value_dim else None, multipliers=self.scale_values[i],
+                                             keys_out=turned, **rotation)
+        if fresh:
+            if keys.dtype != self.compute:
+                self.fresh_k[:tokens].copy_(turned)
+            self.fresh_v[:tokens].copy_(values)
+            self._fresh_buffer.tag = (id(self), layer, tokens, self._reserves)
+        return found
+
     def gather(self, layer, sequence, count):
         """The sequence's first `count` positions of a layer: keys [count][kv_heads][head_dim] and values, in the
         compute dtype (dequantised).  Reference: pages.py:455-477."""
@@ -584,11 +613,10 @@ class KVPool:
         source = self.slots_at(slot, torch.where(keep, start[:, None] + path.long(), -1))
         target = self.slots_at(slot, torch.where(keep, start[:, None] + columns[None, :], -1))
         n, held = len(self.layers), self.stored_slots
-        stores = [self.k.view(n, held, self.kv_heads, self.head_dim)]
-        if self.value_dim:
-            stores.append(self.v.view(n, held, self.kv_heads, self.value_dim))
+        stores = [self.k, self.v] if self.value_dim else [self.k]
         if self.k_scales is not None:
-            stores += [scales.view(n, held, self.kv_heads) for scales in (self.k_scales, self.v_scales)]
+            stores += [self.k_scales, self.v_scales] if self.value_dim else [self.k_scales]
+        stores = [store.view(n, held, -1) for store in stores]
         if self.device.type != "cuda":
             raise RuntimeError("a draft tree's accepted path is moved by the CUDA kernels: this pool is on the CPU "
                                "(page tables and slot maps only)")

@@ -21,7 +21,7 @@
 extern "C" {
 #endif
 
-#define CRIT_B200_ABI_VERSION 3
+#define CRIT_B200_ABI_VERSION 4
 
 /* Page kinds (the reference's KINDS, paged_kv_attention/__init__.py:78, plus the per-page FP8 scale). */
 #define CRIT_B200_KIND_16BIT    0   /* bf16 or fp16 pages (page_dtype says which) */
@@ -29,6 +29,10 @@ extern "C" {
 #define CRIT_B200_KIND_FP8_ROW  2   /* E4M3 codes, FP32 scale per (slot, kv head): scales [slots][kv_heads] */
 #define CRIT_B200_KIND_INT8     3   /* INT8 codes, FP32 scale per (slot, kv head) */
 #define CRIT_B200_KIND_FP8_PAGE 4   /* E4M3 codes, FP32 scale per (page, kv head): scales [pages][kv_heads] */
+#define CRIT_B200_KIND_INT4     5   /* 4-bit codes, two a byte (element 2 i in the low half of byte i): a row of a kv head is dim / 2
+                                       bytes; scales [slots][kv_heads][dim / 32] BYTES (not floats, whatever the pointer's type),
+                                       one a group of 32 elements: bits 14..7 of an FP16 number.  A code stands for (code - 8) x
+                                       the scale.  Extension of this library */
 
 #define CRIT_B200_DTYPE_BF16 0
 #define CRIT_B200_DTYPE_FP16 1
@@ -61,7 +65,7 @@ typedef struct crit_b200_append_params {
     const int64_t* slots;
     void* key_pages;
     void* value_pages;
-    float* key_scales;           /* kinds 2, 3: [slots][kv_heads]; kind 4: [pages][kv_heads]; else NULL */
+    float* key_scales;           /* kinds 2, 3: [slots][kv_heads]; kind 4: [pages][kv_heads]; kind 5: bytes; else NULL */
     float* value_scales;
     int32_t* status;             /* or NULL: set to CRIT_B200_STATUS_BOUNDS when a slot lay outside [0, slots_total) */
     int64_t tokens;
@@ -95,6 +99,59 @@ typedef struct crit_b200_gather_params {
 
 int crit_b200_gather(const crit_b200_gather_params* params, void* stream);
 
+/* 4-bit pages (kind 5) as 16-bit ones: page j of each sequence's table goes to page s * width + j of out_keys and out_values
+ * (bf16 or FP16; every value is exact there, FP16 up to its range), as far as the sequence's positions go (its first new
+ * position + its tokens); out_tables gets the page ids s * width + j, the table that reads them.  What crit_b200_prefill
+ * reads a 4-bit cache through: its chunks read every page once a 256 query rows, so one pass over the codes costs little
+ * and the tcgen05 tiles take the values without a second rounding. */
+typedef struct crit_b200_expand_params {
+    const void* key_pages;       /* kind 5 */
+    const void* value_pages;
+    const void* key_scales;      /* bytes */
+    const void* value_scales;
+    const int32_t* tables;       /* [sequences][table_stride] page ids */
+    const int64_t* positions;    /* [sequences] on the device, or NULL: `position` (one sequence) */
+    const int32_t* starts;       /* [sequences + 1] on the device, or NULL: `tokens` a sequence */
+    void* out_keys;              /* [sequences * width][page][kv_heads][dim] 16-bit */
+    void* out_values;
+    int32_t* out_tables;         /* [sequences][width] */
+    int32_t* status;             /* or NULL: CRIT_B200_STATUS_BOUNDS for a page id outside the page tensors */
+    int64_t position;
+    int64_t slots_total;         /* slots each page tensor stores */
+    int64_t table_stride;
+    int32_t sequences, width, tokens, kv_heads, dim, page, out_dtype;
+} crit_b200_expand_params;
+
+int crit_b200_expand(const crit_b200_expand_params* params, void* stream);
+
+/* -- norm and rotation of queries and keys, with the append ------------------------------------------------------------
+ * The step between a model's projections and crit_b200_append (the reference's models run it as torch operations: "qkv
+ * projection, norm, rope, pool.write").  Each head of q and keys: y = x / sqrt(mean x^2 + eps) * (offset + weight) where a
+ * weight is given, then the first `rotary` elements turned in pairs, (a, b) -> magnitude * (a cos - b sin, b cos + a sin),
+ * pairs (i, rotary / 2 + i), or (2 i, 2 i + 1) with `interleaved`, by the angle positions[axes[i]][token] * frequencies[i]
+ * (made in FP64).  Results are rounded once; q_out may be q and keys_out may be keys.  With `append`, the normed and turned
+ * keys (from their FP32 values) and append->values go to their pages in the same launch, as crit_b200_append encodes them:
+ * every kind but 4 (CRIT_B200_EUNSUPPORTED: two calls), append->keys and its strides are not read. */
+typedef struct crit_b200_norm_rope_params {
+    const void* q;               /* [tokens][q_heads][head_dim], or NULL with q_heads 0 */
+    const void* keys;            /* [tokens][kv_heads][head_dim], or NULL with kv_heads 0 */
+    void* q_out;
+    void* keys_out;              /* or NULL with append */
+    const int64_t* positions;    /* [n_axes][axis_stride] */
+    const float* frequencies;    /* [rotary / 2] */
+    const int32_t* axes;         /* [rotary / 2]: the axis a pair turns with; or NULL: n_axes is 1 */
+    const void* q_weight;        /* [head_dim], or NULL: no norm */
+    const void* key_weight;
+    int32_t* status;             /* or NULL: CRIT_B200_STATUS_BOUNDS for an axis outside [0, n_axes) (the pair becomes zeros) */
+    int64_t tokens, axis_stride;
+    int64_t q_stride_token, q_stride_head, key_stride_token, key_stride_head;
+    int64_t q_out_stride_token, q_out_stride_head, key_out_stride_token, key_out_stride_head;
+    int32_t q_heads, kv_heads, head_dim, rotary, n_axes, interleaved, dtype, weight_dtype;
+    float eps, offset, magnitude;
+} crit_b200_norm_rope_params;
+
+int crit_b200_norm_rope(const crit_b200_norm_rope_params* params, const crit_b200_append_params* append, void* stream);
+
 /* -- slot mapping on the device ----------------------------------------------------------------------------------
  * Replaces KVPool._slots_at (pages.py:653-660) and the per-token host arithmetic of KVPool.reserve (:347, :721-722):
  * slot = tables[row[i]][clamp(p / page)] * page + p % page; with `capacity` (one per table row) a position outside
@@ -122,7 +179,7 @@ typedef struct crit_b200_move_params {
     const int64_t* source;       /* [lists][width] slots */
     const int64_t* target;       /* [lists][width] slots */
     int64_t lists, width, slots; /* slots: rows a layer holds (a slot outside [0, slots) is skipped and reported) */
-    int64_t row_bytes;           /* a multiple of 4 */
+    int64_t row_bytes;           /* (rows of a multiple of 4 bytes move by the word, others byte by byte) */
     int32_t layers;
     int32_t* status;             /* optional device word: CRIT_B200_STATUS_BOUNDS */
 } crit_b200_move_params;
@@ -392,7 +449,8 @@ int64_t crit_b200_pager_grow(void* pager, int32_t rows, const int32_t* have, con
 /* -- housekeeping ------------------------------------------------------------------------------------------------ */
 int crit_b200_abi_version(void);
 /* sizeof of each parameter block, in the order append, gather, slots, attend, merge_shards, prefill: a binding checks
- * its own struct layout against it (the reference's crit_cw_params_size, cuda_window.cu:1495-1497); 6 exchange, 7 move, 8 compact. */
+ * its own struct layout against it (the reference's crit_cw_params_size, cuda_window.cu:1495-1497); 6 exchange, 7 move, 8 compact,
+ * 9 expand, 10 norm_rope. */
 int crit_b200_params_size(int32_t which);
 const char* crit_b200_error(int32_t code);       /* host string; cudaGetErrorString for codes above 0 */
 int crit_b200_device_sms(void);                  /* SMs of the current device, or a negative error */
