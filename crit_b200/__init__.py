@@ -184,16 +184,20 @@ def tcgen05p_serves(kind, head_dim, value_dim, heads, kv_heads, columns, chunk, 
 # Launches below this many positions (window rows x the positions their tables hold) stay on the m16n8k16 kernel: the
 # whole-page-rows kernel deals whole splits to its blocks, and a small launch has too few to fill the device.
 PAGE_ROWS_FROM = 1 << 16
+EVEN_ROWS = 256             # window rows an even launch takes (decode4.cu, D4_MAX_ROWS)
 
 
 def engine_for(kind, head_dim, value_dim, heads, kv_heads, columns, rows=1, positions=None, engine=None):
     """The kernel a launch runs on: `engine` when one is named, else attend's own choice: "tcgen05p" (whole page rows:
     every kv head of a position in one contiguous read) for E4M3 pages of 8 kv heads x 128 with at most 8 query rows a
     kv head, when the launch is large enough to fill the device that way; "tcgen05" for other windows of several
-    columns over E4M3 pages of 128-wide heads; "mma.sync" (m16n8k16) for everything else.  Only the last gives a column
-    the same bits alone and in any window or batch."""
+    columns over E4M3 pages of 128-wide heads; "even" for int4 pages, up to 256 window rows (the m16n8k16 kernel of 4-bit
+    pages with the launch's positions dealt out evenly to the device's blocks, not cut into splits); "mma.sync" (m16n8k16)
+    for everything else.  Only the last gives a column the same bits alone and in any window or batch."""
     if engine is not None:
         return engine
+    if kind == "int4":
+        return "even" if rows <= EVEN_ROWS else "mma.sync"
     if tcgen05p_serves(kind, head_dim, value_dim, heads, kv_heads, columns, DEFAULT_CHUNK, rows) and \
             positions is not None and rows * positions >= PAGE_ROWS_FROM:
         return "tcgen05p"
@@ -607,14 +611,18 @@ def attend(q, key_pages, value_pages, kind, tables, rows, starts, firsts, column
     (TMA wherever the geometry allows it) or "cp.async" (never TMA); the same bits either way.  persistent: a fixed
     number of blocks walk a work list built on the device from the rows' lengths, instead of one block per (split, kv
     head, row) of a 3-D grid (the same bits; measured slower on the bench workloads, hence off).  engine: None (the
-    library's choice), "mma.sync" (the m16n8k16 kernel) or "tcgen05" (E4M3 page bytes straight into tcgen05.mma: E4M3
+    library's choice), "mma.sync" (the m16n8k16 kernel), "even" (int4 pages: no splits, the launch's positions dealt out
+    evenly; the choice for them where the caller names no chunk, partitions or workspace) or "tcgen05" (E4M3 page bytes straight into tcgen05.mma: E4M3
     pages of 128-wide heads, columns x group heads <= 32, chunk a multiple of 128; refused elsewhere).
     shards: a crit_b200.dist.ShardMerge: these pages hold one KV range of a context sharded over the ranks; every
     split state stays in the workspace, the fold of this rank's splits is stored into every rank's exchange buffer and
     out / lse get the merge over all ranks (three launches: decode, fold + push, wait + merge)."""
     _refuse(fresh=fresh, derive=derive)
+    # masks are served by the m16n8k16 kernels: of 4-bit pages under either engine, else "mma.sync"
+    plain = (None, "mma.sync", "even") if kind == "int4" else (None, "mma.sync")
+    masked = engine if kind == "int4" else "mma.sync"
     if context and (parents is not None or blocks is not None or sinks is not None or sliding or shards is not None or
-                    engine not in (None, "mma.sync")):
+                    engine not in plain):
         raise NotImplementedError("context rows (every column sees the positions before its row's first only) are the "
                                   "m16n8k16 kernel's plain rows")
     k_kind = _check_kind(kind, key_scales)
@@ -650,13 +658,13 @@ def attend(q, key_pages, value_pages, kind, tables, rows, starts, firsts, column
     positions = tables.shape[1] * page
     if parents is not None:
         # a draft tree: parents [tokens] is each token's parent column in its row, -1 for none (topological order)
-        if engine not in (None, "mma.sync"):
+        if engine not in plain:
             raise NotImplementedError("draft trees (parents) are served by the m16n8k16 kernel: engine None or mma.sync")
         parents = parents.reshape(-1)
         if parents.dtype not in (torch.int32, torch.int64) or parents.numel() != T:
             raise ValueError("parents are int32 or int64, one per token of q")
         parents = _cuda(parents, "parents").to(torch.int32).contiguous()
-        engine = "mma.sync"
+        engine = masked
     if blocks is not None:
         # block lists: blocks [tokens][k] KV block ids (-1 for none) of block_size positions: a token sees only those
         if blocks.dim() != 2 or blocks.shape[0] != T or not block_size or int(block_size) < 1:
@@ -672,15 +680,15 @@ def attend(q, key_pages, value_pages, kind, tables, rows, starts, firsts, column
                           counts=listed[4], key_scales=key_scales, value_scales=value_scales, multipliers=multipliers,
                           scale=scale, partitions=partitions, out=out, lse=lse, workspace=workspace, chunk=chunk,
                           engine=engine)
-        if engine not in (None, "mma.sync"):
+        if engine not in plain:
             raise NotImplementedError("block lists of blocks that are no multiple of the page, or with a tree, sinks or a "
                                       "sliding window, are a mask of the m16n8k16 kernel: engine None or mma.sync")
-        engine = "mma.sync"             # as a mask over the m16n8k16 kernel's tiles: every position is read
+        engine = masked             # as a mask over the m16n8k16 kernel's tiles: every position is read
     sliding = int(sliding or 0)
     if sinks is not None or sliding:
         # a sink logit a query head (joins the softmax's maximum and sum, and the lse, in the fold of the splits), and a
         # window of the `sliding` positions up to a column's own: the m16n8k16 kernel's
-        if engine not in (None, "mma.sync"):
+        if engine not in plain:
             raise NotImplementedError("sinks and sliding windows are served by the m16n8k16 kernel: engine None or mma.sync")
         if shards is not None and sinks is not None:
             raise NotImplementedError("a sharded context's merge does not take sinks")
@@ -691,12 +699,14 @@ def attend(q, key_pages, value_pages, kind, tables, rows, starts, firsts, column
             if sinks.numel() != hq:
                 raise ValueError(f"sinks are one logit a query head ({hq}), not {sinks.numel()}")
             sinks = sinks.float().contiguous()
-        engine = "mma.sync"
+        engine = masked
     if context:
-        engine = "mma.sync"
+        engine = masked
     chosen = engine is None
     if chosen and (shards is not None or persistent or staging is not None):
         engine = "mma.sync"               # what those arguments are about
+    if chosen and k_kind == 5 and (chunk or partitions or offsets is not None or workspace is not None):
+        engine = "mma.sync"               # the caller cuts the launch itself
     engine = engine_for(kind, d, dv, hq, hkv, int(columns), R, positions, engine)
     chunk = int(chunk or chunk_for(d, dv, hq, hkv, page, kind, engine, int(columns)))
     if partitions:
@@ -711,7 +721,9 @@ def attend(q, key_pages, value_pages, kind, tables, rows, starts, firsts, column
     if out.dtype != q.dtype or out.stride(-1) != 1:
         raise ValueError("out is in q's dtype, its last dimension contiguous")
     p = _lib.AttendParams()
-    if splits > 1 or shards is not None or sinks is not None:
+    if engine == "even" and k_kind != 5:
+        raise NotImplementedError("the even engine reads int4 pages")
+    if engine != "even" and (splits > 1 or shards is not None or sinks is not None):
         floats = workspace_floats(partial_rows, hq, splits, dv)
         space = _workspace(device, floats, workspace)
         p.workspace, p.workspace_floats = _ptr(space), space.numel()
@@ -733,7 +745,7 @@ def attend(q, key_pages, value_pages, kind, tables, rows, starts, firsts, column
     if staging not in (None, "tma", "cp.async"):
         raise ValueError("staging is None, tma or cp.async")
     p.flags = ({None: 0, "cp.async": 1, "tma": 2}[staging] | (4 if persistent else 0) |
-               {"tcgen05": 8, "mma.sync": 16, "tcgen05t": 64, "tcgen05p": 128}[engine] | (32 if shards is not None else 0) | (256 if context else 0))
+               {"tcgen05": 8, "mma.sync": 16, "tcgen05t": 64, "tcgen05p": 128, "even": 512}[engine] | (32 if shards is not None else 0) | (256 if context else 0))
     p.status = _ptr(_status_word(device))
     p.scale = float(scale if scale is not None else d ** -0.5)
     p.key_multiplier, p.value_multiplier = float(multipliers[0]), float(multipliers[1])
@@ -741,6 +753,13 @@ def attend(q, key_pages, value_pages, kind, tables, rows, starts, firsts, column
     if blocks is not None:
         p.blocks, p.blocks_k, p.block_size = _ptr(blocks), blocks.shape[1], int(block_size)
     lib = _lib.load()
+    if engine == "even":
+        with torch.cuda.device(device):
+            floats = lib.crit_b200_attend_floats(ctypes.byref(p))
+            if floats < 0:
+                _lib.check(floats, "crit_b200.attend")
+        space = _workspace(device, floats, workspace)
+        p.workspace, p.workspace_floats = _ptr(space), space.numel()
     if shards is not None:
         if lse is None:
             raise ValueError("a sharded context's merge writes lse too: pass lse")

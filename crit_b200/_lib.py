@@ -113,6 +113,7 @@ SYMBOLS = {
     "crit_b200_gather": (c_int, [POINTER(GatherParams), c_void_p]),
     "crit_b200_slots": (c_int, [POINTER(SlotsParams), c_void_p]),
     "crit_b200_attend_plan": (c_int, [c_int32] * 8 + [POINTER(c_int32)]),
+    "crit_b200_attend_floats": (c_int64, [POINTER(AttendParams)]),
     "crit_b200_decode": (c_int, [POINTER(AttendParams), c_void_p]),
     "crit_b200_merge": (c_int, [POINTER(AttendParams), c_void_p]),
     "crit_b200_attend": (c_int, [POINTER(AttendParams), c_void_p]),

@@ -170,8 +170,10 @@ class DeviceAttention:
         sinks, sliding = getattr(self, "_sinks", None), getattr(self, "_sliding", 0)
         listed = getattr(self, "_blocks", None)
         sparse = listed is not None and listed[1] % pool.page == 0           # the lists as page tables of their own: any kernel
-        if parents is not None or sinks is not None or sliding or (listed is not None and not sparse):
-            named = "mma.sync"             # draft trees, sinks, sliding windows and lists as masks are the m16n8k16 kernel's
+        if (parents is not None or sinks is not None or sliding or (listed is not None and not sparse)) and named != "even":
+            named = "mma.sync"             # draft trees, sinks, sliding windows and lists as masks are the m16n8k16 kernels'
+        if named == "even" and (self.partial_bytes or self.partitions or self.chunk or len(meta) > kernels.EVEN_ROWS):
+            named = "mma.sync"             # (partials from the engine's scratch, or splits as the options cut them)
         chunk = self.chunk or kernels.chunk_for(pool.head_dim, pool.value_dim, q.shape[1], pool.kv_heads, pool.page, pool.dtype,
                                                 named, meta.columns)
         if self.partitions:

@@ -153,6 +153,17 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 
+// A sink logit (natural units of the scaled scores) joins a folded state (top in base-2 units, total relative to it):
+// the maximum and the sum take it, the outputs shrink by 2^(old top - new top).
+__device__ __forceinline__ void sink_fold(float sink, float& top, float& total, float& shrink) {
+    const float s2 = sink * LOG2E;
+    const float up = fmaxf(top, s2);
+    if (up == -INFINITY) return;
+    shrink = top == -INFINITY ? 0.f : ex2(top - up);
+    total = total * shrink + ex2(s2 - up);
+    top = up;
+}
+
 // -- mbarrier and bulk (TMA) copies ---------------------------------------------------------------------------------------
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");

@@ -16,21 +16,12 @@ namespace crit_b200 {
 constexpr int MERGE_WARPS = 8;
 
 int launch_decode4(const crit_b200_attend_params& p, cudaStream_t s);                                   // decode4.cu
+int launch_merge4(const crit_b200_attend_params& p, cudaStream_t s);
+int64_t even_floats4(const crit_b200_attend_params& p);
 int plan_decode4(int q_heads, int kv_heads, int d, int columns, int32_t* out5);
 
 // States a row of L positions has in the workspace: one a split, or two (a split's head and tail; m = -inf marks one
 // that holds nothing, and the folds pass it over) after a launch that deals tiles out evenly.
-// A sink logit (natural units of the scaled scores) joins a folded state (top in base-2 units, total relative to it):
-// the maximum and the sum take it, the outputs shrink by 2^(old top - new top).
-__device__ __forceinline__ void sink_fold(float sink, float& top, float& total, float& shrink) {
-    const float s2 = sink * LOG2E;
-    const float up = fmaxf(top, s2);
-    if (up == -INFINITY) return;
-    shrink = top == -INFINITY ? 0.f : ex2(top - up);
-    total = total * shrink + ex2(s2 - up);
-    top = up;
-}
-
 __device__ __forceinline__ int states_of(const crit_b200_attend_params& p, int64_t L) {
     const int n = (int)((L + p.chunk - 1) / p.chunk);
     return (p.flags & CRIT_B200_ATTEND_TCGEN05P) ? 2 * n : n;
@@ -479,6 +470,12 @@ static int check(const crit_b200_attend_params& p) {
         return CRIT_B200_EALIGN;
     if (p.head_dim < 1 || p.value_dim < 1 || p.head_dim > 1024 || p.value_dim > 1024) return CRIT_B200_EUNSUPPORTED;
     if (p.sliding < 0 || (p.blocks && (p.blocks_k < 1 || p.block_size < 1))) return CRIT_B200_EINVAL;
+    if (p.flags & CRIT_B200_ATTEND_EVEN) {
+        const int64_t floats = even_floats4(p);
+        if (floats < 0) return (int)floats;
+        if (!p.workspace || p.workspace_floats < floats) return CRIT_B200_EWORKSPACE;
+        return aligned(p.workspace, 16) ? 0 : CRIT_B200_EALIGN;
+    }
     if (p.max_splits > 1 || (p.flags & CRIT_B200_ATTEND_PARTIALS) || p.sinks) {
         // partial_rows <= 2^31, q_heads and max_splits below 2^31, value_dim + 2 <= 1026: compared by division, so that no
         // product of the four can wrap
@@ -644,6 +641,7 @@ static int launch_decode(const crit_b200_attend_params& p, cudaStream_t s) {
 }
 
 static int launch_merge(const crit_b200_attend_params& p, cudaStream_t s) {
+    if (p.flags & CRIT_B200_ATTEND_EVEN) return launch_merge4(p, s);
     if (p.max_splits <= 1 && !(p.flags & CRIT_B200_ATTEND_PARTIALS) && !p.sinks) return 0;
     if (p.value_dim > 256 || p.value_dim % 32) return CRIT_B200_EUNSUPPORTED;
     if (p.max_splits <= 32) {
@@ -796,6 +794,18 @@ extern "C" __attribute__((visibility("default"))) int crit_b200_attend_plan(int3
     out5[3] = per_sm;
     out5[4] = sms;
     return 0;
+}
+
+extern "C" __attribute__((visibility("default"))) int64_t crit_b200_attend_floats(const crit_b200_attend_params* params) {
+    if (!params) return CRIT_B200_EINVAL;
+    const crit_b200_attend_params& p = *params;
+    if (p.n_rows < 1 || p.columns < 1 || p.columns > 64 || p.q_heads < 1 || p.kv_heads < 1 || p.q_heads % p.kv_heads || p.value_dim < 1 || p.value_dim > 1024)
+        return CRIT_B200_EINVAL;
+    if (p.flags & CRIT_B200_ATTEND_EVEN) return even_floats4(p);
+    if (p.max_splits < 1 || p.partial_rows < 1) return CRIT_B200_EINVAL;
+    const int64_t per_row = (int64_t)p.q_heads * (p.value_dim + 2);
+    if (per_row > INT64_MAX / p.max_splits / p.partial_rows) return CRIT_B200_EINVAL;
+    return per_row * p.max_splits * p.partial_rows;
 }
 
 extern "C" __attribute__((visibility("default"))) int crit_b200_decode(const crit_b200_attend_params* params, void* stream) {

@@ -1,25 +1,41 @@
 // Split-K decode / speculative-verify attention over 4-bit pages (int4.cuh has the format).
 //
-// A block is a producer warp and a warp for each of HB kv heads (HB = 8, 4, 2 or 1: the most that divides the heads); it
-// reads whole page rows, 16 positions of its HB heads a tile: one box of a tensor map with permuted dimensions, [dim / 2
-// bytes][slots][kv_heads], is HB * dim / 2 contiguous bytes a position and lands head-major, swizzled as wide as a row is.
-// So the bytes asked of HBM are long pieces although a row of one head is 64 bytes (dim 128), and no warp spends
-// instructions on copies.  The tile's scales come by a bulk copy onto the same mbarrier.
+// A block is a warp for each of HB kv heads (8, 4, 2 or 1: the most that divides the heads) and reads whole page rows, 16
+// positions of its HB heads a tile: one box of a tensor map with permuted dimensions, [dim / 2 bytes][slots][kv_heads], is
+// HB * dim / 2 contiguous bytes a position and lands head-major, swizzled as wide as a row is.  So the bytes asked of HBM
+// are long pieces although a row of one head is 64 bytes (dim 128).  The tile's scales come by a bulk copy onto the same
+// mbarrier.  There is no producer warp (a ninth warp would take the registers of two blocks an SM): the warps take turns,
+// warp n mod HB refills the ring when it comes to tile n, with a tile S - 2 ahead and the page id it read a turn before.
 //
 // A warp attends its own head's query rows (up to 8 NT: the columns of a verify window times the heads of the kv head's
-// group) and never waits for another warp.  Scores and outputs are m16n8k16 products, positions or value columns on the
-// instruction's 16 rows, query rows on its 8 columns:
+// group) and waits for the others only through the ring.  Scores and outputs are m16n8k16 products, positions or value
+// columns on the instruction's 16 rows, query rows on its 8 columns:
 //   S^T[16 positions][8 query rows] = K Q^T    one accumulator a group of 32: a group's scale is one number a position,
 //                                              so x = sum over groups of scale[position][group] * S_group, in FP32
-//   O^T[32 values][8 query rows] += V^T (P .* scale)     the values' scales multiply the probabilities, a group at a time
+//   O^T[32 values][8 query rows] += V^T P^T    the values' scales multiply the probabilities (a group at a time), or the
+//                                              codes
 // The codes never pass through a thread one by one: ldmatrix hands a thread the 8 codes of a position and group that its
-// fragments want (K), or, transposed, 4 codes each of two neighbouring positions (V), and a mask, an OR and an add make two
-// FP16 numbers of two codes.  The head dimension is consumed in the order the nibbles come, the queries laid out to match.
+// fragments want (K), or, transposed, 4 codes each of two neighbouring positions (V).  The head dimension is consumed in the
+// order the nibbles come, the queries laid out to match.
+//
+// Codes as FP16 operands.  The nibbles 0 and 4 of a word under the mask 0x000f000f ARE two FP16 numbers, n * 2^-24 (subnormal;
+// the tensor cores take them as they are), the nibbles 1 and 5 under 0x00f000f0 are 16 n * 2^-24: one AND makes two operands,
+// where 1024 + n less 1032 takes an OR and an add more.  The factor 16 is undone in the queries (their odd elements are
+// divided by 16) and in the outputs' odd columns, 2^-24 in a constant.  The 8 that a code stands above its value comes off in
+// the accumulators: K Q^T starts from -8 * the sum of the group's queries, and a product of a constant matrix with P^T
+// gathers -8 * the sum of the group's weights.  Where the accumulators for that do not fit the registers (wide tiles of query
+// rows, the outputs of 256-wide heads), codes become n - 8 one add later.
 //
 // The queries become FP16 with an exponent of their own a row (the largest element between 2^13 and 2^14), so no bf16 query
 // overflows or vanishes.  Weights are 2^(x - ref) with ref at most 2 (in the exponent) above the running maximum and never
 // below it: a weight is at most 1, times a scale of at most 61,440 it stays an FP16 number, and the running reference moves
 // only when a score passes it.  Sums are FP32.
+//
+// Two ways to cut a launch.  By splits: a 3-D grid of (split of `chunk` positions, heads and query tiles, row), states in the
+// workspace as every other decode kernel leaves them: a column's bits do not depend on the launch.  Even
+// (CRIT_B200_ATTEND_EVEN): the launch's tiles, rows in order, are dealt out in equal runs to the blocks the device holds at
+// once; where a run and a row overlap there is one state, slot = block + row (both only grow along the tiles, so the sum
+// names the pair), and merge4_kernel folds a row's consecutive slots.  No block idles while another has two splits to go.
 #include <mutex>
 
 #include "int4.cuh"
@@ -28,19 +44,26 @@
 namespace crit_b200 {
 
 constexpr int D4_MAX_STAGES = 8;
+constexpr int D4_MAX_ROWS = 256;              // window rows an even launch lists
+constexpr int D4_MIN_RUN = 4;                 // tiles an even launch's block takes at least
 
-// The most kv heads a block takes: 8, or 4 where a warp's accumulators want more registers than 9 warps leave (a quarter of
-// an SM holds 3 of 9 warps, 168 registers a thread, and 2 of 5).
+// The most kv heads a block takes, and the blocks an SM is to hold: a warp's accumulators decide (the registers of 16 warps
+// are 128 a thread, of 8 warps 255).
 constexpr __host__ __device__ int decode4_heads(int d, int nt) { return d == 256 || nt == 4 ? 4 : 8; }
+constexpr __host__ __device__ int decode4_blocks(int d, int nt) { return (nt == 1 && d <= 128) || d == 256 || nt == 4 ? 2 : 1; }
 
 struct Decode4Launch {
     int heads;              // kv heads a block takes (HB)
-    int ctiles;             // tiles of 8 NT query rows a window row takes
+    int ctiles;             // tiles of 8 NT query rows a window row takes at most
     int stages;             // of the ring
     int stage_bytes;
+    int blocks;             // of an even launch; 0: splits
 };
 
-// Two FP16 numbers (code - 8 each) from the nibbles 0 and 4 (or 1 and 5) of a word.
+// Two FP16 numbers from the nibbles 0 and 4 (low) or 1 and 5 (high) of a word: n * 2^-24 and 16 n * 2^-24 ...
+__device__ __forceinline__ uint32_t raw_low(uint32_t w) { return w & 0x000f000fu; }
+__device__ __forceinline__ uint32_t raw_high(uint32_t w) { return w & 0x00f000f0u; }
+// ... or n - 8.
 __device__ __forceinline__ uint32_t codes_low(uint32_t w) {
     uint32_t x = (w & 0x000f000fu) | 0x64006400u;                  // 1024 + n
     __half2 h = __hsub2(*reinterpret_cast<__half2*>(&x), __floats2half2_rn(1032.f, 1032.f));
@@ -51,11 +74,14 @@ __device__ __forceinline__ uint32_t codes_high(uint32_t w) {
     __half2 h = __hfma2(*reinterpret_cast<__half2*>(&x), __floats2half2_rn(0.0625f, 0.0625f), __floats2half2_rn(-72.f, -72.f));
     return *reinterpret_cast<uint32_t*>(&h);
 }
-
-// A lane's scales: bytes [a, a', b, b'] of two positions (a, b) and two neighbouring groups -> FP16 pairs (a, b) and (a', b').
-__device__ __forceinline__ void scale_pairs(uint32_t x, uint32_t& even, uint32_t& odd) {
-    even = (x << 7) & 0x7f807f80u;
-    odd = (x >> 1) & 0x7f807f80u;
+template <bool RAW>
+__device__ __forceinline__ void four_operands(uint32_t lo, uint32_t hi, uint32_t (&a1)[4], uint32_t (&a2)[4], int i1, int i2) {
+    // words lo and hi -> operands 0 and i1 of the low nibbles, i2 and 3 of the high ones; a2 from the words' upper bytes
+    a1[0] = RAW ? raw_low(lo) : codes_low(lo), a1[i1] = RAW ? raw_low(hi) : codes_low(hi);
+    a1[i2] = RAW ? raw_high(lo) : codes_high(lo), a1[3] = RAW ? raw_high(hi) : codes_high(hi);
+    lo >>= 8, hi >>= 8;
+    a2[0] = RAW ? raw_low(lo) : codes_low(lo), a2[i1] = RAW ? raw_low(hi) : codes_low(hi);
+    a2[i2] = RAW ? raw_high(lo) : codes_high(lo), a2[3] = RAW ? raw_high(hi) : codes_high(hi);
 }
 
 __device__ __forceinline__ uint32_t hmul2_bits(uint32_t a, uint32_t b) {
@@ -63,8 +89,24 @@ __device__ __forceinline__ uint32_t hmul2_bits(uint32_t a, uint32_t b) {
     return *reinterpret_cast<uint32_t*>(&h);
 }
 // all ones in the halves that are not zero
-__device__ __forceinline__ uint32_t nonzero2(uint32_t a) {
-    return __hne2_mask(*reinterpret_cast<__half2*>(&a), __floats2half2_rn(0.f, 0.f));
+__device__ __forceinline__ uint32_t nonzero2(uint32_t a) { return __hne2_mask(*reinterpret_cast<__half2*>(&a), __floats2half2_rn(0.f, 0.f)); }
+
+// The scales of two positions for a row's groups, as FP16 pairs (first position, second): NG bytes from each address.
+template <int NG>
+__device__ __forceinline__ void scale_pairs(const unsigned char* a, const unsigned char* b, uint32_t (&pair)[NG]) {
+    constexpr int WORDS = NG >= 4 ? NG / 4 : 1;
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) {
+        uint32_t x, y;
+        if constexpr (NG >= 4) x = reinterpret_cast<const uint32_t*>(a)[w], y = reinterpret_cast<const uint32_t*>(b)[w];
+        else x = *reinterpret_cast<const uint16_t*>(a), y = *reinterpret_cast<const uint16_t*>(b);
+#pragma unroll
+        for (int k = 0; k < (NG >= 4 ? 2 : 1); ++k) {
+            const uint32_t four = __byte_perm(x, y, k ? 0x7632 : 0x5410);          // bytes [x, x', y, y']: two groups
+            pair[4 * w + 2 * k] = (four << 7) & 0x7f807f80u;
+            pair[4 * w + 2 * k + 1] = (four >> 1) & 0x7f807f80u;
+        }
+    }
 }
 
 // Byte offset of 16-byte chunk c (a group of 32 codes) of row `row` of a tile, rows of D / 2 bytes with TMA's swizzle of
@@ -76,465 +118,765 @@ __device__ __forceinline__ int chunk4(int row, int c) {
     else return row * 32 + ((c ^ ((row >> 2) & 1)) << 4);
 }
 
+// A row of the launch: its tiles, and how many times they are read (head groups x tiles of query rows).
+__device__ __forceinline__ int row_tiles4(const crit_b200_attend_params& p, int r, int count) {
+    const int64_t L = p.firsts[r] + ((p.flags & CRIT_B200_ATTEND_CONTEXT) ? 0 : count);
+    return count > 0 && L > 0 ? (int)((L + 15) >> 4) : 0;
+}
+__device__ __forceinline__ int row_count4(const crit_b200_attend_params& p, int r) {
+    const int count = p.counts ? p.counts[r] : p.columns;
+    return count > p.columns ? p.columns : count;
+}
+
+// A place among a block's tiles: row, (head group, query tile) of the row, tile.
+struct Place4 {
+    int r, sub, tile, tiles, subs;
+};
+
 // MASKS: draft trees, sliding windows and block lists (else a column sees every position up to its own).
-template <int D, int NT, bool MASKS>
-__global__ void __launch_bounds__(32 * (decode4_heads(D, NT) + 1)) decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u,
-                                                      const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+// FAST: the fewest instructions for the tile's width (raw codes, scales on the weights where NT is 1).  Otherwise every width
+// does the same arithmetic, n - 8 and the scales on the codes, so that a launch cut into splits gives a column the same bits
+// alone and in any window, and a weight is rounded once, which FP16 outputs' 11 bits ask for.
+template <int D, int NT, bool MASKS, bool FAST>
+__global__ void __launch_bounds__(32 * decode4_heads(D, NT), decode4_blocks(D, NT))
+decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     constexpr int NG = D / 32;                // groups of a row
     constexpr int ROWS = 8 * NT;
     constexpr int TPI = 2;                    // tiles an iteration takes
     constexpr float AHEAD = 2.f;
+    constexpr bool RAW_K = FAST && NT <= 2;                 // the 8 of the keys' codes through the accumulators' start
+    constexpr bool RAW_V = FAST && NT == 1 && D <= 128;     // that of the values' through a product of its own
+    constexpr bool SCALE_CODES = !FAST || NT > 1;           // the values' scales on the codes (an exact product), not on the weights:
+                                                            // fewer products where a tile holds several columns of query rows
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     __shared__ __align__(8) uint64_t bars_mem[2 * D4_MAX_STAGES];
+    __shared__ int list_first[D4_MAX_ROWS + 1], list_tiles[D4_MAX_ROWS], list_subs[D4_MAX_ROWS];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int G = p.q_heads / p.kv_heads;
-    const int HB = u.heads;
+    const int HB = u.heads, HG = p.kv_heads / HB;
     const uint32_t full = smem_addr(bars_mem), empty = full + D4_MAX_STAGES * 8;
+    const bool context = (p.flags & CRIT_B200_ATTEND_CONTEXT) != 0;       // the positions before a row's first only
     if (threadIdx.x == 0) {
         for (int s = 0; s < u.stages; ++s) mbar_init(full + s * 8, 1), mbar_init(empty + s * 8, HB);
         mbar_init_fence();
     }
-    __syncthreads();
 
-    // -- the unit --------------------------------------------------------------------------------------------------------
-    const int r = blockIdx.z, split = blockIdx.x;
-    const int hg = blockIdx.y / u.ctiles, ct = blockIdx.y - hg * u.ctiles;
-    int count = p.counts ? p.counts[r] : p.columns;
-    count = count > p.columns ? p.columns : count;
-    if (count <= 0 || ct * ROWS >= count * G) return;
-    const int64_t first = p.firsts[r];
-    const bool context = (p.flags & CRIT_B200_ATTEND_CONTEXT) != 0;       // the positions before `first` only
-    const int64_t L = context ? first : first + count;
-    const int64_t begin = (int64_t)split * p.chunk;
-    if (begin >= L) {
-        // a row that holds no position (a context row at position 0): zeros and -inf, as the fold of no state gives
-        if (L <= 0 && split == 0 && !(p.flags & CRIT_B200_ATTEND_PARTIALS) && warp < HB) {
-            for (int rr = 0; rr < ROWS; ++rr) {
-                const int flat = ct * ROWS + rr, col = flat / G;
-                if (col >= count) break;
-                const int64_t token = p.starts[r] + col, head = (hg * HB + warp) * G + flat - col * G;
-                for (int c = lane; c < D; c += 32) reinterpret_cast<uint16_t*>(p.out)[token * p.out_stride_token + head * p.out_stride_head + c] = 0;
-                if (lane == 0 && p.lse) p.lse[token * p.q_heads + head] = -INFINITY;
+    // -- the block's tiles -------------------------------------------------------------------------------------------------
+    Place4 at;                      // where the block begins
+    int length;                     // tiles it takes
+    if (u.blocks) {
+        if (warp == 0) {
+            int carry = 0;
+            for (int base = 0; base < p.n_rows; base += 32) {
+                const int r = base + lane;
+                int tiles = 0, subs = 0;
+                if (r < p.n_rows) {
+                    const int count = row_count4(p, r);
+                    tiles = row_tiles4(p, r, count), subs = count > 0 ? HG * ((count * G + ROWS - 1) / ROWS) : 0;
+                }
+                int scan = tiles * subs;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int up = __shfl_up_sync(0xffffffffu, scan, o);
+                    if (lane >= o) scan += up;
+                }
+                if (r < p.n_rows) list_first[r + 1] = carry + scan, list_tiles[r] = tiles, list_subs[r] = subs;
+                carry += __shfl_sync(0xffffffffu, scan, 31);
+            }
+            if (lane == 0) list_first[0] = 0;
+        }
+        __syncthreads();
+        const int total = list_first[p.n_rows];
+        const int share = (total + u.blocks - 1) / u.blocks, run = share > D4_MIN_RUN ? share : D4_MIN_RUN;
+        if (blockIdx.x == 0) {      // what the fold reads: the run, and where a row begins
+            int* info = reinterpret_cast<int*>(p.workspace);
+            for (int r = threadIdx.x; r <= p.n_rows; r += blockDim.x) info[1 + r] = list_first[r];
+            if (threadIdx.x == 0) info[0] = run;
+        }
+        const int begin = blockIdx.x * run;
+        length = total - begin < run ? total - begin : run;
+        if (length <= 0) return;
+        int lo = 0, hi = p.n_rows;                  // the row whose tiles hold `begin` (of rows that begin there the last, which has tiles)
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (list_first[mid] <= begin) lo = mid;
+            else hi = mid;
+        }
+        at.r = lo, at.tiles = list_tiles[lo], at.subs = list_subs[lo];
+        at.sub = (begin - list_first[lo]) / at.tiles;
+        at.tile = begin - list_first[lo] - at.sub * at.tiles;
+    } else {
+        __syncthreads();
+        const int r = blockIdx.z, count = row_count4(p, r);
+        const int hg = blockIdx.y / u.ctiles, ct = blockIdx.y - hg * u.ctiles;
+        if (count <= 0 || ct * ROWS >= count * G) return;
+        at.r = r, at.tiles = row_tiles4(p, r, count), at.subs = 0x7fffffff;
+        at.sub = blockIdx.y, at.tile = blockIdx.x * (p.chunk >> 4);
+        length = at.tiles - at.tile < (p.chunk >> 4) ? at.tiles - at.tile : (p.chunk >> 4);
+        if (length <= 0) {
+            // a row that holds no position (a context row at position 0): zeros and -inf, as the fold of no state gives
+            if (at.tiles == 0 && blockIdx.x == 0 && !(p.flags & CRIT_B200_ATTEND_PARTIALS)) {
+                for (int rr = 0; rr < ROWS; ++rr) {
+                    const int flat = ct * ROWS + rr, col = flat / G;
+                    if (col >= count) break;
+                    const int64_t token = p.starts[r] + col, head = (hg * HB + warp) * G + flat - col * G;
+                    for (int c = lane; c < D; c += 32) reinterpret_cast<uint16_t*>(p.out)[token * p.out_stride_token + head * p.out_stride_head + c] = 0;
+                    if (lane == 0 && p.lse) p.lse[token * p.q_heads + head] = -INFINITY;
+                }
+            }
+            return;
+        }
+    }
+
+    const int code_bytes = HB * 16 * (D / 2);                              // a tile's keys, or its values
+    const int row_scales = p.kv_heads * NG;                                // bytes of a position's scales
+    const int scale_bytes = 16 * row_scales;
+    const uint32_t tiles_per_page = (uint32_t)p.page >> 4;
+    const int tshift = (tiles_per_page & (tiles_per_page - 1)) == 0 ? __ffs((int)tiles_per_page) - 1 : -1;
+    const uint32_t pages_total = (uint32_t)(p.slots / p.page);
+    const uint32_t ring = smem_addr(smem);
+
+    // -- refilling the ring (lane 0; a warp's turns are HB tiles apart) ------------------------------------------------------
+    Place4 next = at;               // the tile of this warp's next turn, its page read ahead
+    int next_n = warp, next_page = 0;
+    auto step_to = [&](Place4& c, int by) {
+        c.tile += by;
+        while (c.tile >= c.tiles) {
+            c.tile -= c.tiles;
+            if (++c.sub >= c.subs) {
+                c.sub = 0;
+                do ++c.r; while (c.r < p.n_rows && list_tiles[c.r] * list_subs[c.r] == 0);
+                if (c.r >= p.n_rows) return;         // (past the launch's last tile: no turn comes to it)
+                c.tiles = list_tiles[c.r], c.subs = list_subs[c.r];
             }
         }
-        return;
+    };
+    auto read_page = [&]() {
+        if (next_n < length) {
+            const uint32_t tile = (uint32_t)next.tile;
+            next_page = p.tables[(int64_t)p.rows[next.r] * p.table_stride + (tshift >= 0 ? tile >> tshift : tile / tiles_per_page)];
+        }
+    };
+    bool outside = false;
+    auto refill = [&](int stage) {  // tile next_n into its stage, which is free
+        const uint32_t tile = (uint32_t)next.tile;
+        const uint32_t pidx = tshift >= 0 ? tile >> tshift : tile / tiles_per_page;
+        outside |= (uint32_t)next_page >= pages_total;             // the tensor's last page is read instead; reported below
+        const uint32_t pg = (uint32_t)next_page < pages_total ? (uint32_t)next_page : pages_total - 1;
+        const int64_t slot0 = (int64_t)pg * p.page + ((tile - pidx * tiles_per_page) << 4);
+        const int head0 = (u.blocks ? next.sub / (next.subs / HG) : next.sub / u.ctiles) * HB;
+        const uint32_t bar = full + stage * 8, to = ring + stage * u.stage_bytes;
+        mbar_expect_tx(bar, (uint32_t)(2 * code_bytes + 2 * scale_bytes));
+        tma_load_3d(to, &kmap, 0, (int)slot0, head0, bar);
+        bulk_load(to + 2 * code_bytes, (const char*)p.key_scales + slot0 * row_scales, scale_bytes, bar);
+        tma_load_3d(to + code_bytes, &vmap, 0, (int)slot0, head0, bar);
+        bulk_load(to + 2 * code_bytes + scale_bytes, (const char*)p.value_scales + slot0 * row_scales, scale_bytes, bar);
+    };
+    auto turn_over = [&]() {        // to this warp's next turn
+        next_n += HB;
+        if (lane == 0 && next_n < length) step_to(next, HB), read_page();
+    };
+    if (lane == 0 && warp < length) step_to(next, warp), read_page();
+    while (next_n < u.stages - 2 && next_n < length) {             // the first tiles: two stages stay free
+        if (lane == 0) refill(next_n);
+        turn_over();
     }
-    const int64_t end = begin + p.chunk < L ? begin + p.chunk : L;
-    const int nsplit = (int)((L + p.chunk - 1) / p.chunk);
-    const int tile0 = (int)(begin >> 4), ntiles = (int)((end - begin + 15) >> 4);
-    const int code_bytes = HB * 16 * (D / 2);                              // a tile's keys, or its values
-    const int scale_bytes = 16 * p.kv_heads * NG;
-    const int row_scales = p.kv_heads * NG;                                // bytes of a position's scales
 
     bool dead = false;
-    if (warp == HB) {
-        // -- producer ------------------------------------------------------------------------------------------------------
-        const int32_t* table = p.tables + (int64_t)p.rows[r] * p.table_stride;
-        const uint32_t tiles_per_page = (uint32_t)p.page >> 4;
-        const uint32_t pages_total = (uint32_t)(p.slots / p.page);
-        int stage = 0;
-        uint32_t phase = 0;
-        int pgs = 0;
-        bool outside = false;
-        for (int i = 0; i < ntiles && !dead; ++i) {
-            if ((i & 31) == 0) pgs = i + lane < ntiles ? table[(uint32_t)(tile0 + i + lane) / tiles_per_page] : 0;
-            const uint32_t listed = (uint32_t)__shfl_sync(0xffffffffu, pgs, i & 31);
-            outside |= listed >= pages_total;             // the tensor's last page is read instead; reported below
-            if (lane == 0) {
-                const uint32_t tile = (uint32_t)(tile0 + i);
-                const uint32_t pg = listed < pages_total ? listed : pages_total - 1;
-                const int64_t slot0 = (int64_t)pg * p.page + ((tile % tiles_per_page) << 4);
-                dead = !mbar_wait(empty + stage * 8, phase ^ 1);
-                if (!dead) {
-                    const uint32_t bar = full + stage * 8, at = smem_addr(smem) + stage * u.stage_bytes;
-                    mbar_expect_tx(bar, (uint32_t)(2 * code_bytes + 2 * scale_bytes));
-                    tma_load_3d(at, &kmap, 0, (int)slot0, hg * HB, bar);
-                    bulk_load(at + 2 * code_bytes, (const char*)p.key_scales + slot0 * row_scales, scale_bytes, bar);
-                    tma_load_3d(at + code_bytes, &vmap, 0, (int)slot0, hg * HB, bar);
-                    bulk_load(at + 2 * code_bytes + scale_bytes, (const char*)p.value_scales + slot0 * row_scales, scale_bytes, bar);
-                }
-            }
-            dead = __any_sync(0xffffffffu, dead);
-            if (++stage == u.stages) stage = 0, phase ^= 1;
-        }
-        if (outside && lane == 0 && p.status) atomicExch(p.status, CRIT_B200_STATUS_BOUNDS);
-        if (__syncthreads_or(dead ? 1 : 0)) {
-            // a copy or a reader never came: the copies in flight get a last bounded chance to land
-            if (lane == 0) {
-                for (int s = 0; s < u.stages; ++s) mbar_wait(full + s * 8, 0, 1000000ull);
-                if (p.status) atomicExch(p.status, CRIT_B200_STATUS_TMA);
-            }
-        }
-        return;
-    }
-
-    // -- a head's warp: its queries ----------------------------------------------------------------------------------------
-    const int h = hg * HB + warp;
-    const int start = p.starts[r];
-    uint32_t qb[NT][NG][4];                    // pairs (0, 4), (1, 5), (2, 6), (3, 7) of elements 32 group + 8 t + ..
-    float mul[NT][2];                          // scores of the lane's query rows (8 nt + 2 t + e) into base-2 logits
-    int lastpos[NT][2];                        // the last position they see (-1: a padding row)
-    unsigned long long seen[MASKS ? NT : 1][2];
-    const bool tree = MASKS && p.parents != nullptr;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const int flat = ct * ROWS + nt * 8 + g;
-        const int col = flat / G, gq = flat - col * G;
-        const bool live = col < count;
-        float amax = 0.f;
-        uint4 raw[NG];
-#pragma unroll
-        for (int k = 0; k < NG; ++k) {
-            raw[k] = make_uint4(0, 0, 0, 0);
-            if (live)
-                raw[k] = *reinterpret_cast<const uint4*>((const char*)p.q + ((int64_t)(start + col) * p.q_stride_token +
-                                                                             (int64_t)(h * G + gq) * p.q_stride_head + k * 32 + t * 8) * 2);
-        }
-        auto element = [&](int k, int i) {
-            const uint32_t w = (&raw[k].x)[i >> 1];
-            if (p.q_dtype == CRIT_B200_DTYPE_BF16) return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
-            return __half2float(__ushort_as_half((unsigned short)(i & 1 ? w >> 16 : w)));
-        };
-#pragma unroll
-        for (int k = 0; k < NG; ++k)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(element(k, i)));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        int e = (int)((__float_as_uint(amax) >> 23) & 255u) - 127 - 13;
-        e = amax > 0.f ? (e < -110 ? -110 : (e > 110 ? 110 : e)) : 0;
-        const float down = __int_as_float((127 - e) << 23);
-#pragma unroll
-        for (int k = 0; k < NG; ++k)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) qb[nt][k][j] = pack2<false>(element(k, j) * down, element(k, j + 4) * down);
-        // the lane's columns are query rows 2 t and 2 t + 1: their exponents live with lanes g = 2 t and 2 t + 1
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int er = __shfl_sync(0xffffffffu, e, (2 * t + j) * 4);
-            mul[nt][j] = p.scale * LOG2E * __int_as_float((127 + er) << 23);
-            const int at = ct * ROWS + nt * 8 + 2 * t + j;
-            const int c = at / G;
-            lastpos[nt][j] = c < count ? (int)(context ? first - 1 : first + c) : -1;
-            if constexpr (MASKS) {
-                // of the window's own positions a column of a draft tree sees itself and its ancestors (bit = column)
-                seen[nt][j] = 0ull;
-                if (tree && c < count) {
-                    const int32_t* par = p.parents + start;
-                    int from = c;
-                    for (int hops = 0; from >= 0 && from < count && hops <= count; ++hops) {
-                        seen[nt][j] |= 1ull << from;
-                        from = par[from];
-                    }
-                }
-            }
-        }
-    }
-
-    float acc[NG][2][NT][4], m_run[NT][2], l_run[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int k = 0; k < NG; ++k)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) acc[k][i >> 2][nt][i & 3] = 0.f;
-        m_run[nt][0] = m_run[nt][1] = -INFINITY;
-        l_run[nt][0] = l_run[nt][1] = 0.f;
-    }
-
-    const int first32 = (int)first;
-    int stage = 0;
+    int n = 0, stage = 0;           // tiles taken, the ring's place
     uint32_t phase = 0;
     // ldmatrix rows: lanes 0-7 and 8-15 name positions 0-7 and 8-15 of chunk 2 i, lanes 16-31 the same of chunk 2 i + 1
     const int lrow = (lane & 7) + 8 * ((lane >> 3) & 1), lchunk = lane >> 4;
-    for (int i = 0; i < ntiles; i += TPI) {
-        const int have = ntiles - i < TPI ? ntiles - i : TPI;
-        float x[TPI][NT][4];
-        uint32_t base[TPI];
-        int stages[TPI];
-        bool masked = MASKS;
+
+    while (n < length) {
+        // -- a unit: the tiles of one row, head group and query tile in this block -----------------------------------------
+        const int r = at.r, count = row_count4(p, r);
+        const int64_t first = p.firsts[r];
+        const int first32 = (int)first;
+        const int per_hg = u.blocks ? at.subs / HG : u.ctiles;
+        const int hg = at.sub / per_hg, ct = at.sub - hg * per_hg;
+        const int h = hg * HB + warp, start = p.starts[r];
+        const int tile0 = at.tile, ntiles = at.tiles - tile0 < length - n ? at.tiles - tile0 : length - n;
+
+        uint32_t qb[NT][NG][4];                    // pairs (0, 4), (1, 5), (2, 6), (3, 7) of elements 32 group + 8 t + ..
+        float base8[RAW_K ? NT : 1][NG][2];        // -8 * the sum of a group's queries, in the accumulators' units
+        float mul[NT][2];                          // scores of the lane's query rows (8 nt + 2 t + e) into base-2 logits
+        int lastpos[NT][2];                        // the last position they see (-1: a padding row)
+        unsigned long long seen[MASKS ? NT : 1][2];
+        const bool tree = MASKS && p.parents != nullptr;
 #pragma unroll
-        for (int v = 0; v < TPI; ++v) {
+        for (int nt = 0; nt < NT; ++nt) {
+            const int flat = ct * ROWS + nt * 8 + g;
+            const int col = flat / G, gq = flat - col * G;
+            const bool live = col < count;
+            float amax = 0.f;
+            uint4 raw[NG];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) x[v][nt][c] = v < have ? 0.f : -INFINITY;
-            if (v >= have) continue;
-            stages[v] = stage;
-            base[v] = smem_addr(smem) + stage * u.stage_bytes;
-            if (!__all_sync(0xffffffffu, mbar_wait(full + stage * 8, phase))) {
-                dead = true;
-                break;
+            for (int k = 0; k < NG; ++k) {
+                raw[k] = make_uint4(0, 0, 0, 0);
+                if (live)
+                    raw[k] = *reinterpret_cast<const uint4*>((const char*)p.q + ((int64_t)(start + col) * p.q_stride_token +
+                                                                                 (int64_t)(h * G + gq) * p.q_stride_head + k * 32 + t * 8) * 2);
             }
-            if (++stage == u.stages) stage = 0, phase ^= 1;
-            masked |= ((tile0 + i + v) << 4) + 16 > first32;
-            // scores
-            const uint32_t ktile = base[v] + warp * (16 * (D / 2));
-            const unsigned char* ks = smem + (base[v] - smem_addr(smem)) + 2 * code_bytes + h * NG;
+            auto element = [&](int k, int i) {
+                const uint32_t w = (&raw[k].x)[i >> 1];
+                if (p.q_dtype == CRIT_B200_DTYPE_BF16) return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
+                return __half2float(__ushort_as_half((unsigned short)(i & 1 ? w >> 16 : w)));
+            };
 #pragma unroll
-            for (int k = 0; k < NG; k += 2) {
-                uint32_t w[4];
-                ldmatrix_x4(w, ktile + chunk4<D>(lrow, k + lchunk));
-                // the scales of positions g and g + 8, groups k and k + 1
-                const uint32_t a = *reinterpret_cast<const uint16_t*>(ks + g * row_scales + k);
-                const uint32_t b = *reinterpret_cast<const uint16_t*>(ks + (g + 8) * row_scales + k);
-                uint32_t pair[2];
-                scale_pairs(a | (b << 16), pair[0], pair[1]);
+            for (int k = 0; k < NG; ++k)
 #pragma unroll
-                for (int o = 0; o < 2; ++o) {
-                    const float2 s = __half22float2(*reinterpret_cast<__half2*>(&pair[o]));
-                    const uint32_t lo = w[2 * o], hi = w[2 * o + 1];
-                    const uint32_t a1[4] = {codes_low(lo), codes_low(hi), codes_high(lo), codes_high(hi)};
-                    const uint32_t a2[4] = {codes_low(lo >> 8), codes_low(hi >> 8), codes_high(lo >> 8), codes_high(hi >> 8)};
+                for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(element(k, i)));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            int e = (int)((__float_as_uint(amax) >> 23) & 255u) - 127 - 13;
+            e = amax > 0.f ? (e < -90 ? -90 : (e > 90 ? 90 : e)) : 0;
+            const float down = __int_as_float((127 - e) << 23);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        float c[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma16816<false>(c, a1, qb[nt][k + o][0], qb[nt][k + o][1]);
-                        mma16816<false>(c, a2, qb[nt][k + o][2], qb[nt][k + o][3]);
-                        x[v][nt][0] = fmaf(c[0], s.x, x[v][nt][0]), x[v][nt][1] = fmaf(c[1], s.x, x[v][nt][1]);
-                        x[v][nt][2] = fmaf(c[2], s.y, x[v][nt][2]), x[v][nt][3] = fmaf(c[3], s.y, x[v][nt][3]);
+            for (int k = 0; k < NG; ++k) {
+                float sum = 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float part = RAW_K && (j & 1) ? 0.0625f : 1.f;            // (the odd nibbles' operands are 16 n)
+                    qb[nt][k][j] = pack2<false>(element(k, j) * down * part, element(k, j + 4) * down * part);
+                    const float2 back = __half22float2(*reinterpret_cast<__half2*>(&qb[nt][k][j]));
+                    sum += (back.x + back.y) * (RAW_K && (j & 1) ? 16.f : 1.f);
+                }
+                if constexpr (RAW_K) {
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) base8[nt][k][j] = -0x1p-21f * __shfl_sync(0xffffffffu, sum, (2 * t + j) * 4);
+                }
+            }
+            // the lane's columns are query rows 2 t and 2 t + 1: their exponents live with lanes g = 2 t and 2 t + 1
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int er = __shfl_sync(0xffffffffu, e, (2 * t + j) * 4);
+                mul[nt][j] = p.scale * LOG2E * __int_as_float((127 + er + (RAW_K ? 24 : 0)) << 23);
+                const int c = (ct * ROWS + nt * 8 + 2 * t + j) / G;
+                lastpos[nt][j] = c < count ? (int)(context ? first - 1 : first + c) : -1;
+                if constexpr (MASKS) {
+                    // of the window's own positions a column of a draft tree sees itself and its ancestors (bit = column)
+                    seen[nt][j] = 0ull;
+                    if (tree && c < count) {
+                        const int32_t* par = p.parents + start;
+                        int from = c;
+                        for (int hops = 0; from >= 0 && from < count && hops <= count; ++hops) {
+                            seen[nt][j] |= 1ull << from;
+                            from = par[from];
+                        }
                     }
                 }
+            }
+        }
+
+        float acc[NG][2][NT][4], acc8[RAW_V ? NG : 1][4], m_run[NT][2], l_run[NT][2];
+#pragma unroll
+        for (int k = 0; k < (RAW_V ? NG : 1); ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc8[k][i] = 0.f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int k = 0; k < NG; ++k)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[k][i >> 2][nt][i & 3] = 0.f;
+            m_run[nt][0] = m_run[nt][1] = -INFINITY;
+            l_run[nt][0] = l_run[nt][1] = 0.f;
+        }
+
+        for (int i = 0; i < ntiles; i += TPI) {
+            const int have = ntiles - i < TPI ? ntiles - i : TPI;
+            float x[TPI][NT][4];
+            int stages[TPI];
+            bool masked = MASKS;
+#pragma unroll
+            for (int v = 0; v < TPI; ++v) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) x[v][nt][c] = v < have ? 0.f : -INFINITY;
+                if (v >= have) continue;
+                // this warp's turn: tile n + S - 2 into the stage of tile n - 2, once every warp is done with that
+                if (n + u.stages - 2 == next_n) {
+                    if (lane == 0 && next_n < length) {
+                        int to = stage - 2;
+                        to = to < 0 ? to + u.stages : to;
+                        // the stage's uses so far are (n - 2) / S whole rounds and one: wait for the end of the last
+                        if (n < 2 || mbar_wait(empty + to * 8, (uint32_t)((n - 2) / u.stages) & 1u)) refill(to);
+                        else dead = true;
+                    }
+                    turn_over();
+                }
+                stages[v] = stage;
+                if (!mbar_wait(full + stage * 8, phase)) dead = true;
+                if (++stage == u.stages) stage = 0, phase ^= 1;
+                ++n;
+                if (__any_sync(0xffffffffu, dead)) {
+                    dead = true;
+                    break;
+                }
+                masked |= ((tile0 + i + v) << 4) + 16 > first32;
+                // scores
+                const int from = stages[v] * u.stage_bytes;
+                const uint32_t ktile = ring + from + warp * (16 * (D / 2));
+                const unsigned char* ks = smem + from + 2 * code_bytes + h * NG;
+                uint32_t pair[NG];
+                scale_pairs<NG>(ks + g * row_scales, ks + (g + 8) * row_scales, pair);
+#pragma unroll
+                for (int k = 0; k < NG; k += 2) {
+                    uint32_t w[4];
+                    ldmatrix_x4(w, ktile + chunk4<D>(lrow, k + lchunk));
+#pragma unroll
+                    for (int o = 0; o < 2; ++o) {
+                        const float2 s = __half22float2(*reinterpret_cast<__half2*>(&pair[k + o]));
+                        uint32_t a1[4], a2[4];
+                        four_operands<RAW_K>(w[2 * o], w[2 * o + 1], a1, a2, 1, 2);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            float c[4];
+                            if constexpr (RAW_K) c[0] = c[2] = base8[nt][k + o][0], c[1] = c[3] = base8[nt][k + o][1];
+                            else c[0] = c[1] = c[2] = c[3] = 0.f;
+                            mma16816<false>(c, a1, qb[nt][k + o][0], qb[nt][k + o][1]);
+                            mma16816<false>(c, a2, qb[nt][k + o][2], qb[nt][k + o][3]);
+                            x[v][nt][0] = fmaf(c[0], s.x, x[v][nt][0]), x[v][nt][1] = fmaf(c[1], s.x, x[v][nt][1]);
+                            x[v][nt][2] = fmaf(c[2], s.y, x[v][nt][2]), x[v][nt][3] = fmaf(c[3], s.y, x[v][nt][3]);
+                        }
+                    }
+                }
+            }
+            if (dead) break;
+
+            // masks, online softmax
+            uint32_t pb[TPI][NT][2];
+            bool rescale = false;
+            float alpha[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int v = 0; v < TPI; ++v)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        float y = x[v][nt][c] * mul[nt][c & 1];
+                        if (v >= have) y = -INFINITY;
+                        if (masked) {
+                            const int pos = ((tile0 + i + v) << 4) + g + 8 * (c >> 1), last = lastpos[nt][c & 1];
+                            if (pos > last) y = -INFINITY;
+                            if constexpr (MASKS) {
+                                if (p.sliding > 0 && pos <= last - p.sliding) y = -INFINITY;
+                                if (p.blocks && last >= 0) {
+                                    const int32_t* listed = p.blocks + (int64_t)(start + (last - first32)) * p.blocks_k;
+                                    const int block = pos / p.block_size;
+                                    bool member = false;
+                                    for (int j = 0; j < p.blocks_k; ++j) member |= listed[j] == block;
+                                    if (!member) y = -INFINITY;
+                                }
+                                if (tree && pos >= first32 && (pos - first32 >= count || !((seen[nt][c & 1] >> (pos - first32)) & 1ull)))
+                                    y = -INFINITY;
+                            }
+                        }
+                        x[v][nt][c] = y;
+                        mx[c & 1] = fmaxf(mx[c & 1], y);
+                    }
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 4));
+                    mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 8));
+                    mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 16));
+                    const bool moved = mx[j] > m_run[nt][j];
+                    const float top = moved ? mx[j] + AHEAD : m_run[nt][j];
+                    const float sub = top == -INFINITY ? 0.f : top;
+                    alpha[nt][j] = moved ? ex2(m_run[nt][j] - sub) : 1.f;
+                    rescale |= moved;
+                    m_run[nt][j] = top;
+                    mx[j] = sub;
+                }
+                float sum[2] = {0.f, 0.f};
+#pragma unroll
+                for (int v = 0; v < TPI; ++v) {
+                    float w[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        w[c] = ex2(x[v][nt][c] - mx[c & 1]);
+                        sum[c & 1] += w[c];
+                    }
+                    pb[v][nt][0] = movmatrix_trans(pack2<false>(w[0], w[1]));
+                    pb[v][nt][1] = movmatrix_trans(pack2<false>(w[2], w[3]));
+                }
+                l_run[nt][0] = l_run[nt][0] * alpha[nt][0] + sum[0];
+                l_run[nt][1] = l_run[nt][1] * alpha[nt][1] + sum[1];
+            }
+            if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int k = 0; k < NG; ++k)
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) acc[k][c >> 2][nt][c & 3] *= alpha[nt][c & 1];
+                    if constexpr (RAW_V) {
+#pragma unroll
+                        for (int k = 0; k < NG; ++k)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) acc8[k][c] *= alpha[0][c & 1];
+                    }
+                }
+            }
+
+            // outputs
+#pragma unroll
+            for (int v = 0; v < TPI; ++v) {
+                if (v >= have) continue;
+                const int from = stages[v] * u.stage_bytes;
+                const uint32_t vtile = ring + from + code_bytes + warp * (16 * (D / 2));
+                const unsigned char* vs = smem + from + 2 * code_bytes + scale_bytes + h * NG;
+                uint32_t pair[2][NG];                    // scales of positions 2 t, 2 t + 1 and of 2 t + 8, 2 t + 9
+                scale_pairs<NG>(vs + 2 * t * row_scales, vs + (2 * t + 1) * row_scales, pair[0]);
+                scale_pairs<NG>(vs + (2 * t + 8) * row_scales, vs + (2 * t + 9) * row_scales, pair[1]);
+                if (SCALE_CODES && masked) {
+                    // A position that a query row does not take may have any scale, a NaN too: the scale becomes 0, and the
+                    // weights of the rows that do take the position a NaN.
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {
+                        uint32_t bad = 0u;
+#pragma unroll
+                        for (int k = 0; k < NG; ++k) {
+                            const uint32_t odd = __vcmpgeu2(pair[hf][k], 0x7c007c00u);
+                            pair[hf][k] &= ~odd, bad |= odd;
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) pb[v][nt][hf] |= nonzero2(pb[v][nt][hf]) & bad;
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < NG; k += 2) {
+                    uint32_t w[4];
+                    ldmatrix_x4_trans(w, vtile + chunk4<D>(lrow, k + lchunk));
+#pragma unroll
+                    for (int o = 0; o < 2; ++o) {
+                        // words of positions 0-7 and 8-15: values 4 g .. 4 g + 3 of the group
+                        uint32_t a1[4], a2[4];
+                        four_operands<RAW_V>(w[2 * o], w[2 * o + 1], a1, a2, 2, 1);
+                        if constexpr (SCALE_CODES) {
+                            // the scale over 8 (exact), so that the product stays in FP16's range; the state takes the 8 back
+                            const uint32_t s0 = hmul2_bits(pair[0][k + o], 0x30003000u), s1 = hmul2_bits(pair[1][k + o], 0x30003000u);
+                            a1[0] = hmul2_bits(a1[0], s0), a1[1] = hmul2_bits(a1[1], s0), a1[2] = hmul2_bits(a1[2], s1), a1[3] = hmul2_bits(a1[3], s1);
+                            a2[0] = hmul2_bits(a2[0], s0), a2[1] = hmul2_bits(a2[1], s0), a2[2] = hmul2_bits(a2[2], s1), a2[3] = hmul2_bits(a2[3], s1);
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            uint32_t b0 = pb[v][nt][0], b1 = pb[v][nt][1];
+                            if constexpr (!SCALE_CODES) {
+                                b0 = hmul2_bits(b0, pair[0][k + o]), b1 = hmul2_bits(b1, pair[1][k + o]);
+                                if (masked) b0 &= nonzero2(pb[v][nt][0]), b1 &= nonzero2(pb[v][nt][1]);
+                            }
+                            mma16816<false>(acc[k + o][0][nt], a1, b0, b1);
+                            mma16816<false>(acc[k + o][1][nt], a2, b0, b1);
+                            if constexpr (RAW_V) {
+                                const uint32_t eight[4] = {0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u};      // -8, and -8 * 16
+                                mma16816<false>(acc8[k + o], eight, b0, b1);
+                            }
+                        }
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(empty + stages[v] * 8) : "memory");
             }
         }
         if (dead) break;
 
-        // masks, online softmax
-        uint32_t pb[TPI][NT][2];
-        bool rescale = false;
-        float alpha[NT][2];
+        // -- the state, or the row's output ------------------------------------------------------------------------------------
+        bool whole, fits = true;
+        int64_t state0 = 0, state_row = 0, states = 0;          // an even launch: rows of states before this one's, their number
+        int prow0 = 0, split = 0;
+        if (u.blocks) {
+            whole = ntiles == at.tiles && !p.sinks;
+            states = ((int64_t)u.blocks + (int64_t)p.n_rows * HG * u.ctiles) * HB * ROWS;
+            state0 = ((int64_t)blockIdx.x + ((int64_t)r * HG + hg) * u.ctiles + ct) * HB * ROWS + warp * ROWS;
+        } else {
+            split = blockIdx.x;
+            whole = at.tiles <= (p.chunk >> 4) && !(p.flags & CRIT_B200_ATTEND_PARTIALS) && !p.sinks;     // (sinks join in the fold)
+            states = (int64_t)p.partial_rows * p.q_heads * p.max_splits;
+            prow0 = p.offsets ? p.offsets[r] - p.offsets[0] : r * p.columns;
+            fits = whole || (p.workspace && split < p.max_splits && prow0 >= 0 && prow0 + count <= p.partial_rows);
+            if (!fits && lane == 0 && p.status) atomicExch(p.status, CRIT_B200_STATUS_PLAN);
+        }
+        float* const space = p.workspace + (u.blocks ? (p.n_rows + 2 + 31) / 32 * 32 : 0);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-            for (int v = 0; v < TPI; ++v)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float y = x[v][nt][c] * mul[nt][c & 1];
-                    if (v >= have) y = -INFINITY;
-                    if (masked) {
-                        const int pos = ((tile0 + i + v) << 4) + g + 8 * (c >> 1), last = lastpos[nt][c & 1];
-                        if (pos > last) y = -INFINITY;
-                        if constexpr (MASKS) {
-                            if (p.sliding > 0 && pos <= last - p.sliding) y = -INFINITY;
-                            if (p.blocks && last >= 0) {
-                                const int32_t* listed = p.blocks + (int64_t)(start + (last - first32)) * p.blocks_k;
-                                const int block = pos / p.block_size;
-                                bool member = false;
-                                for (int j = 0; j < p.blocks_k; ++j) member |= listed[j] == block;
-                                if (!member) y = -INFINITY;
-                            }
-                            if (tree && pos >= first32 && (pos - first32 >= count || !((seen[nt][c & 1] >> (pos - first32)) & 1ull)))
-                                y = -INFINITY;
-                        }
-                    }
-                    x[v][nt][c] = y;
-                    mx[c & 1] = fmaxf(mx[c & 1], y);
-                }
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 4));
-                mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 8));
-                mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 16));
-                const bool moved = mx[j] > m_run[nt][j];
-                const float top = moved ? mx[j] + AHEAD : m_run[nt][j];
-                const float sub = top == -INFINITY ? 0.f : top;
-                alpha[nt][j] = moved ? ex2(m_run[nt][j] - sub) : 1.f;
-                rescale |= moved;
-                m_run[nt][j] = top;
-                mx[j] = sub;
-            }
-            float sum[2] = {0.f, 0.f};
+                float l = l_run[nt][j];
+                l += __shfl_xor_sync(0xffffffffu, l, 4);
+                l += __shfl_xor_sync(0xffffffffu, l, 8);
+                l += __shfl_xor_sync(0xffffffffu, l, 16);
+                const int row = nt * 8 + 2 * t + j, flat = ct * ROWS + row;
+                const int col = flat / G, gq = flat - col * G;
+                if (col >= count || !fits) continue;
+                const int token = start + col, head = h * G + gq;
+                const float inv = whole ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;          // (a NaN stays one)
+                auto value = [&](int k, int e) {                 // element 32 k + 4 g + e
+                    float o = acc[k][e >> 1][nt][(e & 1) * 2 + j];
+                    if constexpr (RAW_V) return (o + acc8[k][(e & 1) * 2 + j]) * ((e & 1 ? 0x1p20f : 0x1p24f) * inv);
+                    else return o * (SCALE_CODES ? 8.f * inv : inv);
+                };
+                if (whole) {
+                    char* dst = (char*)p.out + ((int64_t)token * p.out_stride_token + (int64_t)head * p.out_stride_head + 4 * g) * 2;
 #pragma unroll
-            for (int v = 0; v < TPI; ++v) {
-                float w[4];
+                    for (int k = 0; k < NG; ++k)
+                        *reinterpret_cast<uint2*>(dst + k * 64) = p.q_dtype == CRIT_B200_DTYPE_BF16
+                                                                      ? make_uint2(pack2<true>(value(k, 0), value(k, 1)), pack2<true>(value(k, 2), value(k, 3)))
+                                                                      : make_uint2(pack2<false>(value(k, 0), value(k, 1)), pack2<false>(value(k, 2), value(k, 3)));
+                    if (p.lse && g == 0) p.lse[(int64_t)token * p.q_heads + head] = l == 0.f ? -INFINITY : m_run[nt][j] * LN2 + logf(l);
+                } else {
+                    const int64_t where = u.blocks ? state0 + row : ((int64_t)(prow0 + col) * p.q_heads + head) * p.max_splits + split;
+                    float* dst = space + where * D + 4 * g;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    w[c] = ex2(x[v][nt][c] - mx[c & 1]);
-                    sum[c & 1] += w[c];
-                }
-                pb[v][nt][0] = movmatrix_trans(pack2<false>(w[0], w[1]));
-                pb[v][nt][1] = movmatrix_trans(pack2<false>(w[2], w[3]));
-            }
-            l_run[nt][0] = l_run[nt][0] * alpha[nt][0] + sum[0];
-            l_run[nt][1] = l_run[nt][1] * alpha[nt][1] + sum[1];
-        }
-        if (__any_sync(0xffffffffu, rescale)) {
-#pragma unroll
-            for (int k = 0; k < NG; ++k)
-#pragma unroll
-                for (int o = 0; o < 2; ++o)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        acc[k][o][nt][0] *= alpha[nt][0], acc[k][o][nt][1] *= alpha[nt][1];
-                        acc[k][o][nt][2] *= alpha[nt][0], acc[k][o][nt][3] *= alpha[nt][1];
-                    }
-        }
-
-        // outputs
-#pragma unroll
-        for (int v = 0; v < TPI; ++v) {
-            if (v >= have) continue;
-            const uint32_t vtile = base[v] + code_bytes + warp * (16 * (D / 2));
-            const unsigned char* vs = smem + (base[v] - smem_addr(smem)) + 2 * code_bytes + scale_bytes + h * NG;
-            uint32_t keep[NT][2];                     // where a position is masked its scale may be anything, a NaN too
-            if (masked) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) keep[nt][0] = nonzero2(pb[v][nt][0]), keep[nt][1] = nonzero2(pb[v][nt][1]);
-            }
-#pragma unroll
-            for (int k = 0; k < NG; k += 2) {
-                uint32_t w[4];
-                ldmatrix_x4_trans(w, vtile + chunk4<D>(lrow, k + lchunk));
-                // the scales of positions 2 t, 2 t + 1 and 2 t + 8, 2 t + 9, groups k and k + 1
-                uint32_t pair[2][2];
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const uint32_t a = *reinterpret_cast<const uint16_t*>(vs + (2 * t + 8 * hf) * row_scales + k);
-                    const uint32_t b = *reinterpret_cast<const uint16_t*>(vs + (2 * t + 1 + 8 * hf) * row_scales + k);
-                    scale_pairs(a | (b << 16), pair[0][hf], pair[1][hf]);
-                }
-#pragma unroll
-                for (int o = 0; o < 2; ++o) {
-                    const uint32_t lo = w[2 * o], hi = w[2 * o + 1];            // positions 0-7 and 8-15, values 4 g .. 4 g + 3
-                    const uint32_t a1[4] = {codes_low(lo), codes_high(lo), codes_low(hi), codes_high(hi)};
-                    const uint32_t a2[4] = {codes_low(lo >> 8), codes_high(lo >> 8), codes_low(hi >> 8), codes_high(hi >> 8)};
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        uint32_t b0 = hmul2_bits(pb[v][nt][0], pair[o][0]), b1 = hmul2_bits(pb[v][nt][1], pair[o][1]);
-                        if (masked) b0 &= keep[nt][0], b1 &= keep[nt][1];
-                        mma16816<false>(acc[k + o][0][nt], a1, b0, b1);
-                        mma16816<false>(acc[k + o][1][nt], a2, b0, b1);
+                    for (int k = 0; k < NG; ++k) *reinterpret_cast<float4*>(dst + k * 32) = make_float4(value(k, 0), value(k, 1), value(k, 2), value(k, 3));
+                    if (g == 0) {
+                        space[states * D + where] = m_run[nt][j];
+                        space[states * (D + 1) + where] = l;
                     }
                 }
             }
-            __syncwarp();
-            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(empty + stages[v] * 8) : "memory");
-        }
+        step_to(at, ntiles);
     }
-    if (__syncthreads_or(dead ? 1 : 0)) return;
+    if (outside && p.status) atomicExch(p.status, CRIT_B200_STATUS_BOUNDS);
+    if (__syncthreads_or(dead ? 1 : 0) && threadIdx.x == 0) {
+        // a copy or a reader never came: the copies in flight get a last bounded chance to land
+        for (int s = 0; s < u.stages; ++s) mbar_wait(full + s * 8, 0, 1000000ull), mbar_wait(full + s * 8, 1, 1000000ull);
+        if (p.status) atomicExch(p.status, CRIT_B200_STATUS_TMA);
+    }
+}
 
-    // -- the state, or the row's output --------------------------------------------------------------------------------------
-    const bool whole = nsplit == 1 && !(p.flags & CRIT_B200_ATTEND_PARTIALS) && !p.sinks;     // (sinks join in the fold)
-    const int64_t states = (int64_t)p.partial_rows * p.q_heads * p.max_splits;
-    const int prow0 = p.offsets ? p.offsets[r] - p.offsets[0] : r * p.columns;
-    const bool fits = whole || (p.workspace && split < p.max_splits && prow0 >= 0 && prow0 + count <= p.partial_rows);
-    if (!fits) {
-        if (lane == 0 && p.status) atomicExch(p.status, CRIT_B200_STATUS_PLAN);
-        return;
+// The fold of an even launch: a row's states are consecutive slots.  WARPS warps serve a (window token, query head), warp w the
+// slots w, w + WARPS, ..; first the slots' maximum, then sums with weights that are fixed by then, added in warp order.
+template <int D, int WARPS>
+__global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) merge4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const int rows_tile) {
+    constexpr int PER = D / 32;
+    __shared__ float part_l[WARPS], part_o[WARPS > 1 ? WARPS : 1][WARPS > 1 ? D : 1];
+    const int lane = threadIdx.x & 31, warp = WARPS == 1 ? 0 : threadIdx.x >> 5;
+    const int64_t item = WARPS == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+    if (item >= (int64_t)p.n_rows * p.columns * p.q_heads) return;
+    const int head = (int)(item % p.q_heads), rc = (int)(item / p.q_heads);
+    const int r = rc / p.columns, col = rc - r * p.columns;
+    const int* info = reinterpret_cast<const int*>(p.workspace);
+    const int run = info[0], first = info[1 + r];
+    const int count = row_count4(p, r), start = p.starts[r];
+    const int tiles = row_tiles4(p, r, count);
+    if (col >= count) return;
+    const int G = p.q_heads / p.kv_heads, HB = u.heads, HG = p.kv_heads / HB;
+    const int h = head / G, hg = h / HB, flat = col * G + head - h * G, ct = flat / rows_tile;
+    const int ctiles = (count * G + rows_tile - 1) / rows_tile;
+    int lo = 0, n = 0;
+    if (tiles > 0) {
+        const int begin = first + (hg * ctiles + ct) * tiles;
+        lo = begin / run, n = (begin + tiles - 1) / run - lo + 1;
+        if (n == 1 && !p.sinks) return;                              // written by the first launch
     }
+    const float* space = p.workspace + (p.n_rows + 2 + 31) / 32 * 32;
+    const int64_t slots = (int64_t)u.blocks + (int64_t)p.n_rows * HG * u.ctiles, per = (int64_t)HB * rows_tile;
+    const int64_t state0 = ((int64_t)lo + ((int64_t)r * HG + hg) * u.ctiles + ct) * per + (int64_t)(h - hg * HB) * rows_tile + (flat - ct * rows_tile);
+    const float* pm = space + slots * per * D;
+    const float* pl = pm + slots * per;
+    float top = -INFINITY;
+    for (int s = lane; s < n; s += 32) top = fmaxf(top, pm[state0 + s * per]);
+    top = warp_max(top);
+    const float sub = top == -INFINITY ? 0.f : top;
+    float total = 0.f, acc[PER];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+#pragma unroll 4
+    for (int s = warp; s < n; s += WARPS) {
+        const int64_t where = state0 + s * per;
+        const float w = ex2(pm[where] - sub);
+        total += pl[where] * w;
+        const float* o = space + where * D + lane * PER;
+        float v[PER];
+        if constexpr (PER == 2) {
+            const float2 a = *reinterpret_cast<const float2*>(o);
+            v[0] = a.x, v[1] = a.y;
+        } else {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            float l = l_run[nt][j];
-            l += __shfl_xor_sync(0xffffffffu, l, 4);
-            l += __shfl_xor_sync(0xffffffffu, l, 8);
-            l += __shfl_xor_sync(0xffffffffu, l, 16);
-            const int flat = ct * ROWS + nt * 8 + 2 * t + j;
-            const int col = flat / G, gq = flat - col * G;
-            if (col >= count) continue;
-            const int token = start + col, head = h * G + gq;
-            if (whole) {
-                const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);          // (a NaN stays one)
-                char* dst = (char*)p.out + ((int64_t)token * p.out_stride_token + (int64_t)head * p.out_stride_head + 4 * g) * 2;
-#pragma unroll
-                for (int k = 0; k < NG; ++k) {
-                    const float o0 = acc[k][0][nt][j] * inv, o1 = acc[k][0][nt][2 + j] * inv, o2 = acc[k][1][nt][j] * inv, o3 = acc[k][1][nt][2 + j] * inv;
-                    *reinterpret_cast<uint2*>(dst + k * 64) =
-                        p.q_dtype == CRIT_B200_DTYPE_BF16 ? make_uint2(pack2<true>(o0, o1), pack2<true>(o2, o3)) : make_uint2(pack2<false>(o0, o1), pack2<false>(o2, o3));
-                }
-                if (p.lse && g == 0) p.lse[(int64_t)token * p.q_heads + head] = l == 0.f ? -INFINITY : m_run[nt][j] * LN2 + logf(l);
-            } else {
-                const int64_t at = ((int64_t)(prow0 + col) * p.q_heads + head) * p.max_splits + split;
-                float* dst = p.workspace + at * D + 4 * g;
-#pragma unroll
-                for (int k = 0; k < NG; ++k)
-                    *reinterpret_cast<float4*>(dst + k * 32) = make_float4(acc[k][0][nt][j], acc[k][0][nt][2 + j], acc[k][1][nt][j], acc[k][1][nt][2 + j]);
-                if (g == 0) {
-                    p.workspace[states * D + at] = m_run[nt][j];
-                    p.workspace[states * (D + 1) + at] = l;
-                }
+            for (int i = 0; i < PER; i += 4) {
+                const float4 a = *reinterpret_cast<const float4*>(o + i);
+                v[i] = a.x, v[i + 1] = a.y, v[i + 2] = a.z, v[i + 3] = a.w;
             }
         }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) acc[i] = fmaf(v[i], w, acc[i]);
+    }
+    if constexpr (WARPS > 1) {
+        if (lane == 0) part_l[warp] = total;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) part_o[warp][lane * PER + i] = acc[i];
+        __syncthreads();
+        if (warp) return;
+        total = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) total += part_l[w];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            acc[i] = 0.f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) acc[i] += part_o[w][lane * PER + i];
+        }
+    }
+    float shrink = 1.f;                     // the head's sink, last: one position more without a value
+    if (p.sinks) sink_fold(p.sinks[head], top, total, shrink);
+    const float inv = total > 0.f ? shrink / total : (total == 0.f ? 0.f : total);         // (a NaN stays one)
+    const int64_t to = (int64_t)(start + col) * p.out_stride_token + (int64_t)head * p.out_stride_head + lane * PER;
+#pragma unroll
+    for (int i = 0; i < PER; i += 2)
+        *reinterpret_cast<uint32_t*>((char*)p.out + (to + i) * 2) =
+            p.q_dtype == CRIT_B200_DTYPE_BF16 ? pack2<true>(acc[i] * inv, acc[i + 1] * inv) : pack2<false>(acc[i] * inv, acc[i + 1] * inv);
+    if (p.lse && lane == 0) p.lse[(int64_t)(start + col) * p.q_heads + head] = total == 0.f ? -INFINITY : top * LN2 + logf(total);
 }
 
 // -- host side --------------------------------------------------------------------------------------------------------------
 typedef void (*decode4_fn)(const crit_b200_attend_params, const Decode4Launch, const CUtensorMap, const CUtensorMap);
 
 template <int D, int NT>
-static decode4_fn decode4_of(bool masks) {
-    if (masks) return decode4_kernel<D, NT, true>;
-    return decode4_kernel<D, NT, false>;
+static decode4_fn decode4_of(bool masks, bool fast) {
+    if constexpr (NT <= 2)
+        if (fast) return masks ? decode4_kernel<D, NT, true, true> : decode4_kernel<D, NT, false, true>;
+    return masks ? decode4_kernel<D, NT, true, false> : decode4_kernel<D, NT, false, false>;
 }
 
-static decode4_fn decode4_pick(int d, int nt, bool masks) {
+static decode4_fn decode4_pick(int d, int nt, bool masks, bool fast) {
     switch (d) {
-        case 64: return nt == 1 ? decode4_of<64, 1>(masks) : (nt == 2 ? decode4_of<64, 2>(masks) : decode4_of<64, 4>(masks));
-        case 128: return nt == 1 ? decode4_of<128, 1>(masks) : (nt == 2 ? decode4_of<128, 2>(masks) : decode4_of<128, 4>(masks));
-        case 256: return nt == 1 ? decode4_of<256, 1>(masks) : decode4_of<256, 2>(masks);
+        case 64: return nt == 1 ? decode4_of<64, 1>(masks, fast) : (nt == 2 ? decode4_of<64, 2>(masks, fast) : decode4_of<64, 4>(masks, fast));
+        case 128: return nt == 1 ? decode4_of<128, 1>(masks, fast) : (nt == 2 ? decode4_of<128, 2>(masks, fast) : decode4_of<128, 4>(masks, fast));
+        case 256: return nt == 1 ? decode4_of<256, 1>(masks, fast) : decode4_of<256, 2>(masks, fast);
         default: return nullptr;
     }
 }
 
-static int heads_of(int kv_heads, int most) {
-    int heads = most;
-    while (kv_heads % heads) heads >>= 1;
-    return heads;
+struct Decode4Plan {
+    decode4_fn fn;
+    Decode4Launch u;
+    int nt, smem, sms, per_sm;
+};
+
+// Blocks of a kernel an SM of the current device holds, remembered per kernel, block, shared memory and device.
+static int resident4(const void* fn, int threads, int smem, int* sms) {
+    struct Entry { const void* fn; int threads, smem, device, per_sm, sms; };
+    static Entry seen[256];
+    static int n = 0;
+    static std::mutex guard;
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return 0;
+    std::lock_guard<std::mutex> lock(guard);
+    for (int i = 0; i < n; ++i)
+        if (seen[i].fn == fn && seen[i].threads == threads && seen[i].smem == smem && seen[i].device == device) {
+            *sms = seen[i].sms;
+            return seen[i].per_sm;
+        }
+    int per_sm = 0;
+    if (cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
+        cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, fn, threads, smem) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    if (n < 256) seen[n++] = Entry{fn, threads, smem, device, per_sm, *sms};
+    return per_sm;
 }
 
-// The launch of a geometry: query-row tiles, heads a block takes, stages that two blocks' shares of an SM hold.
-static int decode4_shape(int q_heads, int kv_heads, int d, int columns, int* nt, Decode4Launch* u, int* smem) {
+// The launch of a geometry: kernel, heads a block takes, stages that the blocks' shares of an SM hold, blocks of an even launch.
+static int plan4(int q_heads, int kv_heads, int d, int columns, int n_rows, bool masks, bool fp16, bool even, Decode4Plan* out) {
     if (d != 64 && d != 128 && d != 256) return CRIT_B200_EUNSUPPORTED;
     const int rows = columns * (q_heads / kv_heads);
-    *nt = rows <= 8 ? 1 : (rows <= 16 || d == 256 ? 2 : 4);
-    u->heads = heads_of(kv_heads, decode4_heads(d, *nt));
-    u->ctiles = (rows + 8 * *nt - 1) / (8 * *nt);
-    u->stage_bytes = (u->heads * 16 * d + 2 * 16 * kv_heads * (d / 32) + 1023) / 1024 * 1024;
-    const int want = 16 * 1024 * u->heads;                                    // in flight a block: 128 KB for 8 heads
-    const int room = 110 * 1024;
-    int stages = (want < room ? want : room) / u->stage_bytes;
-    u->stages = stages < 2 ? 2 : (stages > D4_MAX_STAGES ? D4_MAX_STAGES : stages);
-    *smem = 1024 + u->stages * u->stage_bytes;
-    return *smem > 226 * 1024 ? CRIT_B200_EUNSUPPORTED : 0;
+    const int nt = rows <= 8 ? 1 : (rows <= 16 || d == 256 ? 2 : 4);
+    Decode4Launch& u = out->u;
+    u.heads = decode4_heads(d, nt);
+    while (kv_heads % u.heads) u.heads >>= 1;
+    u.ctiles = (rows + 8 * nt - 1) / (8 * nt);
+    u.stage_bytes = (u.heads * 16 * d + 2 * 16 * kv_heads * (d / 32) + 1023) / 1024 * 1024;
+    const int blocks = decode4_blocks(d, nt) * decode4_heads(d, nt) / u.heads;           // (the registers hold as many)
+    const int room = (228 * 1024) / blocks - 1024 - 1024 - 4096;                          // (alignment, the driver's, the row lists)
+    const int stages = room / u.stage_bytes;
+    u.stages = stages < 4 ? 4 : (stages > D4_MAX_STAGES ? D4_MAX_STAGES : stages);
+    out->nt = nt, out->smem = 1024 + u.stages * u.stage_bytes;
+    if (out->smem > 220 * 1024) return CRIT_B200_EUNSUPPORTED;
+    out->fn = decode4_pick(d, nt, masks, even && (nt > 1 || !fp16));
+    u.blocks = 0, out->sms = out->per_sm = 0;
+    if (even) {
+        out->per_sm = resident4((const void*)out->fn, 32 * u.heads, out->smem, &out->sms);
+        if (out->per_sm < 1 || n_rows > D4_MAX_ROWS) return CRIT_B200_EUNSUPPORTED;
+        u.blocks = out->sms * out->per_sm;
+    }
+    return 0;
+}
+
+static int plan4(const crit_b200_attend_params& p, Decode4Plan* out) {
+    const bool even = (p.flags & CRIT_B200_ATTEND_EVEN) != 0;
+    if (even && (p.flags & CRIT_B200_ATTEND_PARTIALS)) return CRIT_B200_EUNSUPPORTED;
+    return plan4(p.q_heads, p.kv_heads, p.head_dim, p.columns, p.n_rows, p.parents || p.sliding > 0 || p.blocks,
+                 p.q_dtype == CRIT_B200_DTYPE_FP16, even, out);
+}
+
+// Floats of an even launch's workspace: where the rows begin, and (dim + 2) a state row.
+int64_t even_floats4(const crit_b200_attend_params& p) {
+    Decode4Plan plan;
+    if (p.kind != CRIT_B200_KIND_INT4 || p.head_dim != p.value_dim) return CRIT_B200_EUNSUPPORTED;
+    if (int e = plan4(p, &plan)) return e;
+    const int64_t slots = (int64_t)plan.u.blocks + (int64_t)p.n_rows * (p.kv_heads / plan.u.heads) * plan.u.ctiles;
+    return (p.n_rows + 2 + 31) / 32 * 32 + slots * plan.u.heads * 8 * plan.nt * (p.head_dim + 2);
 }
 
 int launch_decode4(const crit_b200_attend_params& p, cudaStream_t s) {
     if (p.flags & (CRIT_B200_ATTEND_TCGEN05 | CRIT_B200_ATTEND_TCGEN05P | CRIT_B200_ATTEND_TCGEN05T)) return CRIT_B200_EUNSUPPORTED;
     if (p.head_dim != p.value_dim || p.slots < 16 || p.slots > 0x7fffffffLL || p.slots < p.page) return CRIT_B200_EUNSUPPORTED;
     if (!aligned(p.key_scales, 16) || !aligned(p.value_scales, 16)) return CRIT_B200_EALIGN;
-    int nt = 0, smem = 0;
-    Decode4Launch u;
-    if (int e = decode4_shape(p.q_heads, p.kv_heads, p.head_dim, p.columns, &nt, &u, &smem)) return e;
+    Decode4Plan plan;
+    if (int e = plan4(p, &plan)) return e;
+    const Decode4Launch& u = plan.u;
     CUtensorMap kmap, vmap;
     if (!rows4_map(&kmap, p.key_pages, p.head_dim, p.kv_heads, u.heads, p.slots) ||
         !rows4_map(&vmap, p.value_pages, p.head_dim, p.kv_heads, u.heads, p.slots))
         return CRIT_B200_EUNSUPPORTED;
-    const decode4_fn fn = decode4_pick(p.head_dim, nt, p.parents || p.sliding > 0 || p.blocks);
-    cudaError_t ce = cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t ce = cudaFuncSetAttribute((const void*)plan.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, plan.smem);
     if (ce != cudaSuccess) return (int)ce;
     const int64_t hg = p.kv_heads / u.heads;
     if (hg * u.ctiles > 65535 || p.n_rows > 65535) return CRIT_B200_EUNSUPPORTED;
-    dim3 grid((unsigned)p.max_splits, (unsigned)(hg * u.ctiles), (unsigned)p.n_rows);
-    fn<<<grid, 32 * (u.heads + 1), smem, s>>>(p, u, kmap, vmap);
+    const dim3 grid = u.blocks ? dim3((unsigned)u.blocks) : dim3((unsigned)p.max_splits, (unsigned)(hg * u.ctiles), (unsigned)p.n_rows);
+    plan.fn<<<grid, 32 * u.heads, plan.smem, s>>>(p, u, kmap, vmap);
+    CRIT_CHECK_LAUNCH();
+    return 0;
+}
+
+template <int D>
+static void launch_merge4_of(const crit_b200_attend_params& p, const Decode4Plan& plan, bool many, cudaStream_t s) {
+    const int64_t items = (int64_t)p.n_rows * p.columns * p.q_heads;
+    if (many) merge4_kernel<D, 8><<<(unsigned)items, 256, 0, s>>>(p, plan.u, 8 * plan.nt);
+    else merge4_kernel<D, 1><<<(unsigned)((items + 3) / 4), 128, 0, s>>>(p, plan.u, 8 * plan.nt);
+}
+
+int launch_merge4(const crit_b200_attend_params& p, cudaStream_t s) {
+    Decode4Plan plan;
+    if (int e = plan4(p, &plan)) return e;
+    // few rows share the blocks: a row may have a state in each, so a block folds it; many rows have a few states each
+    const bool many = (int64_t)p.n_rows * (p.kv_heads / plan.u.heads) * plan.u.ctiles * 16 < plan.u.blocks;
+    switch (p.head_dim) {
+        case 64: launch_merge4_of<64>(p, plan, many, s); break;
+        case 128: launch_merge4_of<128>(p, plan, many, s); break;
+        case 256: launch_merge4_of<256>(p, plan, many, s); break;
+        default: return CRIT_B200_EUNSUPPORTED;
+    }
     CRIT_CHECK_LAUNCH();
     return 0;
 }
 
 int plan_decode4(int q_heads, int kv_heads, int d, int columns, int32_t* out5) {
-    int nt = 0, smem = 0, device = 0, sms = 0, per_sm = 0;
-    Decode4Launch u;
-    if (int e = decode4_shape(q_heads, kv_heads, d, columns, &nt, &u, &smem)) return e;
-    const decode4_fn fn = decode4_pick(d, nt, false);
-    if (cudaGetDevice(&device) == cudaSuccess) {
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-        if (cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess)
-            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, (const void*)fn, 32 * (u.heads + 1), smem);
-    }
-    cudaGetLastError();
-    out5[0] = 1024, out5[1] = smem, out5[2] = 8 * nt, out5[3] = per_sm, out5[4] = sms;
+    Decode4Plan plan;
+    if (int e = plan4(q_heads, kv_heads, d, columns, 1, false, false, false, &plan)) return e;
+    int sms = 0;
+    const int per_sm = resident4((const void*)plan.fn, 32 * plan.u.heads, plan.smem, &sms);
+    out5[0] = 1024, out5[1] = plan.smem, out5[2] = 8 * plan.nt, out5[3] = per_sm, out5[4] = sms;
     return 0;
 }
 

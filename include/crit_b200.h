@@ -236,6 +236,10 @@ int crit_b200_compact_blocks(const crit_b200_compact_params* params, void* strea
                                         part of a prompt chunk's attention that reads the pages, when the chunk's own keys
                                         and values are read fresh from elsewhere and the two parts merged by their lse);
                                         the m16n8k16 kernel's; both launches (decode and merge) carry the flag */
+#define CRIT_B200_ATTEND_EVEN 512    /* kind 5: the launch's tiles are dealt out in equal runs to the blocks the device holds at once
+                                        (a column's bits then depend on the launch), at most 256 rows; a workspace of
+                                        crit_b200_attend_floats floats in a layout of its own (max_splits, partial_rows and offsets
+                                        are not read); both launches carry the flag */
 #define CRIT_B200_ATTEND_PARTIALS 32 /* every row's split states go to the workspace, a row of one split too (the first launch
                                         writes nothing to out / lse): what crit_b200_merge_push sends, or what
                                         crit_b200_merge folds */
@@ -298,6 +302,10 @@ typedef struct crit_b200_attend_params {
  * workspace_floats (paged_kv_attention/__init__.py:359-362).  Returns 0, or CRIT_B200_EUNSUPPORTED. */
 int crit_b200_attend_plan(int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t value_dim, int32_t page,
                           int32_t kind, int32_t page_dtype, int32_t columns, int32_t* out5);
+
+/* The floats of workspace a launch of these parameters takes on the current device (the pointers are not read), or a
+ * negative CRIT_B200_E* code. */
+int64_t crit_b200_attend_floats(const crit_b200_attend_params* params);
 
 int crit_b200_decode(const crit_b200_attend_params* params, void* stream);   /* the splits' partials */
 int crit_b200_merge(const crit_b200_attend_params* params, void* stream);    /* the fold in split order */

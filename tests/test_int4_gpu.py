@@ -176,7 +176,7 @@ def test_windows_of_every_geometry(hq, hkv, dim, page, before, columns, dtype):
     rows = list(range(len(before)))
     q = _queries(len(before) * columns, hq, dim, dtype, 12)
     starts = [r * columns for r in rows]
-    for kw in ({}, {"chunk": 64}):
+    for kw in ({"engine": "mma.sync"}, {"chunk": 64}, {"engine": "even"}):
         out, lse = _attend(cache, q, rows, starts, before, columns, **kw)
         _check(cache, q, out, lse, rows, starts, before, [columns] * len(rows))
 
@@ -186,11 +186,12 @@ def test_ragged_windows_leave_other_tokens_alone():
     cache = Cache4.filled(8, 128, 16, [n + 4 for n in before], seed=21, poison=True)
     q = _queries(14, 32, 128, torch.bfloat16, 22)
     starts = [0, 4, 5, 9]
-    out, lse = _attend(cache, q, range(4), starts, before, 4, counts, chunk=32)
-    _check(cache, q, out, lse, range(4), starts, before, counts)
-    named = {s + c for s, n in zip(starts, counts) for c in range(n)}
-    for token in set(range(14)) - named:
-        assert out[token].isnan().all() and lse[token].isnan().all()
+    for kw in ({"chunk": 32}, {}):
+        out, lse = _attend(cache, q, range(4), starts, before, 4, counts, **kw)
+        _check(cache, q, out, lse, range(4), starts, before, counts)
+        named = {s + c for s, n in zip(starts, counts) for c in range(n)}
+        for token in set(range(14)) - named:
+            assert out[token].isnan().all() and lse[token].isnan().all()
 
 
 @pytest.mark.parametrize("chunk", [None, 48])
@@ -209,14 +210,15 @@ def test_trees_sliding_windows_sinks_lists_and_context_rows(chunk):
         _check(cache, q, out, lse, [0, 1], starts, before, counts, **masks)
 
 
-def test_a_row_that_sees_nothing_gets_zeros():
+@pytest.mark.parametrize("engine", ["even", "mma.sync"])
+def test_a_row_that_sees_nothing_gets_zeros(engine):
     cache = Cache4.filled(8, 128, 16, [40, 40], seed=41)
     q = _queries(4, 8, 128, torch.bfloat16, 42)
-    out, lse = _attend(cache, q, [0, 1], [0, 2], [0, 30], 2, context=True)          # a context row with nothing before it
+    out, lse = _attend(cache, q, [0, 1], [0, 2], [0, 30], 2, context=True, engine=engine)          # a context row with nothing before it
     assert (out[:2] == 0).all() and (lse[:2] == -float("inf")).all()
     _check(cache, q, out, lse, [1], [2], [30], [2], context=True)
     blocks = torch.full((4, 2), -1, dtype=torch.int32, device="cuda")
-    out, lse = _attend(cache, q, [0, 1], [0, 2], [10, 30], 2, blocks=blocks, block_size=24)
+    out, lse = _attend(cache, q, [0, 1], [0, 2], [10, 30], 2, blocks=blocks, block_size=24, engine=engine)
     assert (out == 0).all() and (lse == -float("inf")).all()
 
 
@@ -252,19 +254,27 @@ def test_far_magnitudes_and_flat_long_rows():
         _check(cache, q, out, lse, [0], [0], [n - 1], [1], scale=gap / 8)
 
 
-def test_rows_with_a_nan_are_not_spread():
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("engine", ["even", "mma.sync"])
+def test_rows_with_a_nan_are_not_spread(engine, dtype):
     cache = Cache4.filled(2, 128, 16, [64, 64], seed=71)
     bad = torch.full((1, 2, 128), float("nan"), dtype=torch.bfloat16, device="cuda")
     cache.write(0, 60, bad, bad)
-    q = _queries(2, 8, 128, torch.bfloat16, 72)
-    out, lse = _attend(cache, q, [0, 1], [0, 1], [59, 63], 1)                    # row 0 ends before the NaN
+    q = _queries(2, 8, 128, dtype, 72)
+    out, lse = _attend(cache, q, [0, 1], [0, 1], [59, 63], 1, engine=engine)     # row 0 ends before the NaN
     _check(cache, q, out, lse, [0, 1], [0, 1], [59, 63], [1, 1])
-    out, lse = _attend(cache, q, [0, 1], [0, 1], [63, 63], 1)
+    out, lse = _attend(cache, q, [0, 1], [0, 1], [63, 63], 1, engine=engine)
     assert out[0].isnan().all() and lse[0].isnan().all()
     _check(cache, q, out, lse, [1], [1], [63], [1])
     parents = torch.tensor([-1, -1], device="cuda")                              # a sibling branch holds the NaN
-    out, lse = _attend(cache, _queries(2, 8, 128, torch.bfloat16, 73), [0], [0], [60], 2, parents=parents)
+    out, lse = _attend(cache, _queries(2, 8, 128, dtype, 73), [0], [0], [60], 2, parents=parents, engine=engine)
     assert out[0].isnan().all() and out[1].isfinite().all()
+    only_v = torch.ones(1, 2, 128, dtype=torch.bfloat16, device="cuda")          # a NaN among the values alone, in a chain's last column
+    cache.write(1, 61, only_v, bad)
+    q = _queries(6, 32, 128, dtype, 74)                                          # (several columns of query rows a tile)
+    out, lse = _attend(cache, q, [1], [0], [56], 6, engine=engine)
+    _check(cache, q, out[:5], lse[:5], [1], [0], [56], [5])
+    assert out[5].isnan().all()
 
 
 def test_bad_page_ids_and_plans_are_reported_and_skipped():
@@ -286,7 +296,40 @@ def test_bad_page_ids_and_plans_are_reported_and_skipped():
     pk._status[str(q.device)].copy_(before)
 
 
-def test_a_captured_step_replays():
+def test_many_rows_share_the_blocks_evenly():
+    """More rows than a list holds fall back to splits; rows of very different lengths, empty ones among them, in one launch."""
+    g = torch.Generator().manual_seed(201)
+    lengths = [int(x) for x in torch.randint(1, 90, (40,), generator=g)] + [900, 1, 16, 17]
+    counts = [1] * 44
+    counts[0] = counts[7] = counts[43] = 0
+    cache = Cache4.filled(8, 128, 16, lengths, seed=202, poison=True)
+    q = _queries(44, 16, 128, torch.bfloat16, 203)
+    firsts = [n - 1 for n in lengths]
+    out, lse = _attend(cache, q, range(44), range(44), firsts, 1, counts)
+    _check(cache, q, out, lse, range(44), range(44), firsts, counts)
+    again, _ = _attend(cache, q, range(44), range(44), firsts, 1, counts)
+    assert torch.equal(out[1:7], again[1:7])
+    many = 300
+    q = _queries(many, 8, 128, torch.bfloat16, 204)
+    rows = [r % 40 for r in range(many)]
+    out, lse = _attend(cache, q, rows, range(many), [firsts[r] for r in rows], 1)
+    picked = [0, 1, 150, 299]
+    _check(cache, q, out, lse, [rows[r] for r in picked], picked, [firsts[rows[r]] for r in picked], [1] * 4)
+    with pytest.raises(ValueError, match="no kernel"):
+        _attend(cache, q, rows, range(many), [firsts[r] for r in rows], 1, engine="even")
+
+
+@pytest.mark.parametrize("hq,hkv,dim,columns", [(8, 4, 256, 1), (40, 8, 128, 6), (16, 2, 128, 1)])
+def test_one_long_row_over_every_block(hq, hkv, dim, columns):
+    n = 9000
+    cache = Cache4.filled(hkv, dim, 64, [n + columns], seed=211)
+    q = _queries(columns, hq, dim, torch.bfloat16, 212)
+    out, lse = _attend(cache, q, [0], [0], [n], columns)
+    _check(cache, q, out, lse, [0], [0], [n], [columns])
+
+
+@pytest.mark.parametrize("engine", ["even", "mma.sync"])
+def test_a_captured_step_replays(engine):
     """write, then attend, captured and replayed over new lengths and new tokens, on a stream of its own."""
     cache = Cache4.filled(8, 128, 16, [50, 120], seed=91, spare=8)
     keys, values = _queries(2, 8, 128, torch.bfloat16, 92), _queries(2, 8, 128, torch.bfloat16, 93)
@@ -299,7 +342,7 @@ def test_a_captured_step_replays():
     def step():
         pk.write(keys, values, slots, cache.k, cache.v, "int4", cache.ks, cache.vs)
         pk.attend(q, cache.k, cache.v, "int4", cache.tables, rows, starts, firsts, 1, 16, key_scales=cache.ks, value_scales=cache.vs,
-                  out=out, lse=lse, chunk=64)
+                  out=out, lse=lse, engine=engine)
     place = lambda p: torch.cat([cache.slots(0, torch.tensor([p[0]])), cache.slots(1, torch.tensor([p[1]]))])
     slots.copy_(place([50, 120]))
     stream = torch.cuda.Stream()
@@ -489,6 +532,12 @@ def test_what_the_entry_points_refuse():
         _attend_with(cache, q, key_scales=cache.ks.float())
     with pytest.raises(ValueError):
         _attend_with(cache, q.float())
+    with pytest.raises(ValueError, match="workspace"):
+        _attend_with(cache, q, engine="even", workspace=torch.empty(100, device="cuda"))
+    with pytest.raises(NotImplementedError, match="int4"):
+        pages = torch.zeros(4, 16, 8, 128, dtype=torch.bfloat16, device="cuda")
+        i32 = torch.zeros(1, dtype=torch.int32, device="cuda")
+        pk.attend(q, pages, pages, "bf16", cache.tables, i32, i32, torch.tensor([5], device="cuda"), 1, 16, engine="even")
     for engine in ("tcgen05", "tcgen05p", "tcgen05t"):
         with pytest.raises(ValueError, match="no kernel"):
             _attend_with(cache, q, engine=engine)
