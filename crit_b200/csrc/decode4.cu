@@ -22,8 +22,8 @@
 // the tensor cores take them as they are), the nibbles 1 and 5 under 0x00f000f0 are 16 n * 2^-24: one AND makes two operands,
 // where 1024 + n less 1032 takes an OR and an add more.  The factor 16 is undone in the queries (their odd elements are
 // divided by 16) and in the outputs' odd columns, 2^-24 in a constant.  The 8 that a code stands above its value comes off in
-// the accumulators: K Q^T starts from -8 * the sum of the group's queries, and a product of a constant matrix with P^T
-// gathers -8 * the sum of the group's weights.  Where the accumulators for that do not fit the registers (wide tiles of query
+// products of their own: the positions' scales with -8 * the sums of the groups' queries (a K of the groups' number, the sums
+// as two FP16 terms), and a constant matrix with P^T, which gathers -8 * the sum of the group's weights.  Where the accumulators for that do not fit the registers (wide tiles of query
 // rows, the outputs of 256-wide heads), codes become n - 8 one add later.
 //
 // The queries become FP16 with an exponent of their own a row (the largest element between 2^13 and 2^14), so no bf16 query
@@ -37,6 +37,7 @@
 // once; where a run and a row overlap there is one state, slot = block + row (both only grow along the tiles, so the sum
 // names the pair), and merge4_kernel folds a row's consecutive slots.  No block idles while another has two splits to go.
 #include <mutex>
+#include <type_traits>
 
 #include "int4.cuh"
 #include "tensor_map.cuh"
@@ -88,18 +89,39 @@ __device__ __forceinline__ uint32_t hmul2_bits(uint32_t a, uint32_t b) {
     __half2 h = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
     return *reinterpret_cast<uint32_t*>(&h);
 }
+// D = A * B.
+__device__ __forceinline__ void mma16816_new(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 // all ones in the halves that are not zero
 __device__ __forceinline__ uint32_t nonzero2(uint32_t a) { return __hne2_mask(*reinterpret_cast<__half2*>(&a), __floats2half2_rn(0.f, 0.f)); }
 
+__device__ __forceinline__ uint32_t shared_u32(uint32_t at) {
+    uint32_t x;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(at) : "memory");
+    return x;
+}
+__device__ __forceinline__ uint32_t shared_u16(uint32_t at) {
+    uint16_t x;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(at) : "memory");
+    return x;
+}
+// Lane 0 tells a barrier that the warp is done with a stage (a predicate, no branch).
+__device__ __forceinline__ void arrive_lane0(uint32_t bar, int lane) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.s32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(bar), "r"(lane) : "memory");
+}
+
 // The scales of two positions for a row's groups, as FP16 pairs (first position, second): NG bytes from each address.
 template <int NG>
-__device__ __forceinline__ void scale_pairs(const unsigned char* a, const unsigned char* b, uint32_t (&pair)[NG]) {
+__device__ __forceinline__ void scale_pairs(uint32_t a, uint32_t b, uint32_t (&pair)[NG]) {
     constexpr int WORDS = NG >= 4 ? NG / 4 : 1;
 #pragma unroll
     for (int w = 0; w < WORDS; ++w) {
         uint32_t x, y;
-        if constexpr (NG >= 4) x = reinterpret_cast<const uint32_t*>(a)[w], y = reinterpret_cast<const uint32_t*>(b)[w];
-        else x = *reinterpret_cast<const uint16_t*>(a), y = *reinterpret_cast<const uint16_t*>(b);
+        if constexpr (NG >= 4) x = shared_u32(a + 4 * w), y = shared_u32(b + 4 * w);
+        else x = shared_u16(a), y = shared_u16(b);
 #pragma unroll
         for (int k = 0; k < (NG >= 4 ? 2 : 1); ++k) {
             const uint32_t four = __byte_perm(x, y, k ? 0x7632 : 0x5410);          // bytes [x, x', y, y']: two groups
@@ -240,7 +262,8 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
 
     // -- refilling the ring (lane 0; a warp's turns are HB tiles apart) ------------------------------------------------------
     Place4 next = at;               // the tile of this warp's next turn, its page read ahead
-    int next_n = warp, next_page = 0;
+    int next_n = warp, next_page = 0, next_head = 0;
+    const int32_t* next_table = nullptr;
     auto step_to = [&](Place4& c, int by) {
         c.tile += by;
         while (c.tile >= c.tiles) {
@@ -253,42 +276,52 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
             }
         }
     };
+    auto read_row = [&]() {         // what stays the same from tile to tile
+        next_table = p.tables + (int64_t)p.rows[next.r] * p.table_stride;
+        next_head = (u.blocks ? next.sub / (next.subs / HG) : next.sub / u.ctiles) * HB;
+    };
     auto read_page = [&]() {
-        if (next_n < length) {
-            const uint32_t tile = (uint32_t)next.tile;
-            next_page = p.tables[(int64_t)p.rows[next.r] * p.table_stride + (tshift >= 0 ? tile >> tshift : tile / tiles_per_page)];
-        }
+        const uint32_t tile = (uint32_t)next.tile;
+        next_page = next_table[tshift >= 0 ? tile >> tshift : tile / tiles_per_page];
     };
     bool outside = false;
     auto refill = [&](int stage) {  // tile next_n into its stage, which is free
         const uint32_t tile = (uint32_t)next.tile;
-        const uint32_t pidx = tshift >= 0 ? tile >> tshift : tile / tiles_per_page;
         outside |= (uint32_t)next_page >= pages_total;             // the tensor's last page is read instead; reported below
         const uint32_t pg = (uint32_t)next_page < pages_total ? (uint32_t)next_page : pages_total - 1;
-        const int64_t slot0 = (int64_t)pg * p.page + ((tile - pidx * tiles_per_page) << 4);
-        const int head0 = (u.blocks ? next.sub / (next.subs / HG) : next.sub / u.ctiles) * HB;
+        const uint32_t slot0 = pg * (uint32_t)p.page + ((tshift >= 0 ? tile & (tiles_per_page - 1) : tile % tiles_per_page) << 4);
+        const uint64_t scales0 = (uint64_t)slot0 * (uint32_t)row_scales;
         const uint32_t bar = full + stage * 8, to = ring + stage * u.stage_bytes;
         mbar_expect_tx(bar, (uint32_t)(2 * code_bytes + 2 * scale_bytes));
-        tma_load_3d(to, &kmap, 0, (int)slot0, head0, bar);
-        bulk_load(to + 2 * code_bytes, (const char*)p.key_scales + slot0 * row_scales, scale_bytes, bar);
-        tma_load_3d(to + code_bytes, &vmap, 0, (int)slot0, head0, bar);
-        bulk_load(to + 2 * code_bytes + scale_bytes, (const char*)p.value_scales + slot0 * row_scales, scale_bytes, bar);
+        tma_load_3d(to, &kmap, 0, (int)slot0, next_head, bar);
+        bulk_load(to + 2 * code_bytes, (const char*)p.key_scales + scales0, scale_bytes, bar);
+        tma_load_3d(to + code_bytes, &vmap, 0, (int)slot0, next_head, bar);
+        bulk_load(to + 2 * code_bytes + scale_bytes, (const char*)p.value_scales + scales0, scale_bytes, bar);
     };
     auto turn_over = [&]() {        // to this warp's next turn
         next_n += HB;
-        if (lane == 0 && next_n < length) step_to(next, HB), read_page();
+        if (lane == 0 && next_n < length) {
+            next.tile += HB;
+            if (next.tile >= next.tiles) step_to(next, 0), read_row();
+            read_page();
+        }
     };
-    if (lane == 0 && warp < length) step_to(next, warp), read_page();
+    if (lane == 0 && warp < length) step_to(next, warp), read_row(), read_page();
     while (next_n < u.stages - 2 && next_n < length) {             // the first tiles: two stages stay free
         if (lane == 0) refill(next_n);
         turn_over();
     }
 
+    // -8 (rows of the low nibbles) and -8 * 16 (of the high ones), in the raw codes' units; made so that they stay in registers
+    uint32_t eight[4];
+    asm volatile("mov.b32 %0, 0x80088008;\n\tmov.b32 %1, 0x80808080;\n\tmov.b32 %2, 0x80088008;\n\tmov.b32 %3, 0x80808080;"
+                 : "=r"(eight[0]), "=r"(eight[1]), "=r"(eight[2]), "=r"(eight[3]));
     bool dead = false;
     int n = 0, stage = 0;           // tiles taken, the ring's place
     uint32_t phase = 0;
-    // ldmatrix rows: lanes 0-7 and 8-15 name positions 0-7 and 8-15 of chunk 2 i, lanes 16-31 the same of chunk 2 i + 1
-    const int lrow = (lane & 7) + 8 * ((lane >> 3) & 1), lchunk = lane >> 4;
+    // ldmatrix rows: lanes 0-7 and 8-15 name positions 0-7 and 8-15 of chunk 2 i, lanes 16-31 the same of chunk 2 i + 1 (whose
+    // address is chunk lane / 16's with the bits of 2 i changed: a warp's part of a tile lies on a multiple of its swizzle)
+    const uint32_t lane_codes = ring + warp * (16 * (D / 2)) + chunk4<D>((lane & 7) + 8 * ((lane >> 3) & 1), lane >> 4);
 
     while (n < length) {
         // -- a unit: the tiles of one row, head group and query tile in this block -----------------------------------------
@@ -298,10 +331,12 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
         const int per_hg = u.blocks ? at.subs / HG : u.ctiles;
         const int hg = at.sub / per_hg, ct = at.sub - hg * per_hg;
         const int h = hg * HB + warp, start = p.starts[r];
+        const uint32_t lane_kscales = ring + 2 * code_bytes + h * NG + g * row_scales;
+        const uint32_t lane_vscales = ring + 2 * code_bytes + scale_bytes + h * NG + 2 * t * row_scales;
         const int tile0 = at.tile, ntiles = at.tiles - tile0 < length - n ? at.tiles - tile0 : length - n;
 
         uint32_t qb[NT][NG][4];                    // pairs (0, 4), (1, 5), (2, 6), (3, 7) of elements 32 group + 8 t + ..
-        float base8[RAW_K ? NT : 1][NG][2];        // -8 * the sum of a group's queries, in the accumulators' units
+        uint32_t q8[RAW_K ? NT : 1][2];            // -8 * the sums of the groups' queries as an operand: two FP16 terms of groups 2 t, 2 t + 1
         float mul[NT][2];                          // scores of the lane's query rows (8 nt + 2 t + e) into base-2 logits
         int lastpos[NT][2];                        // the last position they see (-1: a padding row)
         unsigned long long seen[MASKS ? NT : 1][2];
@@ -333,7 +368,8 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
             int e = (int)((__float_as_uint(amax) >> 23) & 255u) - 127 - 13;
             e = amax > 0.f ? (e < -90 ? -90 : (e > 90 ? 90 : e)) : 0;
-            const float down = __int_as_float((127 - e) << 23);
+            const float down = __int_as_float(((127 - e) << 23) | (p.scale < 0.f ? (int)0x80000000 : 0));       // (mul is not negative)
+            if constexpr (RAW_K) q8[nt][0] = q8[nt][1] = 0u;
 #pragma unroll
             for (int k = 0; k < NG; ++k) {
                 float sum = 0.f;
@@ -347,15 +383,19 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
                 if constexpr (RAW_K) {
                     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) base8[nt][k][j] = -0x1p-21f * __shfl_sync(0xffffffffu, sum, (2 * t + j) * 4);
+                    sum *= -0x1p-21f;                                                  // (8 * 2^-24)
+                    const __half hi = __float2half_rn(sum), lo = __float2half_rn(sum - __half2float(hi));
+                    if (2 * t == (k & ~1)) {
+                        q8[nt][0] |= (uint32_t)__half_as_ushort(hi) << (16 * (k & 1));
+                        q8[nt][1] |= (uint32_t)__half_as_ushort(lo) << (16 * (k & 1));
+                    }
                 }
             }
             // the lane's columns are query rows 2 t and 2 t + 1: their exponents live with lanes g = 2 t and 2 t + 1
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int er = __shfl_sync(0xffffffffu, e, (2 * t + j) * 4);
-                mul[nt][j] = p.scale * LOG2E * __int_as_float((127 + er + (RAW_K ? 24 : 0)) << 23);
+                mul[nt][j] = fmaxf(fabsf(p.scale) * LOG2E * __int_as_float((127 + er + (RAW_K ? 24 : 0)) << 23), 1e-37f);
                 const int c = (ct * ROWS + nt * 8 + 2 * t + j) / G;
                 lastpos[nt][j] = c < count ? (int)(context ? first - 1 : first + c) : -1;
                 if constexpr (MASKS) {
@@ -388,18 +428,21 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
             l_run[nt][0] = l_run[nt][1] = 0.f;
         }
 
-        for (int i = 0; i < ntiles; i += TPI) {
-            const int have = ntiles - i < TPI ? ntiles - i : TPI;
+        // An iteration over `have` tiles from tile i of the unit.  GENERAL false: TPI tiles that every query row sees whole, the
+        // bulk of a long row, in code of its own so that no instruction of it is about masks.
+        auto iterate = [&](auto general, const int i, const int have) {
+            constexpr bool GENERAL = decltype(general)::value;
             float x[TPI][NT][4];
             int stages[TPI];
-            bool masked = MASKS;
 #pragma unroll
             for (int v = 0; v < TPI; ++v) {
+                if (GENERAL && v >= have) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) x[v][nt][c] = v < have ? 0.f : -INFINITY;
-                if (v >= have) continue;
+                        for (int c = 0; c < 4; ++c) x[v][nt][c] = -INFINITY;
+                    continue;
+                }
                 // this warp's turn: tile n + S - 2 into the stage of tile n - 2, once every warp is done with that
                 if (n + u.stages - 2 == next_n) {
                     if (lane == 0 && next_n < length) {
@@ -413,23 +456,27 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
                 }
                 stages[v] = stage;
                 if (!mbar_wait(full + stage * 8, phase)) dead = true;
+                __syncwarp();
                 if (++stage == u.stages) stage = 0, phase ^= 1;
                 ++n;
-                if (__any_sync(0xffffffffu, dead)) {
-                    dead = true;
-                    break;
-                }
-                masked |= ((tile0 + i + v) << 4) + 16 > first32;
                 // scores
-                const int from = stages[v] * u.stage_bytes;
-                const uint32_t ktile = ring + from + warp * (16 * (D / 2));
-                const unsigned char* ks = smem + from + 2 * code_bytes + h * NG;
+                const uint32_t from = stages[v] * u.stage_bytes;
                 uint32_t pair[NG];
-                scale_pairs<NG>(ks + g * row_scales, ks + (g + 8) * row_scales, pair);
+                scale_pairs<NG>(lane_kscales + from, lane_kscales + from + 8 * row_scales, pair);
+                if constexpr (RAW_K) {
+                    // scale[position][group] * (-8 * sum of the group's queries): groups 2 t and 2 t + 1 are this lane's columns
+                    uint32_t even = pair[0], odd = pair[1];
+#pragma unroll
+                    for (int k = 2; k < NG; k += 2) even = 2 * t == k ? pair[k] : even, odd = 2 * t == k ? pair[k + 1] : odd;
+                    uint32_t a[4];
+                    a[0] = a[2] = __byte_perm(even, odd, 0x5410), a[1] = a[3] = __byte_perm(even, odd, 0x7632);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma16816_new(x[v][nt], a, q8[nt][0], q8[nt][1]);
+                }
 #pragma unroll
                 for (int k = 0; k < NG; k += 2) {
                     uint32_t w[4];
-                    ldmatrix_x4(w, ktile + chunk4<D>(lrow, k + lchunk));
+                    ldmatrix_x4(w, (lane_codes + from) ^ (k << 4));
 #pragma unroll
                     for (int o = 0; o < 2; ++o) {
                         const float2 s = __half22float2(*reinterpret_cast<__half2*>(&pair[k + o]));
@@ -438,22 +485,22 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             float c[4];
-                            if constexpr (RAW_K) c[0] = c[2] = base8[nt][k + o][0], c[1] = c[3] = base8[nt][k + o][1];
-                            else c[0] = c[1] = c[2] = c[3] = 0.f;
-                            mma16816<false>(c, a1, qb[nt][k + o][0], qb[nt][k + o][1]);
+                            mma16816_new(c, a1, qb[nt][k + o][0], qb[nt][k + o][1]);
                             mma16816<false>(c, a2, qb[nt][k + o][2], qb[nt][k + o][3]);
-                            x[v][nt][0] = fmaf(c[0], s.x, x[v][nt][0]), x[v][nt][1] = fmaf(c[1], s.x, x[v][nt][1]);
-                            x[v][nt][2] = fmaf(c[2], s.y, x[v][nt][2]), x[v][nt][3] = fmaf(c[3], s.y, x[v][nt][3]);
+                            if (!RAW_K && k + o == 0) {
+                                x[v][nt][0] = c[0] * s.x, x[v][nt][1] = c[1] * s.x, x[v][nt][2] = c[2] * s.y, x[v][nt][3] = c[3] * s.y;
+                            } else {
+                                x[v][nt][0] = fmaf(c[0], s.x, x[v][nt][0]), x[v][nt][1] = fmaf(c[1], s.x, x[v][nt][1]);
+                                x[v][nt][2] = fmaf(c[2], s.y, x[v][nt][2]), x[v][nt][3] = fmaf(c[3], s.y, x[v][nt][3]);
+                            }
                         }
                     }
                 }
             }
-            if (dead) break;
 
             // masks, online softmax
-            uint32_t pb[TPI][NT][2];
-            bool rescale = false;
-            float alpha[NT][2];
+            bool passed = false;
+            float top[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float mx[2] = {-INFINITY, -INFINITY};
@@ -461,9 +508,8 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
                 for (int v = 0; v < TPI; ++v)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        float y = x[v][nt][c] * mul[nt][c & 1];
-                        if (v >= have) y = -INFINITY;
-                        if (masked) {
+                        float y = x[v][nt][c];
+                        if constexpr (GENERAL) {
                             const int pos = ((tile0 + i + v) << 4) + g + 8 * (c >> 1), last = lastpos[nt][c & 1];
                             if (pos > last) y = -INFINITY;
                             if constexpr (MASKS) {
@@ -482,61 +528,65 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
                         x[v][nt][c] = y;
                         mx[c & 1] = fmaxf(mx[c & 1], y);
                     }
+                top[nt][0] = mx[0] * mul[nt][0], top[nt][1] = mx[1] * mul[nt][1];
+                passed |= top[nt][0] > m_run[nt][0] || top[nt][1] > m_run[nt][1];
+            }
+            // The reference of a row moves only when a score of it passes it; the lanes' maxima are compared across the warp, and
+            // the sums brought to the new reference, only then.
+            if (__any_sync(0xffffffffu, passed)) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 4));
-                    mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 8));
-                    mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 16));
-                    const bool moved = mx[j] > m_run[nt][j];
-                    const float top = moved ? mx[j] + AHEAD : m_run[nt][j];
-                    const float sub = top == -INFINITY ? 0.f : top;
-                    alpha[nt][j] = moved ? ex2(m_run[nt][j] - sub) : 1.f;
-                    rescale |= moved;
-                    m_run[nt][j] = top;
-                    mx[j] = sub;
+                for (int nt = 0; nt < NT; ++nt) {
+                    float alpha[2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float high = top[nt][j];
+                        high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 4));
+                        high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 8));
+                        high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 16));
+                        const bool moved = high > m_run[nt][j];
+                        alpha[j] = moved ? ex2(m_run[nt][j] - (high + AHEAD)) : 1.f;
+                        m_run[nt][j] = moved ? high + AHEAD : m_run[nt][j];
+                        l_run[nt][j] *= alpha[j];
+                    }
+#pragma unroll
+                    for (int k = 0; k < NG; ++k)
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) acc[k][c >> 2][nt][c & 3] *= alpha[c & 1];
+                    if constexpr (RAW_V) {
+#pragma unroll
+                        for (int k = 0; k < NG; ++k)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) acc8[k][c] *= alpha[c & 1];
+                    }
                 }
-                float sum[2] = {0.f, 0.f};
+            }
+            uint32_t pb[TPI][NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                // (a row that has seen nothing has no reference: its scores are all -inf)
+                const float sub[2] = {GENERAL && m_run[nt][0] == -INFINITY ? 0.f : m_run[nt][0], GENERAL && m_run[nt][1] == -INFINITY ? 0.f : m_run[nt][1]};
 #pragma unroll
                 for (int v = 0; v < TPI; ++v) {
                     float w[4];
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        w[c] = ex2(x[v][nt][c] - mx[c & 1]);
-                        sum[c & 1] += w[c];
+                        w[c] = ex2(fmaf(x[v][nt][c], mul[nt][c & 1], -sub[c & 1]));
+                        l_run[nt][c & 1] += w[c];
                     }
                     pb[v][nt][0] = movmatrix_trans(pack2<false>(w[0], w[1]));
                     pb[v][nt][1] = movmatrix_trans(pack2<false>(w[2], w[3]));
-                }
-                l_run[nt][0] = l_run[nt][0] * alpha[nt][0] + sum[0];
-                l_run[nt][1] = l_run[nt][1] * alpha[nt][1] + sum[1];
-            }
-            if (__any_sync(0xffffffffu, rescale)) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                    for (int k = 0; k < NG; ++k)
-#pragma unroll
-                        for (int c = 0; c < 8; ++c) acc[k][c >> 2][nt][c & 3] *= alpha[nt][c & 1];
-                    if constexpr (RAW_V) {
-#pragma unroll
-                        for (int k = 0; k < NG; ++k)
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) acc8[k][c] *= alpha[0][c & 1];
-                    }
                 }
             }
 
             // outputs
 #pragma unroll
             for (int v = 0; v < TPI; ++v) {
-                if (v >= have) continue;
-                const int from = stages[v] * u.stage_bytes;
-                const uint32_t vtile = ring + from + code_bytes + warp * (16 * (D / 2));
-                const unsigned char* vs = smem + from + 2 * code_bytes + scale_bytes + h * NG;
+                if (GENERAL && v >= have) continue;
+                const uint32_t from = stages[v] * u.stage_bytes;
                 uint32_t pair[2][NG];                    // scales of positions 2 t, 2 t + 1 and of 2 t + 8, 2 t + 9
-                scale_pairs<NG>(vs + 2 * t * row_scales, vs + (2 * t + 1) * row_scales, pair[0]);
-                scale_pairs<NG>(vs + (2 * t + 8) * row_scales, vs + (2 * t + 9) * row_scales, pair[1]);
-                if (SCALE_CODES && masked) {
+                scale_pairs<NG>(lane_vscales + from, lane_vscales + from + row_scales, pair[0]);
+                scale_pairs<NG>(lane_vscales + from + 8 * row_scales, lane_vscales + from + 9 * row_scales, pair[1]);
+                if constexpr (SCALE_CODES && GENERAL) {
                     // A position that a query row does not take may have any scale, a NaN too: the scale becomes 0, and the
                     // weights of the rows that do take the position a NaN.
 #pragma unroll
@@ -554,7 +604,7 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
 #pragma unroll
                 for (int k = 0; k < NG; k += 2) {
                     uint32_t w[4];
-                    ldmatrix_x4_trans(w, vtile + chunk4<D>(lrow, k + lchunk));
+                    ldmatrix_x4_trans(w, (lane_codes + from + code_bytes) ^ (k << 4));
 #pragma unroll
                     for (int o = 0; o < 2; ++o) {
                         // words of positions 0-7 and 8-15: values 4 g .. 4 g + 3 of the group
@@ -571,22 +621,29 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
                             uint32_t b0 = pb[v][nt][0], b1 = pb[v][nt][1];
                             if constexpr (!SCALE_CODES) {
                                 b0 = hmul2_bits(b0, pair[0][k + o]), b1 = hmul2_bits(b1, pair[1][k + o]);
-                                if (masked) b0 &= nonzero2(pb[v][nt][0]), b1 &= nonzero2(pb[v][nt][1]);
+                                if constexpr (GENERAL) b0 &= nonzero2(pb[v][nt][0]), b1 &= nonzero2(pb[v][nt][1]);
                             }
                             mma16816<false>(acc[k + o][0][nt], a1, b0, b1);
                             mma16816<false>(acc[k + o][1][nt], a2, b0, b1);
                             if constexpr (RAW_V) {
-                                const uint32_t eight[4] = {0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u};      // -8, and -8 * 16
                                 mma16816<false>(acc8[k + o], eight, b0, b1);
                             }
                         }
                     }
                 }
                 __syncwarp();
-                if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(empty + stages[v] * 8) : "memory");
+                arrive_lane0(empty + stages[v] * 8, lane);
             }
+        };
+        // (a wait that ran out ends the warp's work after its iteration; what it computed is not written)
+        int i = 0;
+        if constexpr (!MASKS) {
+            const int clear = (first32 >> 4) - tile0;           // tiles whose positions are all before the row's first
+            const int plain = (clear < ntiles ? clear : ntiles) / TPI * TPI;
+            for (; i < plain && !__any_sync(0xffffffffu, dead); i += TPI) iterate(std::false_type(), i, TPI);
         }
-        if (dead) break;
+        for (; i < ntiles && !__any_sync(0xffffffffu, dead); i += TPI) iterate(std::true_type(), i, ntiles - i < TPI ? ntiles - i : TPI);
+        if (__any_sync(0xffffffffu, dead)) break;
 
         // -- the state, or the row's output ------------------------------------------------------------------------------------
         bool whole, fits = true;
