@@ -33,6 +33,8 @@ __all__ = ["KINDS", "MAX_COLUMNS", "attend", "chunk_for", "gather", "merge_shard
            "partitions", "parts_for", "rope_axes", "engine_for", "piece_size", "plan", "prefill", "prefill_serves", "release", "slots_at", "states_for", "status", "tcgen05_serves",
            "tcgen05p_serves", "tile_for", "workspace_floats", "write"]
 
+_STAGINGS = {None: 0, "cp.async": 1, "tma": 2}
+_ENGINES = {"tcgen05": 8, "mma.sync": 16, "tcgen05t": 64, "tcgen05p": 128, "even": 512}
 KINDS = {"bf16": 0, "fp16": 0, "fp8": 1, "fp8:row": 2, "int8": 3, "fp8:page": 4, "int4": 5}
 GROUP4 = 32                 # elements of an "int4" row that share a scale
 MAX_COLUMNS = 64            # columns of one row a launch reads
@@ -53,15 +55,15 @@ def _check_kind(kind, key_scales):
 
 def _check4(pages, scales, what):
     """An "int4" page tensor [...][kv_heads][dim / 2] and its scales [...][kv_heads][dim / 32]: (kv_heads, dim)."""
-    hkv, dim = pages.shape[-2], 2 * pages.shape[-1]
-    if pages.dtype != torch.uint8 or scales.dtype != torch.uint8:
+    hkv, half = pages.shape[-2:]
+    if pages.dtype is not torch.uint8 or scales.dtype is not torch.uint8:
         raise ValueError(f"int4 pages and their scales are uint8 tensors: {what} are {pages.dtype} with scales of {scales.dtype}")
-    if dim % GROUP4 or scales.numel() * GROUP4 != pages.numel() * 2 or not scales.is_contiguous():
-        raise ValueError(f"int4 {what} of [{hkv}][{dim}] rows have contiguous scales [...][{hkv}][{dim // GROUP4}], a byte for "
+    if half % (GROUP4 // 2) or scales.numel() * (GROUP4 // 2) != pages.numel() or not scales.is_contiguous() or not pages.is_contiguous():
+        raise ValueError(f"int4 {what} of [{hkv}][{2 * half}] rows have contiguous scales [...][{hkv}][{2 * half // GROUP4}], a byte for "
                          f"each group of {GROUP4} elements")
-    if scales.device != pages.device:
+    if scales.get_device() != pages.get_device():
         raise ValueError(f"int4 {what} and their scales are on one device")
-    return hkv, dim
+    return hkv, 2 * half
 
 
 def _cuda(tensor, what):
@@ -71,11 +73,23 @@ def _cuda(tensor, what):
 
 
 def _ptr(tensor):
-    return ctypes.c_void_p(tensor.data_ptr()) if tensor is not None else None
+    return tensor.data_ptr() if tensor is not None else None
 
 
-def _stream(device):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+# (the handle alone: a Stream object takes longer to make than a launch's other host work)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _run(name, what, device, *params):
+    """The library's entry point `name` on the device's current stream, with that device current; errors raised."""
+    call, index, current = getattr(_lib.load(), name), device.index, torch.cuda.current_device()
+    if index is None or index == current:
+        code = call(*params, _raw_stream(current))
+    else:
+        with torch.cuda.device(index):
+            code = call(*params, _raw_stream(index))
+    if code:
+        _lib.check(code, what)
 
 
 def _page_dtype(kind, pages):
@@ -118,7 +132,7 @@ def _workspace(device, floats, given):
             raise ValueError(f"attend's workspace holds {given.numel()} floats; this launch needs {floats} "
                              "(workspace_floats)")
         return given
-    at = (str(device), getattr(_owner, "key", None))
+    at = (device.index, getattr(_owner, "key", None))
     found = _workspaces.get(at)
     if found is None or found.numel() < floats:
         if torch.cuda.is_current_stream_capturing():
@@ -130,16 +144,22 @@ def _workspace(device, floats, given):
     return found
 
 
-_status = {}
+_status, _status_at = {}, {}
+_even_floats = {}           # an even launch's workspace, by device and shape (the library's answer)
 
 
 def _status_word(device):
     """One int32 a device: a kernel sets it (and never clears it) when one of its bounded waits gave up."""
+    found = _status_at.get(device.index)
+    if found is not None:
+        return found
     found = _status.get(str(device))
     if found is None:
         if torch.cuda.is_current_stream_capturing():
             return None
         found = _status[str(device)] = torch.zeros(1, dtype=torch.int32, device=device)
+    if device.index is not None:
+        _status_at[device.index] = found
     return found
 
 
@@ -287,50 +307,44 @@ def write(keys, values, slots, key_pages, value_pages, kind, key_scales=None, va
         _check_kind(kind, key_scales)
         return
     p, _held = _append_params(keys, values, slots, key_pages, value_pages, kind, key_scales, value_scales, multipliers)
-    with torch.cuda.device(keys.device):
-        _lib.check(_lib.load().crit_b200_append(ctypes.byref(p), _stream(keys.device)), "crit_b200.write")
+    _run("crit_b200_append", "crit_b200.write", keys.device, p)
 
 
 def _append_params(keys, values, slots, key_pages, value_pages, kind, key_scales, value_scales, multipliers):
     """The append's parameter block, its arguments checked, and the tensors it points at that were made here."""
     k_kind = _check_kind(kind, key_scales)
     T, hkv, d = keys.shape
-    if keys.dtype not in _DTYPES or (values is not None and values.dtype != keys.dtype):
+    in_dtype, place = _DTYPES.get(keys.dtype), keys.get_device()
+    if in_dtype is None or (values is not None and values.dtype != keys.dtype):
         raise ValueError("keys and values are bf16, fp16 or fp32 tensors of one dtype")
     if keys.stride(-1) != 1:
         keys = keys.contiguous()
     if values is not None and values.stride(-1) != 1:
         values = values.contiguous()
-    if slots.dtype != torch.int64 or not slots.is_contiguous() or slots.numel() != T:
-        raise ValueError(f"slots are contiguous int64 [{T}]")
+    if slots.dtype is not torch.int64 or not slots.is_contiguous() or slots.numel() != T or slots.get_device() != place:
+        raise ValueError(f"slots are contiguous int64 [{T}] on the keys' device")
     if not key_pages.is_contiguous() or (value_pages is not None and not value_pages.is_contiguous()):
         raise ValueError("pages are contiguous [slots][kv_heads][dim] storage")
-    page = 1
+    page, dv = 1, d
     if k_kind == 5:
-        for rows, pages, scales, what in ((keys, key_pages, key_scales, "keys"), (values, value_pages, value_scales, "values")):
-            if rows is not None:
-                if pages is None or scales is None:
-                    raise ValueError(f"write stores int4 {what} in pages with scales beside them")
-                if _check4(pages, scales, what) != tuple(rows.shape[1:]) or rows.shape[0] != T or pages.device != keys.device:
-                    raise ValueError(f"int4 {what} [{T}][{hkv}][{rows.shape[-1]}] go to pages [...][{hkv}][{rows.shape[-1] // 2}]")
-    if k_kind == 4:
+        if key_pages is None or (hkv, d) != _check4(key_pages, key_scales, "keys") or key_pages.get_device() != place:
+            raise ValueError(f"int4 keys [{T}][{hkv}][{d}] go to pages [...][{hkv}][{d // 2}] on their device")
+        if values is not None:
+            if value_pages is None or value_scales is None:
+                raise ValueError("write stores int4 values in pages with scales beside them")
+            if values.shape != (T, *_check4(value_pages, value_scales, "values")) or value_pages.get_device() != place or values.get_device() != place:
+                raise ValueError(f"int4 values {list(values.shape)} go to pages [...][{hkv}][{values.shape[-1] // 2}] on their device, a row a token")
+    elif k_kind == 4:
         if key_pages.dim() != 4:
             raise ValueError("fp8:page pages are given as [pages][page][kv_heads][dim]")
         page = key_pages.shape[1]
-    p = _lib.AppendParams()
-    p.keys, p.values, p.slots = _ptr(keys), _ptr(values), _ptr(slots)
-    p.key_pages, p.value_pages = _ptr(key_pages), _ptr(value_pages)
-    p.key_scales, p.value_scales = _ptr(key_scales), _ptr(value_scales)
-    p.tokens = T
-    p.slots_total = key_pages.numel() // (hkv * key_pages.shape[-1])
-    p.status = _ptr(_status_word(keys.device))
-    p.key_stride_token, p.key_stride_head = keys.stride(0), keys.stride(1)
+    value_at = value_token = value_head = 0
     if values is not None:
-        p.value_stride_token, p.value_stride_head = values.stride(0), values.stride(1)
-    p.kv_heads, p.head_dim, p.page = hkv, d, page
-    p.value_dim = values.shape[-1] if values is not None else d
-    p.kind, p.in_dtype, p.page_dtype = k_kind, _DTYPES[keys.dtype], _page_dtype(kind, key_pages)
-    p.key_multiplier, p.value_multiplier = float(multipliers[0]), float(multipliers[1])
+        value_at, (value_token, value_head, _), dv = values.data_ptr(), values.stride(), values.shape[-1]
+    key_token, key_head, _ = keys.stride()
+    p = _lib.block(_lib.AppendParams, keys.data_ptr(), value_at, slots.data_ptr(), key_pages.data_ptr(), _ptr(value_pages), _ptr(key_scales), _ptr(value_scales),
+                   _ptr(_status_word(keys.device)), T, key_pages.numel() // (hkv * key_pages.shape[-1]), key_token, key_head, value_token, value_head,
+                   hkv, d, dv, page, k_kind, in_dtype, _page_dtype(kind, key_pages), multipliers[0], multipliers[1])
     return p, (keys, values)
 
 
@@ -352,7 +366,8 @@ def rope_axes(sections, interleaved=False, device="cuda"):
 
 def _vectors_fit(x):
     """Whether rows are read or written in the kernel's vectors of four elements as they lie."""
-    return x.stride(-1) == 1 and not (x.stride(0) | x.stride(1)) % 4 and not x.data_ptr() % (4 * x.element_size())
+    token, head, element = x.stride()
+    return element == 1 and not (token | head) % 4 and not x.data_ptr() % (4 * x.element_size())
 
 
 def _vectors(x):
@@ -363,51 +378,54 @@ def _vectors(x):
 def _norm_rope_params(q, keys, positions, frequencies, q_weight, key_weight, eps, offset, axes, interleaved, magnitude, q_out, keys_out, writes):
     """norm_rope's arguments checked: (parameter block, [q, keys] as they are read, [q, keys] outputs, outputs to copy)."""
     given = q if q is not None else keys
-    T, d, device, dtype = given.shape[0], given.shape[-1], given.device, given.dtype
-    for x, what in ((q, "q"), (keys, "keys")):
-        if x is not None and (x.dim() != 3 or x.shape[0] != T or x.shape[-1] != d or x.dtype != dtype or x.device != device or x.dtype not in _DTYPES):
-            raise ValueError(f"q and keys are bf16, fp16 or fp32 tensors [tokens][heads][dim] of one dtype, width and device: {what} is not")
-    if frequencies.dtype != torch.float32 or frequencies.dim() != 1 or not frequencies.is_contiguous() or frequencies.device != device:
+    if given.dim() != 3:
+        raise ValueError("q and keys are [tokens][heads][dim]")
+    (T, _, d), device, place, dtype = given.shape, given.device, given.get_device(), given.dtype
+    half, n_axes, axis_stride, weight_dtype = frequencies.numel(), 1, 0, None
+    if dtype not in _DTYPES or (q is not None and keys is not None and
+                                (keys.dim() != 3 or keys.shape[0] != T or keys.shape[-1] != d or keys.dtype != dtype or keys.get_device() != place)):
+        raise ValueError("q and keys are bf16, fp16 or fp32 tensors [tokens][heads][dim] of one dtype, width and device")
+    if frequencies.dtype is not torch.float32 or frequencies.dim() != 1 or not frequencies.is_contiguous() or frequencies.get_device() != place:
         raise ValueError("frequencies are contiguous FP32 [rotary / 2] on the queries' device")
-    if positions.dtype != torch.int64 or positions.dim() not in (1, 2) or positions.shape[-1] != T or positions.device != device or \
-            (T and positions.stride(-1) != 1):
+    if positions.dim() == 2:
+        n_axes, axis_stride = positions.shape[0], positions.stride(0)
+    if positions.dtype is not torch.int64 or positions.dim() not in (1, 2) or positions.shape[-1] != T or positions.get_device() != place or \
+            (T > 1 and positions.stride(-1) != 1):
         raise ValueError(f"positions are int64 [{T}], or [axes][{T}], on the queries' device")
-    n_axes = positions.shape[0] if positions.dim() == 2 else 1
-    if axes is not None and (axes.dtype != torch.int32 or axes.numel() != frequencies.numel() or not axes.is_contiguous() or axes.device != device):
-        raise ValueError("axes are contiguous int32, one for each frequency (rope_axes)")
-    if axes is None and n_axes > 1:
+    if axes is not None:
+        if axes.dtype is not torch.int32 or axes.numel() != half or not axes.is_contiguous() or axes.get_device() != place:
+            raise ValueError("axes are contiguous int32, one for each frequency (rope_axes)")
+    elif n_axes > 1:
         raise ValueError("positions of several axes come with the axis of each pair: axes (rope_axes)")
-    weights = [w for w in (q_weight if q is not None else None, key_weight if keys is not None else None) if w is not None]
-    for w in weights:
-        if w.dtype not in _DTYPES or w.dtype != weights[0].dtype or w.numel() != d or not w.is_contiguous() or w.device != device:
-            raise ValueError(f"q_weight and key_weight are contiguous [{d}] of one bf16, fp16 or fp32 type, on the queries' device")
-    p = _lib.NormRopeParams()
-    reads, outs, copies = [], [], []
-    for x, out, what, side in ((q, q_out, "q", "q"), (keys, keys_out, "keys", "key")):
-        if out is not None and (x is None or out.shape != x.shape or out.dtype != dtype or out.device != device):
-            raise ValueError(f"the {what} output has the shape, dtype and device of {what}")
-        if x is not None and out is None and not (writes and what == "keys"):
-            out = torch.empty(x.shape, dtype=dtype, device=device)
-        outs.append(out)
-        reads.append(None if x is None else _vectors(x))
-        if x is not None:
-            setattr(p, what, x.data_ptr() if reads[-1] is x else reads[-1].data_ptr())
-            setattr(p, side + "_stride_token", reads[-1].stride(0)), setattr(p, side + "_stride_head", reads[-1].stride(1))
-        if out is not None:
-            into = out
+    for w in (q_weight if q is not None else None, key_weight if keys is not None else None):
+        if w is not None:
+            weight_dtype = weight_dtype or w.dtype
+            if w.dtype not in _DTYPES or w.dtype != weight_dtype or w.numel() != d or not w.is_contiguous() or w.get_device() != place:
+                raise ValueError(f"q_weight and key_weight are contiguous [{d}] of one bf16, fp16 or fp32 type, on the queries' device")
+    reads, outs, copies, at, strides = [], [], [], [], []
+    for x, out, what in ((q, q_out, "q"), (keys, keys_out, "keys")):
+        if x is None:
+            if out is not None:
+                raise ValueError(f"there are no {what} for the {what} output, whose shape, dtype and device are theirs")
+            reads.append(None), outs.append(None), at.append((0, 0)), strides.append((0, 0, 0, 0, 0, 0))
+            continue
+        read, into = _vectors(x), out
+        if out is None and not (writes and what == "keys"):
+            out = into = torch.empty_like(x, memory_format=torch.contiguous_format)
+        elif out is not None:
+            if out.shape != x.shape or out.dtype != dtype or out.get_device() != place:
+                raise ValueError(f"the {what} output has the shape, dtype and device of {what}")
             if not _vectors_fit(out):                  # made beside it and copied
-                into = torch.empty(out.shape, dtype=dtype, device=device)
+                into = torch.empty_like(x, memory_format=torch.contiguous_format)
                 copies.append((out, into))
-            setattr(p, what + "_out", into.data_ptr())
-            setattr(p, side + "_out_stride_token", into.stride(0)), setattr(p, side + "_out_stride_head", into.stride(1))
-    p.q_heads, p.kv_heads = (q.shape[1] if q is not None else 0), (keys.shape[1] if keys is not None else 0)
-    p.positions, p.frequencies, p.axes = _ptr(positions), _ptr(frequencies), _ptr(axes)
-    p.q_weight, p.key_weight = _ptr(q_weight), _ptr(key_weight)
-    p.status = _ptr(_status_word(device))
-    p.tokens, p.axis_stride = T, positions.stride(0) if positions.dim() == 2 else 0
-    p.head_dim, p.rotary, p.n_axes, p.interleaved = d, 2 * frequencies.numel(), n_axes, int(bool(interleaved))
-    p.dtype, p.weight_dtype = _DTYPES[dtype], _DTYPES[weights[0].dtype] if weights else 0
-    p.eps, p.offset, p.magnitude = float(eps), float(offset), float(magnitude)
+        reads.append(read), outs.append(out), at.append((read.data_ptr(), _ptr(into)))
+        strides.append(read.stride() + (into.stride() if into is not None else (0, 0, 0)))
+    (q_at, q_to), (k_at, k_to) = at
+    a, b = strides
+    p = _lib.block(_lib.NormRopeParams, q_at, k_at, q_to, k_to, positions.data_ptr(), frequencies.data_ptr(), _ptr(axes), _ptr(q_weight), _ptr(key_weight),
+                   _ptr(_status_word(device)), T, axis_stride, a[0], a[1], b[0], b[1], a[3], a[4], b[3], b[4],
+                   q.shape[1] if q is not None else 0, keys.shape[1] if keys is not None else 0, d, 2 * half, n_axes, bool(interleaved),
+                   _DTYPES[dtype], _DTYPES[weight_dtype] if weight_dtype else 0, eps, offset, magnitude)
     return p, reads, outs, copies
 
 
@@ -435,8 +453,7 @@ def _launch_norm_rope(p, append, reads, copies, what):
     if p.tokens == 0:
         return
     device = (reads[0] if reads[0] is not None else reads[1]).device
-    with torch.cuda.device(device):
-        _lib.check(_lib.load().crit_b200_norm_rope(ctypes.byref(p), ctypes.byref(append) if append is not None else None, _stream(device)), what)
+    _run("crit_b200_norm_rope", what, device, p, append)
     for out, made in copies:
         out.copy_(made)
 
@@ -474,35 +491,33 @@ def gather(pages, kind, page, *, table=None, slots=None, count=None, scales=None
     _cuda(pages, "pages")
     k_kind = _check_kind(kind, scales)
     hkv, dim = _check4(pages, scales, "rows") if k_kind == 5 else pages.shape[-2:]
-    shape = None
+    place = pages.get_device()
     if slots is not None:
-        shape, slots = tuple(slots.shape), slots.reshape(-1).contiguous()
-        count = slots.numel()
+        shape = (*slots.shape, hkv, dim)
+        if slots.dim() != 1 or not slots.is_contiguous():
+            slots = slots.reshape(-1).contiguous()
+        count, listed = slots.numel(), slots
     elif table is None or count is None:
         raise ValueError("gather reads a page table's first `count` positions, or rows at `slots`")
-    if out is None:
-        out = torch.empty((count, hkv, dim), dtype=dtype, device=pages.device)
-    elif out.numel() != count * hkv * dim or not out.is_contiguous() or out.dtype not in _DTYPES or out.device != pages.device:
-        raise ValueError(f"gather's out is a contiguous bf16, fp16 or fp32 tensor of [{count}][{hkv}][{dim}] on the pages' device")
     else:
-        dtype = out.dtype
-        out = out.view(count, hkv, dim)
+        table = listed = table.contiguous()
+        shape = (count, hkv, dim)
+    if listed.get_device() != place:
+        raise ValueError("gather's slots or page table are on the pages' device")
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=pages.device)
+    elif out.numel() != count * hkv * dim or not out.is_contiguous() or out.dtype not in _DTYPES or out.get_device() != place:
+        raise ValueError(f"gather's out is a contiguous bf16, fp16 or fp32 tensor of [{count}][{hkv}][{dim}] on the pages' device")
+    elif out.shape != shape:
+        out = out.view(shape)
     if count == 0:
-        return out if shape is None else out.view(*shape, hkv, dim)
-    p = _lib.GatherParams()
-    p.pages, p.scales, p.out = _ptr(pages), _ptr(scales), _ptr(out)
-    p.table = _ptr(table.contiguous()) if table is not None else None
-    p.slots = _ptr(slots)
+        return out
     if not pages.is_contiguous():
         raise ValueError("pages are contiguous [slots][kv_heads][dim] storage")
-    p.slots_total = pages.numel() // (hkv * pages.shape[-1])
-    p.status = _ptr(_status_word(pages.device))
-    p.count, p.kv_heads, p.dim, p.page = count, hkv, dim, int(page)
-    p.kind, p.page_dtype, p.out_dtype = k_kind, _page_dtype(kind, pages), _DTYPES[dtype]
-    p.multiplier = float(multiplier)
-    with torch.cuda.device(pages.device):
-        _lib.check(_lib.load().crit_b200_gather(ctypes.byref(p), _stream(pages.device)), "crit_b200.gather")
-    return out if shape is None else out.view(*shape, hkv, dim)
+    p = _lib.block(_lib.GatherParams, pages.data_ptr(), _ptr(scales), _ptr(table), _ptr(slots), out.data_ptr(), _ptr(_status_word(pages.device)), count,
+                   pages.numel() // (hkv * pages.shape[-1]), hkv, dim, page, k_kind, _page_dtype(kind, pages), _DTYPES[out.dtype], multiplier)
+    _run("crit_b200_gather", "crit_b200.gather", pages.device, p)
+    return out
 
 
 def slots_at(tables, rows, positions, page, dump, capacity=None, out=None):
@@ -519,8 +534,7 @@ def slots_at(tables, rows, positions, page, dump, capacity=None, out=None):
     p.tables, p.rows, p.positions, p.capacity, p.slots = _ptr(tables), _ptr(rows), _ptr(positions), _ptr(capacity), _ptr(out)
     p.n, p.table_stride, p.table_width = positions.numel(), tables.stride(0), tables.shape[1]
     p.page, p.dump = int(page), int(dump)
-    with torch.cuda.device(tables.device):
-        _lib.check(_lib.load().crit_b200_slots(ctypes.byref(p), _stream(tables.device)), "crit_b200.slots_at")
+    _run("crit_b200_slots", "crit_b200.slots_at", tables.device, p)
     return out.view(shape)
 
 
@@ -542,8 +556,7 @@ def move_rows(store, source, target):
     p.store, p.source, p.target = _ptr(store), _ptr(source), _ptr(target)
     p.lists, p.width, p.slots, p.row_bytes, p.layers = source.shape[0], source.shape[1], slots, row_bytes, layers
     p.status = _ptr(_status_word(store.device))
-    with torch.cuda.device(store.device):
-        _lib.check(_lib.load().crit_b200_move_rows(ctypes.byref(p), _stream(store.device)), "crit_b200.move_rows")
+    _run("crit_b200_move_rows", "crit_b200.move_rows", store.device, p)
 
 
 def _listed_rows(tables, rows, starts, counts, firsts, blocks, block_size, page, columns, out, lse):
@@ -564,8 +577,7 @@ def _listed_rows(tables, rows, starts, counts, firsts, blocks, block_size, page,
     p.columns, p.blocks_k, p.block_size, p.page = columns, blocks.shape[1], block_size, page
     p.dump = 0              # (entries past a row's listed pages are never read: its last position ends before them)
     p.q_heads, p.value_dim, p.out_dtype = out.shape[1], out.shape[2], _DTYPES[out.dtype]
-    with torch.cuda.device(device):
-        _lib.check(_lib.load().crit_b200_compact_blocks(ctypes.byref(p), _stream(device)), "crit_b200.attend (block lists)")
+    _run("crit_b200_compact_blocks", "crit_b200.attend (block lists)", device, p)
     tokens = (starts[:, None] + torch.arange(columns, dtype=torch.int32, device=device)[None, :]).reshape(-1).contiguous()
     return t2, torch.arange(n, dtype=torch.int32, device=device), tokens, f2, c2
 
@@ -646,6 +658,11 @@ def attend(q, key_pages, value_pages, kind, tables, rows, starts, firsts, column
         raise ValueError("q is bf16 or fp16")
     if (offsets is None) != (tokens is None):
         raise ValueError("offsets come with the partial rows they take (tokens)")
+    if k_kind == 5:
+        place = q.get_device()
+        for x in (tables, rows, starts, firsts, counts, offsets, out, lse):
+            if x is not None and x.get_device() != place:
+                raise ValueError("attend's tensors are on q's device")
     if tables.dtype != torch.int32 or tables.stride(-1) != 1 or rows.dtype != torch.int32 or \
             starts.dtype != torch.int32 or firsts.dtype != torch.int64:
         raise ValueError("tables, rows and starts are int32, firsts int64")
@@ -720,44 +737,34 @@ def attend(q, key_pages, value_pages, kind, tables, rows, starts, firsts, column
     out = torch.empty(T, hq, dv, dtype=q.dtype, device=device) if out is None else out
     if out.dtype != q.dtype or out.stride(-1) != 1:
         raise ValueError("out is in q's dtype, its last dimension contiguous")
-    p = _lib.AttendParams()
     if engine == "even" and k_kind != 5:
         raise NotImplementedError("the even engine reads int4 pages")
-    if engine != "even" and (splits > 1 or shards is not None or sinks is not None):
-        floats = workspace_floats(partial_rows, hq, splits, dv)
-        space = _workspace(device, floats, workspace)
-        p.workspace, p.workspace_floats = _ptr(space), space.numel()
-    p.q, p.out, p.lse = _ptr(q), _ptr(out), _ptr(lse)
-    if lse is not None and (lse.dtype != torch.float32 or not lse.is_contiguous() or tuple(lse.shape) != (T, hq)):
+    if lse is not None and (lse.dtype != torch.float32 or not lse.is_contiguous() or lse.shape != (T, hq)):
         raise ValueError(f"lse is contiguous FP32 [{T}][{hq}]")
-    p.key_pages, p.value_pages = _ptr(key_pages), _ptr(value_pages)
-    p.key_scales, p.value_scales = _ptr(key_scales), _ptr(value_scales)
-    p.tables, p.rows, p.starts, p.counts = _ptr(tables), _ptr(rows), _ptr(starts), _ptr(counts)
-    p.firsts, p.offsets = _ptr(firsts), _ptr(offsets)
-    p.q_stride_token, p.q_stride_head = q.stride(0), q.stride(1)
-    p.out_stride_token, p.out_stride_head = out.stride(0), out.stride(1)
-    p.table_stride = tables.stride(0)
-    p.n_rows, p.columns, p.partial_rows = R, int(columns), partial_rows
-    p.q_heads, p.kv_heads, p.head_dim, p.value_dim, p.page = hq, hkv, d, dv, page
-    p.kind, p.page_dtype, p.q_dtype = k_kind, _page_dtype(kind, key_pages), _DTYPES[q.dtype]
-    p.chunk, p.max_splits = chunk, splits
-    p.slots = key_pages.numel() // (hkv * key_pages.shape[-1])
     if staging not in (None, "tma", "cp.async"):
         raise ValueError("staging is None, tma or cp.async")
-    p.flags = ({None: 0, "cp.async": 1, "tma": 2}[staging] | (4 if persistent else 0) |
-               {"tcgen05": 8, "mma.sync": 16, "tcgen05t": 64, "tcgen05p": 128, "even": 512}[engine] | (32 if shards is not None else 0) | (256 if context else 0))
-    p.status = _ptr(_status_word(device))
-    p.scale = float(scale if scale is not None else d ** -0.5)
-    p.key_multiplier, p.value_multiplier = float(multipliers[0]), float(multipliers[1])
-    p.parents, p.sinks, p.sliding = _ptr(parents), _ptr(sinks), sliding
-    if blocks is not None:
-        p.blocks, p.blocks_k, p.block_size = _ptr(blocks), blocks.shape[1], int(block_size)
+    space = None
+    if engine != "even" and (splits > 1 or shards is not None or sinks is not None):
+        space = _workspace(device, workspace_floats(partial_rows, hq, splits, dv), workspace)
+    columns = int(columns)
+    flags = (_STAGINGS[staging] | (4 if persistent else 0) | _ENGINES[engine] | (32 if shards is not None else 0) | (256 if context else 0))
+    p = _lib.block(_lib.AttendParams, _ptr(q), _ptr(out), _ptr(lse), _ptr(key_pages), _ptr(value_pages), _ptr(key_scales), _ptr(value_scales),
+                   _ptr(tables), _ptr(rows), _ptr(starts), _ptr(counts), _ptr(firsts), _ptr(offsets), _ptr(space), _ptr(_status_word(device)),
+                   space.numel() if space is not None else 0, key_pages.numel() // (hkv * key_pages.shape[-1]), q.stride(0), q.stride(1),
+                   out.stride(0), out.stride(1), tables.stride(0), R, columns, partial_rows, hq, hkv, d, dv, page, k_kind,
+                   _page_dtype(kind, key_pages), _DTYPES[q.dtype], chunk, splits, flags, float(scale if scale is not None else d ** -0.5),
+                   float(multipliers[0]), float(multipliers[1]), _ptr(parents), _ptr(sinks), sliding,
+                   blocks.shape[1] if blocks is not None else 0, int(block_size) if blocks is not None else 0, _ptr(blocks))
     lib = _lib.load()
     if engine == "even":
-        with torch.cuda.device(device):
-            floats = lib.crit_b200_attend_floats(ctypes.byref(p))
+        key = (device.index, R, columns, hq, hkv, d, q.dtype, parents is not None or sliding > 0 or blocks is not None)
+        floats = _even_floats.get(key)
+        if floats is None:
+            with torch.cuda.device(device):
+                floats = lib.crit_b200_attend_floats(ctypes.byref(p))
             if floats < 0:
                 _lib.check(floats, "crit_b200.attend")
+            _even_floats[key] = floats
         space = _workspace(device, floats, workspace)
         p.workspace, p.workspace_floats = _ptr(space), space.numel()
     if shards is not None:
@@ -765,15 +772,13 @@ def attend(q, key_pages, value_pages, kind, tables, rows, starts, firsts, column
             raise ValueError("a sharded context's merge writes lse too: pass lse")
         with torch.cuda.device(device):
             if launch in ("both", "decode", "push"):
-                _lib.check(lib.crit_b200_decode(ctypes.byref(p), _stream(device)), "crit_b200.attend")
+                _run("crit_b200_decode", "crit_b200.attend", device, p)
             if launch in ("both", "merge"):
                 shards.attend(p, out, lse)
             elif launch == "push":             # decode and fold + push, no wait: a measurement's
                 shards.attend(p, out, lse, wait=False)
         return out
-    call = {"both": lib.crit_b200_attend, "decode": lib.crit_b200_decode, "merge": lib.crit_b200_merge}[launch]
-    with torch.cuda.device(device):
-        _lib.check(call(ctypes.byref(p), _stream(device)), "crit_b200.attend")
+    _run({"both": "crit_b200_attend", "decode": "crit_b200_decode", "merge": "crit_b200_merge"}[launch], "crit_b200.attend", device, p)
     return out
 
 
@@ -797,8 +802,7 @@ def merge_shards(outs, lses, dtype=None):
     p = _lib.MergeShardsParams()
     p.outs, p.lses, p.out, p.lse = _ptr(outs), _ptr(lses), _ptr(out), _ptr(lse)
     p.n, p.parts, p.dim, p.in_dtype, p.out_dtype = n, parts, dim, _DTYPES[outs.dtype], _DTYPES[dtype]
-    with torch.cuda.device(outs.device):
-        _lib.check(_lib.load().crit_b200_merge_shards(ctypes.byref(p), _stream(outs.device)), "crit_b200.merge_shards")
+    _run("crit_b200_merge_shards", "crit_b200.merge_shards", outs.device, p)
     return out, lse
 
 
@@ -814,38 +818,31 @@ def _expanded(p, q, key_pages, value_pages, key_scales, value_scales, table, pos
     """4-bit pages as 16-bit ones of q's type in the workspace, one launch, in the order of the sequences' tables: (keys,
     values, the table that reads them)."""
     hkv, d = key_pages.shape[-2], q.shape[-1]
+    place = q.get_device()
     if value_scales is None or _check4(key_pages, key_scales, "keys") != (hkv, d) or _check4(value_pages, value_scales, "values") != (hkv, d) or \
-            key_pages.numel() != value_pages.numel() or key_pages.device != q.device or value_pages.device != q.device:
+            key_pages.numel() != value_pages.numel() or key_pages.get_device() != place or value_pages.get_device() != place or table.get_device() != place:
         raise ValueError(f"int4 pages hold keys and values of q's width, [...][kv_heads][{d // 2}] with their scales, on q's device")
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("q is bf16 or fp16")
     several = table.dim() == 2
     sequences, width = table.shape if several else (1, table.shape[0])
     if longest is not None:
-        width = min(width, -(-longest // page))
+        if longest > width * page:
+            raise ValueError(f"a chunk's positions go up to {longest}; its page table holds {width * page}")
+        width = -(-longest // page)
     pages = sequences * width
     half = pages * page * hkv * d // 2                                 # floats of the keys, or the values
     floats = 2 * half + pages
     # (a workspace that a launch outgrew is kept: large ones grow by powers of two)
     space = _workspace(q.device, floats if workspace is not None or floats < 1 << 24 else 1 << (floats - 1).bit_length(), workspace)
-    e = _lib.ExpandParams()
-    e.key_pages, e.value_pages, e.key_scales, e.value_scales = _ptr(key_pages), _ptr(value_pages), _ptr(key_scales), _ptr(value_scales)
-    e.tables, e.table_stride = _ptr(table), table.stride(0) if several else 0
-    if several:
-        e.positions, e.starts = p.positions, p.starts
-    elif torch.is_tensor(position):
-        e.positions = _ptr(position)
-    else:
-        e.position = int(position)
     keys = space[:half].view(q.dtype).view(pages, page, hkv, d)
     values = space[half:2 * half].view(q.dtype).view(pages, page, hkv, d)
     found = space[2 * half:2 * half + pages].view(torch.int32).view(table.shape[:-1] + (width,))
-    e.out_keys, e.out_values, e.out_tables = _ptr(keys), _ptr(values), _ptr(found)
-    e.status, e.slots_total = _ptr(_status_word(q.device)), key_pages.numel() * 2 // (hkv * d)
-    e.sequences, e.width, e.tokens, e.kv_heads, e.dim, e.page = sequences, width, tokens, hkv, d, page
-    e.out_dtype = _DTYPES[q.dtype]
-    with torch.cuda.device(q.device):
-        _lib.check(_lib.load().crit_b200_expand(ctypes.byref(e), _stream(q.device)), "crit_b200.prefill")
+    on_device = p.positions if several else (position.data_ptr() if torch.is_tensor(position) else None)
+    e = _lib.block(_lib.ExpandParams, _ptr(key_pages), _ptr(value_pages), _ptr(key_scales), _ptr(value_scales), _ptr(table), on_device, p.starts,
+                   _ptr(keys), _ptr(values), _ptr(found), _ptr(_status_word(q.device)), int(position) if on_device is None else 0,
+                   key_pages.numel() * 2 // (hkv * d), table.stride(0) if several else 0, sequences, width, tokens, hkv, d, page, _DTYPES[q.dtype])
+    _run("crit_b200_expand", "crit_b200.prefill", q.device, e)
     return keys, values, found
 
 
@@ -883,28 +880,30 @@ def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scale
     p = _lib.PrefillParams()
     longest = None if torch.is_tensor(position) or table.dim() == 2 else int(position) + T       # positions, where the host knows them
     if table.dim() == 2:             # several sequences, one launch
-        S = table.shape[0]
+        S, ahead = table.shape[0], None
         if not torch.is_tensor(position):
             if len(position) != S:
                 raise ValueError("one position a sequence")
-            longest = max((int(x) for x in position), default=0)
-            position = torch.tensor([int(x) for x in position], dtype=torch.int64, device=q.device)
+            ahead = [int(x) for x in position]
+            position = torch.tensor(ahead, dtype=torch.int64, device=q.device)
         if position.dtype != torch.int64 or position.numel() != S or not position.is_cuda or not position.is_contiguous():
             raise ValueError("the sequences' positions are an int64 tensor [S] on the device")
         if starts is None:
             if T % S:
                 raise ValueError("sequences of unequal token counts give `starts`")
             most = T // S
+            counts = [most] * S
         else:
             starts = [int(x) for x in starts]
             if len(starts) != S + 1 or starts[0] != 0 or starts[-1] != T or any(b < a for a, b in zip(starts, starts[1:])):
                 raise ValueError("starts: S + 1 rising row numbers from 0 to the number of tokens")
-            most = max(b - a for a, b in zip(starts, starts[1:]))
+            counts = [b - a for a, b in zip(starts, starts[1:])]
+            most = max(counts)
             starts = torch.tensor(starts, dtype=torch.int32, device=q.device)
             p.starts = _ptr(starts)
         p.positions, p.sequences, p.table_stride = _ptr(position), S, table.stride(0)
         T, position, held = most, 0, position
-        longest = None if longest is None else longest + most
+        longest = max((a + n for a, n in zip(ahead, counts)), default=0) if ahead is not None else None
     elif starts is not None:
         raise ValueError("starts goes with a table of several sequences")
     if torch.is_tensor(position) and (position.dtype != torch.int64 or position.numel() != 1 or not position.is_cuda):
@@ -933,6 +932,5 @@ def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scale
     p.kind, p.page_dtype, p.q_dtype = k_kind, _page_dtype(kind, key_pages), _DTYPES[q.dtype]
     p.scale = float(scale if scale is not None else d ** -0.5)
     p.key_multiplier, p.value_multiplier = float(multipliers[0]), float(multipliers[1])
-    with torch.cuda.device(q.device):
-        _lib.check(_lib.load().crit_b200_prefill(ctypes.byref(p), _stream(q.device)), "crit_b200.prefill")
+    _run("crit_b200_prefill", "crit_b200.prefill", q.device, p)
     return out

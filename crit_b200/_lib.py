@@ -1,6 +1,7 @@
 """ctypes binding of libcrit_b200.so (include/crit_b200.h).  There is no fallback: without the library every call
 raises."""
 import ctypes
+import struct
 from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
 from pathlib import Path
 
@@ -106,6 +107,16 @@ class NormRopeParams(Structure):
 
 STRUCTS = (AppendParams, GatherParams, SlotsParams, AttendParams, MergeShardsParams, PrefillParams, ExchangeParams, MoveParams,
            CompactParams, ExpandParams, NormRopeParams)
+
+_CODES = {c_void_p: "P", c_int64: "q", c_int32: "i", c_float: "f"}
+_LAYOUTS = {kind: struct.Struct("@" + "".join(_CODES[field[1]] for field in kind._fields_) + "0P") for kind in STRUCTS}
+
+
+def block(kind, *values):
+    """A parameter block from its fields' values in order (a pointer None is NULL): one pack, where a block filled field by
+    field costs a launch more host time than all its checks."""
+    return kind.from_buffer_copy(_LAYOUTS[kind].pack(*[0 if value is None else value for value in values]))
+
 
 # name -> (restype, argtypes): every symbol include/crit_b200.h declares
 SYMBOLS = {

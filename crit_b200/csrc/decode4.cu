@@ -89,11 +89,22 @@ __device__ __forceinline__ uint32_t hmul2_bits(uint32_t a, uint32_t b) {
     __half2 h = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
     return *reinterpret_cast<uint32_t*>(&h);
 }
-// D = A * B.
+// D = A * B, and D += A * B (FP16 operands, FP32 sums; not volatile: nothing but the registers is touched, and the compiler
+// may place them between the loads and the conversions).
 __device__ __forceinline__ void mma16816_new(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma16816_add(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed8(uint32_t a) {
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
 }
 // all ones in the halves that are not zero
 __device__ __forceinline__ uint32_t nonzero2(uint32_t a) { return __hne2_mask(*reinterpret_cast<__half2*>(&a), __floats2half2_rn(0.f, 0.f)); }
@@ -486,7 +497,7 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
                         for (int nt = 0; nt < NT; ++nt) {
                             float c[4];
                             mma16816_new(c, a1, qb[nt][k + o][0], qb[nt][k + o][1]);
-                            mma16816<false>(c, a2, qb[nt][k + o][2], qb[nt][k + o][3]);
+                            mma16816_add(c, a2, qb[nt][k + o][2], qb[nt][k + o][3]);
                             if (!RAW_K && k + o == 0) {
                                 x[v][nt][0] = c[0] * s.x, x[v][nt][1] = c[1] * s.x, x[v][nt][2] = c[2] * s.y, x[v][nt][3] = c[3] * s.y;
                             } else {
@@ -573,8 +584,8 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
                         w[c] = ex2(fmaf(x[v][nt][c], mul[nt][c & 1], -sub[c & 1]));
                         l_run[nt][c & 1] += w[c];
                     }
-                    pb[v][nt][0] = movmatrix_trans(pack2<false>(w[0], w[1]));
-                    pb[v][nt][1] = movmatrix_trans(pack2<false>(w[2], w[3]));
+                    pb[v][nt][0] = transposed8(pack2<false>(w[0], w[1]));
+                    pb[v][nt][1] = transposed8(pack2<false>(w[2], w[3]));
                 }
             }
 
@@ -623,10 +634,10 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
                                 b0 = hmul2_bits(b0, pair[0][k + o]), b1 = hmul2_bits(b1, pair[1][k + o]);
                                 if constexpr (GENERAL) b0 &= nonzero2(pb[v][nt][0]), b1 &= nonzero2(pb[v][nt][1]);
                             }
-                            mma16816<false>(acc[k + o][0][nt], a1, b0, b1);
-                            mma16816<false>(acc[k + o][1][nt], a2, b0, b1);
+                            mma16816_add(acc[k + o][0][nt], a1, b0, b1);
+                            mma16816_add(acc[k + o][1][nt], a2, b0, b1);
                             if constexpr (RAW_V) {
-                                mma16816<false>(acc8[k + o], eight, b0, b1);
+                                mma16816_add(acc8[k + o], eight, b0, b1);
                             }
                         }
                     }

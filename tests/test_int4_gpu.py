@@ -514,11 +514,17 @@ def test_what_the_entry_points_refuse():
     refuse({0: rows[..., :64]}, match="go to pages")
     refuse({1: rows[:2]}, match="go to pages")
     refuse({2: slots.int()}, match="int64")
+    refuse({2: slots.cpu()}, match="device")
+    refuse({3: cache.k.cpu(), 6: cache.ks.cpu()}, match="device")
     refuse({0: rows.cpu()}, RuntimeError, match="CUDA devices only")
     with pytest.raises(ValueError, match="uint8"):
         pk.gather(cache.k.view(torch.int8), "int4", 16, slots=slots, scales=cache.ks)
     with pytest.raises(ValueError, match="take scales"):
         pk.gather(cache.k, "int4", 16, slots=slots)
+    with pytest.raises(ValueError, match="device"):
+        pk.gather(cache.k, "int4", 16, slots=slots.cpu(), scales=cache.ks)
+    with pytest.raises(ValueError, match="device"):
+        _attend_with(cache, _queries(1, 32, 128, torch.bfloat16, 103), counts=torch.ones(1, dtype=torch.int32))
     for out in (torch.empty(2, 8, 128, device="cuda"), torch.empty(3, 8, 128), torch.empty(3, 128, 8, device="cuda").transpose(1, 2),
                 torch.empty(3, 8, 128, dtype=torch.float64, device="cuda")):
         with pytest.raises(ValueError, match="out is a contiguous"):

@@ -247,7 +247,7 @@ def test_what_the_entry_points_refuse():
            ((q, keys), {"positions": positions.expand(2, 3)}, "several axes"), ((q, keys), {"frequencies": frequencies.double()}, "FP32"),
            ((q, keys), {"frequencies": frequencies.cpu()}, "FP32"), ((q, keys), {"axes": frequencies.long()}, "int32"),
            ((q, keys), {"q_weight": qw[:32]}, "contiguous"), ((q, keys), {"q_weight": qw, "key_weight": kw.float()}, "one bf16"),
-           ((q, keys), {"q_out": q[:2]}, "shape"), ((q, keys), {"keys_out": keys.float()}, "shape"), ((q, None), {"keys_out": keys}, "shape"),
+           ((q, keys), {"q_out": q[:2]}, "shape"), ((q, keys), {"keys_out": keys.float()}, "shape"), ((q, None), {"keys_out": keys}, "no keys"), ((q[0], None), {}, "heads"),
            ((q, keys), {"frequencies": frequencies[:30].contiguous()}, "no kernel"), ((q, keys), {"frequencies": frequencies.repeat(2)}, "no kernel"),
            ((q[..., :40].contiguous(), None), {"frequencies": frequencies[:16].contiguous()}, "no kernel")]
     for (a, b), change, match in bad:
