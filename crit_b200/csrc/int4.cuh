@@ -30,14 +30,21 @@ __device__ __forceinline__ uint32_t int4_scale_byte(float amax, bool nan) {
 
 __device__ __forceinline__ float int4_scale(uint32_t byte) { return __half2float(__ushort_as_half((unsigned short)(byte << 7))); }
 
-// Eight elements of one group -> eight codes, element i in bits 4 i.
+// Eight elements of one group -> eight codes, element i in bits 4 i: rint(x / s), ties to even.  x is brought within 7 s first
+// (exact: s has 4 significant bits).  The quotient is Markstein's: with r the reciprocal of s rounded to nearest, q = x r is
+// corrected once by its remainder x - q s, exact in one FMA, and q + (x - q s) r is then x / s rounded to nearest, so that
+// quotients half way between two codes, common where x has few bits, come out half way.  Adding 3 * 2^22 + 8 rounds to a
+// whole number and leaves the code in the low bits.
 __device__ __forceinline__ uint32_t int4_codes(const float (&x)[8], float s) {
+    if (!(s > 0.f)) return 0x88888888u;                    // 0, or a NaN
+    const float r = __frcp_rn(s), top = 7.f * s;
     uint32_t w = 0u;
-    const bool some = s > 0.f;                    // (false for 0 and for a NaN)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float n = fminf(fmaxf(rintf(__fdiv_rn(x[i], some ? s : 1.f)), -7.f), 7.f);
-        w |= (some ? (uint32_t)((int)n + 8) : 8u) << (4 * i);
+    for (int i = 7; i >= 0; --i) {
+        const float y = fminf(fmaxf(x[i], -top), top);
+        const float q = __fmul_rn(y, r);
+        const float n = __fmaf_rn(__fmaf_rn(-q, s, y), r, q);
+        w = (w << 4) | (__float_as_uint(__fadd_rn(n, 12582920.f)) & 15u);
     }
     return w;
 }

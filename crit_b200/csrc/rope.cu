@@ -6,12 +6,14 @@
 //   (a, b) -> magnitude * (a cos - b sin, b cos + a sin)                     pairs (i, rotary / 2 + i), or (2 i, 2 i + 1)
 //   angle of pair i = positions[axes[i]][token] * frequencies[i]             (axes NULL: positions[token])
 //
-// A block takes one token, or a few where a token has few heads.  Its threads first make the tokens' sines and cosines in
-// shared memory, once for every head: the angle is a product in FP64 (a position of 2^20 times a frequency loses 2^-4 of a
-// radian in FP32), reduced to a part of a turn there and handed to sincospi in FP32.  Then 8, 16 or 32 lanes share a row of up to 64,
-// 128 or 256 elements: a lane holds four pairs, two vectors of four elements, so nothing crosses lanes but the sum of
-// squares.  A row that goes to a page is laid out again through shared memory, eight neighbouring elements a lane, and
-// encoded from its FP32 values as crit_b200_append encodes rows (16-bit pages, E4M3, INT8 and 4-bit codes).
+// A warp takes a token's heads, or a part of them where there are too few tokens to fill the device: it makes the sines and
+// cosines once (32 lanes, two pairs each of a rotation of 128; the angle is a product in FP64, since a position of 2^20 times
+// a frequency loses 2^-4 of a radian in FP32, reduced to a part of a turn there and handed to sincospi in FP32), multiplies
+// the head weights into them, and walks the queries' rows, the keys' and (when it writes) the values'.  8, 16 or 32 lanes
+// share a row of up to 64, 128 or 256 elements: a lane holds four pairs, two vectors of four elements, so nothing crosses
+// lanes but the sum of squares, and a row is in flight while the one before it is worked on.  A row that goes to a page is
+// laid out again through shared memory, eight neighbouring elements a lane, and encoded from its FP32 values as
+// crit_b200_append encodes rows (16-bit pages, E4M3, INT8 and 4-bit codes).
 // All sums are FP32; a result is rounded once.  Every element is read and written once: bound by HBM for prompt chunks, by
 // the launch for decode steps.
 #include <type_traits>
@@ -21,24 +23,7 @@
 namespace crit_b200 {
 
 constexpr int ROPE_WARPS = 8;
-constexpr int ROPE_MAX_TOKENS = 16;         // tokens a block takes
 
-template <typename T>
-__device__ __forceinline__ void load4(const T* src, float (&x)[4]) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 v = *reinterpret_cast<const float4*>(src);
-        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-    } else {
-        const uint2 v = *reinterpret_cast<const uint2*>(src);
-        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-            x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xffff0000u);
-            x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xffff0000u);
-        } else {
-            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
-            x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
-        }
-    }
-}
 template <typename T>
 __device__ __forceinline__ void store4(T* dst, const float (&x)[4]) {
     if constexpr (sizeof(T) == 4) {
@@ -47,12 +32,6 @@ __device__ __forceinline__ void store4(T* dst, const float (&x)[4]) {
         constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
         *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<BF16>(x[0], x[1]), pack2<BF16>(x[2], x[3]));
     }
-}
-
-__device__ __forceinline__ float weight_at(const void* w, int dtype, int i) {
-    if (dtype == CRIT_B200_DTYPE_BF16) return __bfloat162float(((const __nv_bfloat16*)w)[i]);
-    if (dtype == CRIT_B200_DTYPE_FP16) return __half2float(((const __half*)w)[i]);
-    return ((const float*)w)[i];
 }
 
 // A lane's eight neighbouring elements of a row (lane `part` of the row's lanes, `span` of them) into the row's page slot.
@@ -108,24 +87,87 @@ __device__ __forceinline__ void encode_row(const crit_b200_append_params& a, con
     *reinterpret_cast<uint2*>(pages + row * dim + part * 8) = make_uint2(w[0], w[1]);
 }
 
-// LANES: of a row (8, 16 or 32: the widest head has up to 8 elements a lane).
-template <typename T, int LANES, bool WRITE>
-__global__ void __launch_bounds__(ROPE_WARPS * 32) norm_rope_kernel(const crit_b200_norm_rope_params p, const crit_b200_append_params a, const int per_block) {
-    constexpr int ROWS = 32 / LANES;                         // rows a warp holds at once
-    extern __shared__ float rope_smem[];
-    float2* turns = reinterpret_cast<float2*>(rope_smem);    // [tokens of the block][rotary / 2] (cos, sin)
-    const int half = p.rotary >> 1;
-    const int64_t token0 = (int64_t)blockIdx.x * per_block;
-    const int tokens = (int)(p.tokens - token0 < per_block ? p.tokens - token0 : per_block);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane % LANES, sub = lane / LANES;
-    float* relay = rope_smem + 2 * per_block * half + (warp * ROWS + sub) * (LANES * 8 + 4);
+// Four elements as they lie in memory, and as FP32.
+template <typename T>
+struct Raw4 {
+    typename std::conditional<sizeof(T) == 4, float4, uint2>::type v;
+    __device__ __forceinline__ void load(const T* src) { v = *reinterpret_cast<const decltype(v)*>(src); }
+    __device__ __forceinline__ void floats(float (&x)[4]) const {
+        if constexpr (sizeof(T) == 4) {
+            x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+        } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xffff0000u);
+            x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xffff0000u);
+        } else {
+            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+            x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+        }
+    }
+};
 
-    for (int i = threadIdx.x; i < tokens * half; i += ROPE_WARPS * 32) {
-        const int tok = i / half, pair = i - tok * half;
+// offset + a weight's four elements from e.
+__device__ __forceinline__ void weight4(const void* weight, int dtype, int e, float offset, float (&w)[4]) {
+    if (dtype == CRIT_B200_DTYPE_FP32) {
+        const float* at = (const float*)weight + e;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = at[i];
+    } else {
+        const uint16_t* at = (const uint16_t*)weight + e;
+        uint2 v;
+        if ((reinterpret_cast<uintptr_t>(at) & 7) == 0) v = *reinterpret_cast<const uint2*>(at);
+        else v = make_uint2(at[0] | ((uint32_t)at[1] << 16), at[2] | ((uint32_t)at[3] << 16));
+        if (dtype == CRIT_B200_DTYPE_BF16) {
+            Raw4<__nv_bfloat16> raw;
+            raw.v = v, raw.floats(w);
+        } else {
+            Raw4<__half> raw;
+            raw.v = v, raw.floats(w);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] += offset;
+}
+
+// LANES: of a row (8, 16 or 32: the widest head has up to 8 elements a lane).  parts: warps that share a token.
+template <typename T, int LANES, bool WRITE>
+__global__ void __launch_bounds__(ROPE_WARPS * 32) norm_rope_kernel(const crit_b200_norm_rope_params p, const crit_b200_append_params a, const int parts,
+                                                                    const float inv_dim) {
+    constexpr int ROWS = 32 / LANES;                         // rows a warp holds at once
+    __shared__ float2 turns_mem[ROPE_WARPS][128];            // (cos, sin) of the warp's token
+    __shared__ __align__(16) float relay_mem[WRITE ? ROPE_WARPS * ROWS : 1][WRITE ? LANES * 8 + 4 : 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane % LANES, sub = lane / LANES;
+    const int64_t job = (int64_t)blockIdx.x * ROPE_WARPS + warp;
+    const int64_t t = job / parts;
+    if (t >= p.tokens) return;                               // (no barrier of the block follows)
+    const int piece = (int)(job - t * parts);
+    const int half = p.rotary >> 1;
+    float2* turns = turns_mem[warp];
+
+    // the lane's two vectors of four elements in a row: of a turned chunk the pairs' halves (or four neighbouring pairs), of
+    // the rest eight neighbours
+    const bool turned = part * 4 < half;
+    const int e0 = turned ? (p.interleaved ? part * 8 : part * 4) : p.rotary + (part - (half >> 2)) * 8;
+    const int e1 = turned && !p.interleaved ? half + part * 4 : e0 + 4;
+    const bool inside = part * 8 < p.head_dim;
+
+    // this warp's share of the token's rows, the queries' first, then the keys', then the values'
+    const int row_heads = p.q_heads + p.kv_heads + (WRITE && a.values ? p.kv_heads : 0);
+    const int share = (row_heads + parts - 1) / parts, begin = piece * share, end = begin + share;
+    const int q0 = begin < p.q_heads ? begin : p.q_heads, q1 = end < p.q_heads ? end : p.q_heads;
+    auto within = [&](int x) { x -= p.q_heads; return x < 0 ? 0 : (x > p.kv_heads ? p.kv_heads : x); };
+    const int k0 = within(begin), k1 = within(end), v0 = within(begin - p.kv_heads), v1 = WRITE && a.values ? within(end - p.kv_heads) : 0;
+
+    const T* q_row = (const T*)p.q + t * p.q_stride_token + (int64_t)(q0 + sub) * p.q_stride_head;
+    const T* k_row = (const T*)p.keys + t * p.key_stride_token + (int64_t)(k0 + sub) * p.key_stride_head;
+    Raw4<T> ra, rb, ka, kb;                                  // the first rows are asked for before the sines are made
+    if (inside && q0 + sub < q1) ra.load(q_row + e0), rb.load(q_row + e1);
+    if (inside && k0 + sub < k1) ka.load(k_row + e0), kb.load(k_row + e1);
+
+    for (int pair = lane; pair < half; pair += 32) {
         const int axis = p.axes ? p.axes[pair] : 0;
         float2 turn = make_float2(0.f, 0.f);
         if (axis >= 0 && axis < p.n_axes) {
-            const double at = (double)p.positions[(int64_t)axis * p.axis_stride + token0 + tok] * (double)p.frequencies[pair];
+            const double at = (double)p.positions[(int64_t)axis * p.axis_stride + t] * (double)p.frequencies[pair];
             // at / (2 pi) less its whole turns: 1 / (2 pi) as a sum of two FP64 numbers, the product's rounding put back
             const double turns_of = at * 0.15915494309189535;
             const double rest = fma(at, 0.15915494309189535, -turns_of) + at * -9.839338337591243e-18;
@@ -135,94 +177,128 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32) norm_rope_kernel(const crit_b
         } else if (p.status) {
             atomicExch(p.status, CRIT_B200_STATUS_BOUNDS);   // an axis that positions has not: the pair becomes zeros
         }
-        turns[i] = turn;
+        turns[pair] = turn;
     }
-    __syncthreads();
+    __syncwarp();
 
-    const int row_heads = p.q_heads + p.kv_heads + (WRITE && a.values ? p.kv_heads : 0);
-    const int rows = tokens * row_heads;
-    for (int row0 = warp * ROWS; row0 < rows; row0 += ROPE_WARPS * ROWS) {
-        const int row = row0 + sub;
-        const bool here = row < rows;
-        const int tok = here ? row / row_heads : 0;
-        const int head = row - tok * row_heads;
-        const bool is_q = head < p.q_heads, is_v = head >= p.q_heads + p.kv_heads;
-        const int h = is_q ? head : (is_v ? head - p.q_heads - p.kv_heads : head - p.q_heads);
-        const int64_t t = token0 + tok;
-        const int dim = is_v ? a.value_dim : p.head_dim;
-        // the lane's two vectors of four elements: of a turned chunk the pairs' halves (or four neighbouring pairs)
-        const bool turned = !is_v && part * 4 < half;
-        const int e0 = turned ? (p.interleaved ? part * 8 : part * 4) : (is_v ? part * 8 : p.rotary + (part - (half >> 2)) * 8);
-        const int e1 = turned && !p.interleaved ? half + part * 4 : e0 + 4;
-        const bool live = here && part * 8 < dim;
-        float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-        if (live) {
-            const T* src = is_q ? (const T*)p.q + t * p.q_stride_token + (int64_t)h * p.q_stride_head
-                                : (is_v ? (const T*)a.values + t * a.value_stride_token + (int64_t)h * a.value_stride_head
-                                        : (const T*)p.keys + t * p.key_stride_token + (int64_t)h * p.key_stride_head);
-            load4<T>(src + e0, x);
-            load4<T>(src + e1, y);
-        }
-        const void* weight = is_q ? p.q_weight : (is_v ? nullptr : p.key_weight);
-        float sum = 0.f;
+    // A result is an element and its partner times two factors: the first vector's own and partner's, the second's own and
+    // partner's (cos and sin with the head's weights; 1 and 0 past the rotation).
+    float own0[4], other0[4], own1[4], other1[4];
+    auto factors = [&](const void* weight) {
+        float w0[4] = {1.f, 1.f, 1.f, 1.f}, w1[4] = {1.f, 1.f, 1.f, 1.f};
+        if (weight && inside) weight4(weight, p.weight_dtype, e0, p.offset, w0), weight4(weight, p.weight_dtype, e1, p.offset, w1);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum = fmaf(x[i], x[i], fmaf(y[i], y[i], sum));
-#pragma unroll
-        for (int o = 1; o < LANES; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (weight && live) {
-            const float inv = 1.f / sqrtf(sum / (float)dim + p.eps);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[i] *= inv * (p.offset + weight_at(weight, p.weight_dtype, e0 + i));
-                y[i] *= inv * (p.offset + weight_at(weight, p.weight_dtype, e1 + i));
-            }
-        }
-        if (turned && live) {
-            const float2* turn = turns + tok * half + part * 4;
-            if (p.interleaved) {
-#pragma unroll
-                for (int i = 0; i < 4; i += 2) {
-                    const float2 u = turn[i >> 1], v = turn[2 + (i >> 1)];
-                    const float xa = x[i], ya = y[i];
-                    x[i] = xa * u.x - x[i + 1] * u.y, x[i + 1] = x[i + 1] * u.x + xa * u.y;
-                    y[i] = ya * v.x - y[i + 1] * v.y, y[i + 1] = y[i + 1] * v.x + ya * v.y;
-                }
+        for (int i = 0; i < 4; ++i) {
+            if (!turned) {
+                own0[i] = w0[i], own1[i] = w1[i], other0[i] = other1[i] = 0.f;
+            } else if (p.interleaved) {
+                const float2 u = turns[part * 4 + (i >> 1)], v = turns[part * 4 + 2 + (i >> 1)];
+                own0[i] = u.x * w0[i], other0[i] = (i & 1 ? u.y : -u.y) * w0[i ^ 1];
+                own1[i] = v.x * w1[i], other1[i] = (i & 1 ? v.y : -v.y) * w1[i ^ 1];
             } else {
+                const float2 u = turns[part * 4 + i];
+                own0[i] = u.x * w0[i], other0[i] = -u.y * w1[i];
+                own1[i] = u.x * w1[i], other1[i] = u.y * w0[i];
+            }
+        }
+    };
+    auto turn_row = [&](float (&x)[4], float (&y)[4], bool normed) {
+        float inv = 1.f;
+        if (normed) {
+            float sum = 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 u = turn[i];
-                    const float xa = x[i];
-                    x[i] = xa * u.x - y[i] * u.y, y[i] = y[i] * u.x + xa * u.y;
+            for (int i = 0; i < 4; ++i) sum = fmaf(x[i], x[i], fmaf(y[i], y[i], sum));
+#pragma unroll
+            for (int o = 1; o < LANES; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            inv = rsqrtf(fmaf(sum, inv_dim, p.eps));
+        }
+        float u[4], v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float partner0 = p.interleaved ? x[i ^ 1] : y[i], partner1 = p.interleaved ? y[i ^ 1] : x[i];
+            u[i] = fmaf(partner0, other0[i], x[i] * own0[i]) * inv, v[i] = fmaf(partner1, other1[i], y[i] * own1[i]) * inv;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = u[i], y[i] = v[i];
+    };
+
+    // -- the queries' rows --------------------------------------------------------------------------------------------------
+    if (q0 < q1) {
+        factors(p.q_weight);
+        T* out = (T*)p.q_out + t * p.q_out_stride_token + (int64_t)(q0 + sub) * p.q_out_stride_head;
+        for (int h = q0; h < q1; h += ROWS) {                // (the same for every lane; a lane's own row is h + sub)
+            float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+            const bool live = inside && h + sub < q1;
+            if (live) ra.floats(x), rb.floats(y);
+            q_row += ROWS * p.q_stride_head;
+            if (inside && h + ROWS + sub < q1) ra.load(q_row + e0), rb.load(q_row + e1);
+            turn_row(x, y, p.q_weight != nullptr);
+            if (live) store4<T>(out + e0, x), store4<T>(out + e1, y);
+            out += ROWS * p.q_out_stride_head;
+        }
+    }
+
+    // -- the keys' rows, and their pages -------------------------------------------------------------------------------------
+    int64_t slot = -1;
+    if (WRITE && (k0 < k1 || v0 < v1)) {
+        slot = a.slots[t];
+        if (slot >= 0 && a.slots_total && slot >= a.slots_total) {       // outside the page tensor: skipped and reported
+            if (lane == 0 && a.status) atomicExch(a.status, CRIT_B200_STATUS_BOUNDS);
+            slot = -1;
+        }
+    }
+    if (k0 < k1) {
+        factors(p.key_weight);
+        T* out = p.keys_out ? (T*)p.keys_out + t * p.key_out_stride_token + (int64_t)(k0 + sub) * p.key_out_stride_head : nullptr;
+        for (int h = k0; h < k1; h += ROWS) {
+            float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+            const bool live = inside && h + sub < k1;
+            if (live) ka.floats(x), kb.floats(y);
+            k_row += ROWS * p.key_stride_head;
+            if (inside && h + ROWS + sub < k1) ka.load(k_row + e0), kb.load(k_row + e1);
+            turn_row(x, y, p.key_weight != nullptr);
+            if (out) {
+                if (live) store4<T>(out + e0, x), store4<T>(out + e1, y);
+                out += ROWS * p.key_out_stride_head;
+            }
+            if constexpr (WRITE) {
+                if (slot < 0) continue;                      // (the warp's token: the same for every lane)
+                float* relay = relay_mem[warp * ROWS + sub];  // the row as eight neighbouring elements a lane
+                if (live) {
+                    *reinterpret_cast<float4*>(relay + e0) = make_float4(x[0], x[1], x[2], x[3]);
+                    *reinterpret_cast<float4*>(relay + e1) = make_float4(y[0], y[1], y[2], y[3]);
                 }
+                __syncwarp();
+                float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (live) {
+                    const float4 u = *reinterpret_cast<const float4*>(relay + part * 8), v = *reinterpret_cast<const float4*>(relay + part * 8 + 4);
+                    z[0] = u.x, z[1] = u.y, z[2] = u.z, z[3] = u.w, z[4] = v.x, z[5] = v.y, z[6] = v.z, z[7] = v.w;
+                }
+                __syncwarp();
+                encode_row(a, z, live, false, slot, h + sub, p.head_dim, part, LANES);
             }
         }
-        T* out = is_q ? (T*)p.q_out : (is_v ? nullptr : (T*)p.keys_out);
-        if (out && live) {
-            out += t * (is_q ? p.q_out_stride_token : p.key_out_stride_token) + (int64_t)h * (is_q ? p.q_out_stride_head : p.key_out_stride_head);
-            store4<T>(out + e0, x);
-            store4<T>(out + e1, y);
-        }
-        if constexpr (WRITE) {
-            if (__all_sync(0xffffffffu, is_q || !here)) continue;
-            // the row as eight neighbouring elements a lane, and into its page
-            if (live && !is_q) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) relay[e0 + i] = x[i], relay[e1 + i] = y[i];
+    }
+
+    // -- the values' rows go to their pages as they are ----------------------------------------------------------------------
+    if (WRITE && v0 < v1 && slot >= 0) {
+        const bool held = part * 8 < a.value_dim;
+        const T* v_row = (const T*)a.values + t * a.value_stride_token + (int64_t)(v0 + sub) * a.value_stride_head + part * 8;
+        for (int h = v0; h < v1; h += ROWS) {
+            float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            const bool live = held && h + sub < v1;
+            if (live) {
+                Raw4<T> va, vb;
+                va.load(v_row), vb.load(v_row + 4);
+                va.floats(reinterpret_cast<float(&)[4]>(z[0])), vb.floats(reinterpret_cast<float(&)[4]>(z[4]));
             }
-            __syncwarp();
-            float z[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) z[i] = live && !is_q ? relay[part * 8 + i] : 0.f;
-            __syncwarp();
-            const int64_t slot = here && !is_q ? a.slots[t] : -1;
-            const bool outside = slot >= 0 && a.slots_total && slot >= a.slots_total;
-            if (outside && part == 0 && a.status) atomicExch(a.status, CRIT_B200_STATUS_BOUNDS);
-            encode_row(a, z, live && slot >= 0 && !outside, is_v, slot, h, dim, part, LANES);
+            v_row += ROWS * a.value_stride_head;
+            encode_row(a, z, live, true, slot, h + sub, a.value_dim, part, LANES);
         }
     }
 }
 
-typedef void (*norm_rope_fn)(const crit_b200_norm_rope_params, const crit_b200_append_params, const int);
+typedef void (*norm_rope_fn)(const crit_b200_norm_rope_params, const crit_b200_append_params, const int, const float);
 
 template <typename T, bool WRITE>
 static norm_rope_fn norm_rope_lanes(int width) {
@@ -269,18 +345,21 @@ extern "C" __attribute__((visibility("default"))) int crit_b200_norm_rope(const 
             width = a.value_dim > width ? a.value_dim : width;
         }
     }
+    // Warps a token: one for a prompt of many tokens (a token's sines are made once), as many as it has rows for a step's few,
+    // so that the launch has four times the warps that the device holds or a warp an iteration.
     const int row_heads = p.q_heads + p.kv_heads + (a.values ? p.kv_heads : 0);
-    int per_block = 32 / row_heads;                                                        // a few rows a warp at least
-    per_block = per_block < 1 ? 1 : (per_block > ROPE_MAX_TOKENS ? ROPE_MAX_TOKENS : per_block);
-    const int lanes = width <= 64 ? 8 : (width <= 128 ? 16 : 32);
-    const int smem = per_block * (p.rotary >> 1) * 8 + (append ? ROPE_WARPS * (32 / lanes) * (lanes * 8 + 4) * 4 : 0);
-    const int64_t blocks = (p.tokens + per_block - 1) / per_block;
+    const int rows_at_once = 32 / (width <= 64 ? 8 : (width <= 128 ? 16 : 32)), most = (row_heads + rows_at_once - 1) / rows_at_once;
+    int device = 0, sms = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) sms = 1;
+    const int64_t wanted = ((int64_t)sms * 128 + p.tokens - 1) / p.tokens;
+    const int parts = (int)(wanted < most ? wanted : most);
+    const int64_t blocks = (p.tokens * parts + ROPE_WARPS - 1) / ROPE_WARPS;
     if (blocks > 0x7fffffffLL) return CRIT_B200_EINVAL;
     norm_rope_fn fn;
     if (p.dtype == CRIT_B200_DTYPE_BF16) fn = norm_rope_pick<__nv_bfloat16>(width, append != nullptr);
     else if (p.dtype == CRIT_B200_DTYPE_FP16) fn = norm_rope_pick<__half>(width, append != nullptr);
     else fn = norm_rope_pick<float>(width, append != nullptr);
-    fn<<<(unsigned)blocks, ROPE_WARPS * 32, smem, (cudaStream_t)stream>>>(p, a, per_block);
+    fn<<<(unsigned)blocks, ROPE_WARPS * 32, 0, (cudaStream_t)stream>>>(p, a, parts, 1.f / (float)p.head_dim);
     CRIT_CHECK_LAUNCH();
     return 0;
 }
