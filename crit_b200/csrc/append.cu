@@ -219,44 +219,63 @@ __device__ __forceinline__ void load8(const TIN* src, float (&x)[8]) {
 }
 
 // 4-bit rows.  Four lanes serve a group of 32 elements of one (token, kv head) of the keys or the values: 8 elements a
-// lane in one 16-byte load, the group's maximum by two shuffles, 8 codes in one 4-byte store.  Every byte is read and
-// written once; bound by HBM for prompt chunks, by the launch for decode steps.
-template <typename TIN>
-__global__ void __launch_bounds__(256) append4_kernel(const crit_b200_append_params p, const int per_head, const int key_groups,
-                                                      const int per_token) {
-    const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 2;         // a group; the last quads have none
+// lane in one 16-byte load, the group's maximum by two shuffles, 8 codes in one 4-byte store.  A block takes 64 groups of a
+// token, or a few tokens of fewer groups (grid: tokens, parts of a token), so that no index needs a 64-bit division, and does so
+// for TOKENS tokens in turn, whose loads are in flight together.  Every byte is read and written once.
+template <typename TIN, int TOKENS>
+__global__ void __launch_bounds__(256) append4_kernel(const crit_b200_append_params p, const int key_groups, const int per_token, const int per_block,
+                                                      const uint32_t magic_k, const uint32_t magic_v) {
+    const uint32_t item = threadIdx.x >> 2;                                      // a group of the block; some quads may have none
     const int part = threadIdx.x & 3;
-    const int64_t t = item / per_token;
-    int g = (int)(item - t * per_token);
+    const uint32_t tok = per_block > 1 ? item / (uint32_t)per_token : 0u;
+    int g = (int)(item - tok * (uint32_t)per_token) + blockIdx.y * 64;
+    const bool none = (int)tok >= per_block || g >= per_token;
     const bool is_v = g >= key_groups;
     if (is_v) g -= key_groups;
-    const int groups = is_v ? p.value_dim >> 5 : per_head;
-    const int h = g / groups;
-    g -= h * groups;
-    const int64_t slot = t < p.tokens ? p.slots[t] : -1;
-    const bool outside = slot >= 0 && p.slots_total && slot >= p.slots_total;    // skipped and reported, never written
-    if (outside && part == 0 && p.status) atomicExch(p.status, CRIT_B200_STATUS_BOUNDS);
-    const bool live = slot >= 0 && !outside;
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (live) {
-        const TIN* src = is_v ? (const TIN*)p.values + t * p.value_stride_token + (int64_t)h * p.value_stride_head
-                              : (const TIN*)p.keys + t * p.key_stride_token + (int64_t)h * p.key_stride_head;
-        load8<TIN>(src + g * 32 + part * 8, x);
+    const int groups = (is_v ? p.value_dim : p.head_dim) >> 5;
+    const int h = (int)(((uint32_t)g * (is_v ? magic_v : magic_k)) >> 16);      // g / groups
+    const TIN* src = is_v ? (const TIN*)p.values + (int64_t)h * p.value_stride_head : (const TIN*)p.keys + (int64_t)h * p.key_stride_head;
+    src += (g - h * groups) * 32 + part * 8;
+    const int64_t stride = is_v ? p.value_stride_token : p.key_stride_token;
+    const int row = p.kv_heads * groups;                                        // groups of a slot
+    const int64_t t0 = (int64_t)blockIdx.x * (per_block * TOKENS) + tok;
+    int64_t slot[TOKENS];
+    float x[TOKENS][8];
+#pragma unroll
+    for (int u = 0; u < TOKENS; ++u) {
+        const int64_t t = t0 + u * per_block;
+        slot[u] = !none && t < p.tokens ? p.slots[t] : -1;
+        if (slot[u] >= 0 && p.slots_total && slot[u] >= p.slots_total) {         // outside the page tensor: skipped and reported
+            if (part == 0 && p.status) atomicExch(p.status, CRIT_B200_STATUS_BOUNDS);
+            slot[u] = -1;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
+        if (!none && t < p.tokens) load8<TIN>(src + t * stride, x[u]);
     }
-    uint32_t byte;
-    const uint32_t w = int4_quantise(x, byte);
-    if (!live) return;
-    const int64_t at = (slot * p.kv_heads + h) * groups + g;
-    reinterpret_cast<uint32_t*>(is_v ? p.value_pages : p.key_pages)[at * 4 + part] = w;
-    if (part == 0) reinterpret_cast<uint8_t*>(is_v ? p.value_scales : p.key_scales)[at] = (uint8_t)byte;
+#pragma unroll
+    for (int u = 0; u < TOKENS; ++u) {
+        uint32_t byte;
+        const uint32_t w = int4_quantise(x[u], byte);
+        if (slot[u] < 0) continue;
+        const int64_t at = slot[u] * row + g;
+        reinterpret_cast<uint32_t*>(is_v ? p.value_pages : p.key_pages)[at * 4 + part] = w;
+        if (part == 0) reinterpret_cast<uint8_t*>(is_v ? p.value_scales : p.key_scales)[at] = (uint8_t)byte;
+    }
 }
 
 template <typename TIN>
 static void launch_append4(const crit_b200_append_params& p, cudaStream_t s) {
-    const int per_head = p.head_dim >> 5, key_groups = p.kv_heads * per_head;
-    const int per_token = key_groups + (p.values ? p.kv_heads * (p.value_dim >> 5) : 0);
-    const int64_t quads = p.tokens * per_token;
-    append4_kernel<TIN><<<(unsigned)((quads + 63) / 64), 256, 0, s>>>(p, per_head, key_groups, per_token);
+    const int groups_k = p.head_dim >> 5, groups_v = p.values ? p.value_dim >> 5 : 1;
+    const int key_groups = p.kv_heads * groups_k, per_token = key_groups + (p.values ? p.kv_heads * groups_v : 0);
+    const int per_block = per_token < 64 ? 64 / per_token : 1, parts = (per_token + 63) / 64;
+    // g / groups as (g * ceil(2^16 / groups)) >> 16: exact for g below 2^13 (the excess is below 8 / 2^16 a unit)
+    const uint32_t magic_k = (65536u + groups_k - 1) / groups_k, magic_v = (65536u + groups_v - 1) / groups_v;
+    // several tokens a block once one each would be more blocks than the device holds several times over
+    const int64_t blocks = (p.tokens + per_block - 1) / per_block;
+    if (blocks * parts >= 4096)
+        append4_kernel<TIN, 4><<<dim3((unsigned)((blocks + 3) / 4), (unsigned)parts), 256, 0, s>>>(p, key_groups, per_token, per_block, magic_k, magic_v);
+    else append4_kernel<TIN, 1><<<dim3((unsigned)blocks, (unsigned)parts), 256, 0, s>>>(p, key_groups, per_token, per_block, magic_k, magic_v);
 }
 
 int check_append(const crit_b200_append_params& p) {
@@ -265,6 +284,7 @@ int check_append(const crit_b200_append_params& p) {
     auto width_ok = [](int d) { return d >= 32 && d <= 256 && d % 32 == 0; };
     if (!width_ok(p.head_dim) || (p.values && !width_ok(p.value_dim))) return CRIT_B200_EUNSUPPORTED;
     if (p.kind < 0 || p.kind > CRIT_B200_KIND_INT4) return CRIT_B200_EUNSUPPORTED;
+    if (p.kind == CRIT_B200_KIND_INT4 && (int64_t)p.kv_heads * (p.head_dim > p.value_dim ? p.head_dim : p.value_dim) >= 32 * 8192) return CRIT_B200_EUNSUPPORTED;
     if (p.kind == CRIT_B200_KIND_INT4 && (!aligned(p.key_pages, 4) || (p.values && !aligned(p.value_pages, 4)))) return CRIT_B200_EALIGN;
     if (p.kind >= CRIT_B200_KIND_FP8_ROW && (!p.key_scales || (p.values && !p.value_scales))) return CRIT_B200_EINVAL;
     if (p.kind == CRIT_B200_KIND_16BIT && p.page_dtype == CRIT_B200_DTYPE_FP32 && p.in_dtype != CRIT_B200_DTYPE_FP32)

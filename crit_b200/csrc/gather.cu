@@ -43,34 +43,53 @@ __global__ void __launch_bounds__(128) gather_kernel(const crit_b200_gather_para
 }
 
 // 4-bit rows back: a thread takes 8 codes (one 4-byte load) to 8 values, (code - 8) * scale in FP32 (exact), in one 16-byte
-// store for 16-bit types.  Bound by the bytes it writes.
-template <typename TOUT>
-__global__ void __launch_bounds__(256) gather4_kernel(const crit_b200_gather_params p, const int words) {
-    const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;                // a word of 8 codes; words: those of one position
-    if (item >= p.count * words) return;
-    const int64_t n = item / words;
-    const int w = (int)(item - n * words);
-    const int64_t slot = p.slots ? p.slots[n] : (int64_t)p.table[n / p.page] * p.page + n % p.page;
-    float v[8];
-    if (p.slots_total && (slot < 0 || slot >= p.slots_total)) {      // outside the page tensor: zeros, and reported
-        if (w == 0 && p.status) atomicExch(p.status, CRIT_B200_STATUS_BOUNDS);
+// store for 16-bit types.  A block takes 256 words of a position, or a few positions of fewer words, and does so for
+// POSITIONS positions in turn, whose loads are in flight together.  Bound by the bytes it writes.
+template <typename TOUT, int POSITIONS>
+__global__ void __launch_bounds__(256) gather4_kernel(const crit_b200_gather_params p, const int words, const int per_block) {
+    const uint32_t tok = per_block > 1 ? threadIdx.x / (uint32_t)words : 0u;
+    const int w = (int)(threadIdx.x - tok * words) + blockIdx.y * 256;            // the word of 8 codes among the position's
+    if ((int)tok >= per_block || w >= words) return;
+    const int64_t n0 = (int64_t)blockIdx.x * (per_block * POSITIONS) + tok;
+    uint32_t codes[POSITIONS], byte[POSITIONS];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.f;
-    } else {
+    for (int u = 0; u < POSITIONS; ++u) {
+        const int64_t n = n0 + u * per_block;
+        codes[u] = 0x88888888u, byte[u] = 0u;
+        if (n >= p.count) continue;
+        const int64_t slot = p.slots ? p.slots[n] : (int64_t)p.table[n / p.page] * p.page + n % p.page;
+        if (p.slots_total && (slot < 0 || slot >= p.slots_total)) {      // outside the page tensor: zeros, and reported
+            if (w == 0 && p.status) atomicExch(p.status, CRIT_B200_STATUS_BOUNDS);
+            continue;
+        }
         const int64_t at = slot * words + w;
-        const uint32_t codes = reinterpret_cast<const uint32_t*>(p.pages)[at];
-        const float s = int4_scale(reinterpret_cast<const uint8_t*>(p.scales)[at >> 2]);
+        codes[u] = reinterpret_cast<const uint32_t*>(p.pages)[at];
+        byte[u] = reinterpret_cast<const uint8_t*>(p.scales)[at >> 2];
+    }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __fmul_rn((float)((int)((codes >> (4 * i)) & 15u) - 8), s);
+    for (int u = 0; u < POSITIONS; ++u) {
+        const int64_t n = n0 + u * per_block;
+        if (n >= p.count) return;
+        float v[8];
+        int4_values(codes[u], int4_scale(byte[u]), v);
+        TOUT* dst = (TOUT*)p.out + (n * words + w) * 8;
+        if constexpr (sizeof(TOUT) == 2) {
+            constexpr bool BF16 = std::is_same<TOUT, __nv_bfloat16>::value;
+            *reinterpret_cast<uint4*>(dst) = make_uint4(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]), pack2<BF16>(v[4], v[5]), pack2<BF16>(v[6], v[7]));
+        } else {
+            *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        }
     }
-    TOUT* dst = (TOUT*)p.out + item * 8;
-    if constexpr (sizeof(TOUT) == 2) {
-        constexpr bool BF16 = std::is_same<TOUT, __nv_bfloat16>::value;
-        *reinterpret_cast<uint4*>(dst) = make_uint4(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]), pack2<BF16>(v[4], v[5]), pack2<BF16>(v[6], v[7]));
-    } else {
-        *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
-    }
+}
+
+template <typename TOUT>
+static void launch_gather4(const crit_b200_gather_params& p, int words, cudaStream_t s) {
+    const int per_block = words < 256 ? 256 / words : 1;
+    const unsigned parts = (unsigned)((words + 255) / 256);
+    const int64_t blocks = (p.count + per_block - 1) / per_block;
+    if (blocks * parts >= 4096) gather4_kernel<TOUT, 4><<<dim3((unsigned)((blocks + 3) / 4), parts), 256, 0, s>>>(p, words, per_block);
+    else gather4_kernel<TOUT, 1><<<dim3((unsigned)blocks, parts), 256, 0, s>>>(p, words, per_block);
 }
 
 // The sequences' 4-bit pages as 16-bit ones, in the order of their tables: block = (page of the table, sequence, keys or
@@ -97,8 +116,7 @@ __global__ void __launch_bounds__(256) expand4_kernel(const crit_b200_expand_par
         const uint32_t w = codes[i];
         const float f = int4_scale(scales[i >> 2]);
         float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = __fmul_rn((float)((int)((w >> (4 * e)) & 15u) - 8), f);
+        int4_values(w, f, v);
         if constexpr (!BF16) {                     // (a scale above FP16's range over 7: its largest number, not infinity)
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = v[e] > 65504.f ? 65504.f : (v[e] < -65504.f ? -65504.f : v[e]);
@@ -163,11 +181,10 @@ extern "C" __attribute__((visibility("default"))) int crit_b200_gather(const cri
         if (p.dim % 32) return CRIT_B200_EUNSUPPORTED;
         if (!aligned(p.pages, 4) || !aligned(p.out, 16)) return CRIT_B200_EALIGN;
         const int words = p.kv_heads * (p.dim >> 3);
-        const unsigned blocks = (unsigned)((p.count * words + 255) / 256);
         switch (p.out_dtype) {
-            case CRIT_B200_DTYPE_BF16: gather4_kernel<__nv_bfloat16><<<blocks, 256, 0, (cudaStream_t)stream>>>(p, words); break;
-            case CRIT_B200_DTYPE_FP16: gather4_kernel<__half><<<blocks, 256, 0, (cudaStream_t)stream>>>(p, words); break;
-            case CRIT_B200_DTYPE_FP32: gather4_kernel<float><<<blocks, 256, 0, (cudaStream_t)stream>>>(p, words); break;
+            case CRIT_B200_DTYPE_BF16: launch_gather4<__nv_bfloat16>(p, words, (cudaStream_t)stream); break;
+            case CRIT_B200_DTYPE_FP16: launch_gather4<__half>(p, words, (cudaStream_t)stream); break;
+            case CRIT_B200_DTYPE_FP32: launch_gather4<float>(p, words, (cudaStream_t)stream); break;
             default: return CRIT_B200_EINVAL;
         }
         CRIT_CHECK_LAUNCH();

@@ -23,6 +23,7 @@
 namespace crit_b200 {
 
 constexpr int ROPE_WARPS = 8;
+constexpr int ROPE_FILL = 32;               // warps an SM that a launch of few tokens is to have
 
 template <typename T>
 __device__ __forceinline__ void store4(T* dst, const float (&x)[4]) {
@@ -36,7 +37,7 @@ __device__ __forceinline__ void store4(T* dst, const float (&x)[4]) {
 
 // A lane's eight neighbouring elements of a row (lane `part` of the row's lanes, `span` of them) into the row's page slot.
 // Every lane of the warp comes here: lanes without elements (or whose row is not written) with live false.
-__device__ __forceinline__ void encode_row(const crit_b200_append_params& a, const float (&x)[8], bool live, bool is_v, int64_t slot, int h,
+__device__ __forceinline__ void encode_row(const crit_b200_append_params& a, float (&x)[8], bool live, bool is_v, int64_t slot, int h,
                                            int dim, int part, int span) {
     const int64_t row = slot * a.kv_heads + h;
     char* pages = (char*)(is_v ? a.value_pages : a.key_pages);
@@ -128,12 +129,14 @@ __device__ __forceinline__ void weight4(const void* weight, int dtype, int e, fl
     for (int i = 0; i < 4; ++i) w[i] += offset;
 }
 
-// LANES: of a row (8, 16 or 32: the widest head has up to 8 elements a lane).  parts: warps that share a token.
-template <typename T, int LANES, bool WRITE>
-__global__ void __launch_bounds__(ROPE_WARPS * 32) norm_rope_kernel(const crit_b200_norm_rope_params p, const crit_b200_append_params a, const int parts,
+// LANES: of a row (8, 16 or 32: the widest head has up to 8 elements a lane).  NEIGHBOURS: pairs (2 i, 2 i + 1).  parts: warps that
+// share a token.
+template <typename T, int LANES, bool WRITE, bool NEIGHBOURS>
+__global__ void __launch_bounds__(ROPE_WARPS * 32, 4) norm_rope_kernel(const crit_b200_norm_rope_params p, const crit_b200_append_params a, const int parts,
                                                                     const float inv_dim) {
     constexpr int ROWS = 32 / LANES;                         // rows a warp holds at once
-    __shared__ float2 turns_mem[ROPE_WARPS][128];            // (cos, sin) of the warp's token
+    constexpr int DEPTH = 3;
+    __shared__ __align__(16) float2 turns_mem[ROPE_WARPS][128];            // (cos, sin) of the warp's token
     __shared__ __align__(16) float relay_mem[WRITE ? ROPE_WARPS * ROWS : 1][WRITE ? LANES * 8 + 4 : 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane % LANES, sub = lane / LANES;
     const int64_t job = (int64_t)blockIdx.x * ROPE_WARPS + warp;
@@ -146,8 +149,8 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32) norm_rope_kernel(const crit_b
     // the lane's two vectors of four elements in a row: of a turned chunk the pairs' halves (or four neighbouring pairs), of
     // the rest eight neighbours
     const bool turned = part * 4 < half;
-    const int e0 = turned ? (p.interleaved ? part * 8 : part * 4) : p.rotary + (part - (half >> 2)) * 8;
-    const int e1 = turned && !p.interleaved ? half + part * 4 : e0 + 4;
+    const int e0 = turned ? (NEIGHBOURS ? part * 8 : part * 4) : p.rotary + (part - (half >> 2)) * 8;
+    const int e1 = turned && !NEIGHBOURS ? half + part * 4 : e0 + 4;
     const bool inside = part * 8 < p.head_dim;
 
     // this warp's share of the token's rows, the queries' first, then the keys', then the values'
@@ -157,11 +160,15 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32) norm_rope_kernel(const crit_b
     auto within = [&](int x) { x -= p.q_heads; return x < 0 ? 0 : (x > p.kv_heads ? p.kv_heads : x); };
     const int k0 = within(begin), k1 = within(end), v0 = within(begin - p.kv_heads), v1 = WRITE && a.values ? within(end - p.kv_heads) : 0;
 
-    const T* q_row = (const T*)p.q + t * p.q_stride_token + (int64_t)(q0 + sub) * p.q_stride_head;
-    const T* k_row = (const T*)p.keys + t * p.key_stride_token + (int64_t)(k0 + sub) * p.key_stride_head;
-    Raw4<T> ra, rb, ka, kb;                                  // the first rows are asked for before the sines are made
-    if (inside && q0 + sub < q1) ra.load(q_row + e0), rb.load(q_row + e1);
-    if (inside && k0 + sub < k1) ka.load(k_row + e0), kb.load(k_row + e1);
+    // Rows on their way from memory: DEPTH of them ahead of the one that is worked on (h + d ROWS + sub is a lane's row).
+    Raw4<T> ra[DEPTH], rb[DEPTH];
+    auto ask = [&](const T* rows, int64_t stride, int row, int upto, int d) {
+        if (inside && row < upto) ra[d].load(rows + row * stride + e0), rb[d].load(rows + row * stride + e1);
+    };
+    const T* q_rows = (const T*)p.q + t * p.q_stride_token;
+    const T* k_rows = (const T*)p.keys + t * p.key_stride_token;
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) ask(q_rows, p.q_stride_head, q0 + d * ROWS + sub, q1, d);           // (before the sines are made)
 
     for (int pair = lane; pair < half; pair += 32) {
         const int axis = p.axes ? p.axes[pair] : 0;
@@ -191,7 +198,7 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32) norm_rope_kernel(const crit_b
         for (int i = 0; i < 4; ++i) {
             if (!turned) {
                 own0[i] = w0[i], own1[i] = w1[i], other0[i] = other1[i] = 0.f;
-            } else if (p.interleaved) {
+            } else if (NEIGHBOURS) {
                 const float2 u = turns[part * 4 + (i >> 1)], v = turns[part * 4 + 2 + (i >> 1)];
                 own0[i] = u.x * w0[i], other0[i] = (i & 1 ? u.y : -u.y) * w0[i ^ 1];
                 own1[i] = v.x * w1[i], other1[i] = (i & 1 ? v.y : -v.y) * w1[i ^ 1];
@@ -215,7 +222,7 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32) norm_rope_kernel(const crit_b
         float u[4], v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float partner0 = p.interleaved ? x[i ^ 1] : y[i], partner1 = p.interleaved ? y[i ^ 1] : x[i];
+            const float partner0 = NEIGHBOURS ? x[i ^ 1] : y[i], partner1 = NEIGHBOURS ? y[i ^ 1] : x[i];
             u[i] = fmaf(partner0, other0[i], x[i] * own0[i]) * inv, v[i] = fmaf(partner1, other1[i], y[i] * own1[i]) * inv;
         }
 #pragma unroll
@@ -225,16 +232,22 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32) norm_rope_kernel(const crit_b
     // -- the queries' rows --------------------------------------------------------------------------------------------------
     if (q0 < q1) {
         factors(p.q_weight);
-        T* out = (T*)p.q_out + t * p.q_out_stride_token + (int64_t)(q0 + sub) * p.q_out_stride_head;
-        for (int h = q0; h < q1; h += ROWS) {                // (the same for every lane; a lane's own row is h + sub)
-            float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-            const bool live = inside && h + sub < q1;
-            if (live) ra.floats(x), rb.floats(y);
-            q_row += ROWS * p.q_stride_head;
-            if (inside && h + ROWS + sub < q1) ra.load(q_row + e0), rb.load(q_row + e1);
-            turn_row(x, y, p.q_weight != nullptr);
-            if (live) store4<T>(out + e0, x), store4<T>(out + e1, y);
-            out += ROWS * p.q_out_stride_head;
+        T* out = (T*)p.q_out + t * p.q_out_stride_token;
+        for (int h0 = q0; h0 < q1; h0 += ROWS * DEPTH) {
+#pragma unroll
+            for (int d = 0; d < DEPTH; ++d) {
+                const int h = h0 + d * ROWS;                 // (the same for every lane)
+                if (h >= q1) break;
+                float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+                const bool live = inside && h + sub < q1;
+                if (live) ra[d].floats(x), rb[d].floats(y);
+                ask(q_rows, p.q_stride_head, h + DEPTH * ROWS + sub, q1, d);
+                turn_row(x, y, p.q_weight != nullptr);
+                if (live) {
+                    T* to = out + (h + sub) * p.q_out_stride_head;
+                    store4<T>(to + e0, x), store4<T>(to + e1, y);
+                }
+            }
         }
     }
 
@@ -248,18 +261,23 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32) norm_rope_kernel(const crit_b
         }
     }
     if (k0 < k1) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) ask(k_rows, p.key_stride_head, k0 + d * ROWS + sub, k1, d);
         factors(p.key_weight);
-        T* out = p.keys_out ? (T*)p.keys_out + t * p.key_out_stride_token + (int64_t)(k0 + sub) * p.key_out_stride_head : nullptr;
-        for (int h = k0; h < k1; h += ROWS) {
+        T* out = p.keys_out ? (T*)p.keys_out + t * p.key_out_stride_token : nullptr;
+        for (int h0 = k0; h0 < k1; h0 += ROWS * DEPTH) {
+#pragma unroll
+          for (int d = 0; d < DEPTH; ++d) {
+            const int h = h0 + d * ROWS;
+            if (h >= k1) break;
             float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
             const bool live = inside && h + sub < k1;
-            if (live) ka.floats(x), kb.floats(y);
-            k_row += ROWS * p.key_stride_head;
-            if (inside && h + ROWS + sub < k1) ka.load(k_row + e0), kb.load(k_row + e1);
+            if (live) ra[d].floats(x), rb[d].floats(y);
+            ask(k_rows, p.key_stride_head, h + DEPTH * ROWS + sub, k1, d);
             turn_row(x, y, p.key_weight != nullptr);
-            if (out) {
-                if (live) store4<T>(out + e0, x), store4<T>(out + e1, y);
-                out += ROWS * p.key_out_stride_head;
+            if (out && live) {
+                T* to = out + (h + sub) * p.key_out_stride_head;
+                store4<T>(to + e0, x), store4<T>(to + e1, y);
             }
             if constexpr (WRITE) {
                 if (slot < 0) continue;                      // (the warp's token: the same for every lane)
@@ -277,6 +295,7 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32) norm_rope_kernel(const crit_b
                 __syncwarp();
                 encode_row(a, z, live, false, slot, h + sub, p.head_dim, part, LANES);
             }
+          }
         }
     }
 
@@ -300,15 +319,17 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32) norm_rope_kernel(const crit_b
 
 typedef void (*norm_rope_fn)(const crit_b200_norm_rope_params, const crit_b200_append_params, const int, const float);
 
-template <typename T, bool WRITE>
-static norm_rope_fn norm_rope_lanes(int width) {
-    if (width <= 64) return norm_rope_kernel<T, 8, WRITE>;
-    if (width <= 128) return norm_rope_kernel<T, 16, WRITE>;
-    return norm_rope_kernel<T, 32, WRITE>;
+template <typename T, int LANES>
+static norm_rope_fn norm_rope_of(bool write, bool neighbours) {
+    if (write) return neighbours ? norm_rope_kernel<T, LANES, true, true> : norm_rope_kernel<T, LANES, true, false>;
+    return neighbours ? norm_rope_kernel<T, LANES, false, true> : norm_rope_kernel<T, LANES, false, false>;
 }
 
 template <typename T>
-static norm_rope_fn norm_rope_pick(int width, bool write) { return write ? norm_rope_lanes<T, true>(width) : norm_rope_lanes<T, false>(width); }
+static norm_rope_fn norm_rope_pick(int width, bool write, bool neighbours) {
+    if (width <= 64) return norm_rope_of<T, 8>(write, neighbours);
+    return width <= 128 ? norm_rope_of<T, 16>(write, neighbours) : norm_rope_of<T, 32>(write, neighbours);
+}
 
 int check_append(const crit_b200_append_params& p);                                       // append.cu
 
@@ -346,19 +367,19 @@ extern "C" __attribute__((visibility("default"))) int crit_b200_norm_rope(const 
         }
     }
     // Warps a token: one for a prompt of many tokens (a token's sines are made once), as many as it has rows for a step's few,
-    // so that the launch has four times the warps that the device holds or a warp an iteration.
+    // so that the launch fills the device once or a warp has one iteration.
     const int row_heads = p.q_heads + p.kv_heads + (a.values ? p.kv_heads : 0);
     const int rows_at_once = 32 / (width <= 64 ? 8 : (width <= 128 ? 16 : 32)), most = (row_heads + rows_at_once - 1) / rows_at_once;
     int device = 0, sms = 0;
     if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) sms = 1;
-    const int64_t wanted = ((int64_t)sms * 128 + p.tokens - 1) / p.tokens;
+    const int64_t wanted = ((int64_t)sms * ROPE_FILL + p.tokens - 1) / p.tokens;
     const int parts = (int)(wanted < most ? wanted : most);
     const int64_t blocks = (p.tokens * parts + ROPE_WARPS - 1) / ROPE_WARPS;
     if (blocks > 0x7fffffffLL) return CRIT_B200_EINVAL;
     norm_rope_fn fn;
-    if (p.dtype == CRIT_B200_DTYPE_BF16) fn = norm_rope_pick<__nv_bfloat16>(width, append != nullptr);
-    else if (p.dtype == CRIT_B200_DTYPE_FP16) fn = norm_rope_pick<__half>(width, append != nullptr);
-    else fn = norm_rope_pick<float>(width, append != nullptr);
+    if (p.dtype == CRIT_B200_DTYPE_BF16) fn = norm_rope_pick<__nv_bfloat16>(width, append != nullptr, p.interleaved != 0);
+    else if (p.dtype == CRIT_B200_DTYPE_FP16) fn = norm_rope_pick<__half>(width, append != nullptr, p.interleaved != 0);
+    else fn = norm_rope_pick<float>(width, append != nullptr, p.interleaved != 0);
     fn<<<(unsigned)blocks, ROPE_WARPS * 32, 0, (cudaStream_t)stream>>>(p, a, parts, 1.f / (float)p.head_dim);
     CRIT_CHECK_LAUNCH();
     return 0;

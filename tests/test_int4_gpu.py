@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import crit_b200 as pk
-from int4_oracle import Cache4, attention4, bounds4, quantise4, values4
+from int4_oracle import SCALES, Cache4, attention4, bounds4, quantise4, values4
 
 pytestmark = pytest.mark.gpu
 
@@ -57,6 +57,26 @@ def test_rows_are_written_and_read_back_bit_for_bit(tokens, heads, dim, dtype):
     left[slots.cpu()] = False
     assert not cache.k.flatten(0, 1)[left.cuda()].any() and not cache.vs.flatten(0, 1)[left.cuda()].any()
     assert pk.status() == 0
+
+
+def test_every_scale_with_quotients_on_and_beside_every_border():
+    """For each of the 247 scales: elements half way between two codes, one step of their type beside them, and in between."""
+    for dtype in (torch.bfloat16, torch.float32):
+        rows = []
+        for byte in range(1, 248):
+            s = float(SCALES[byte])
+            x = torch.tensor([(k + 0.5) * s for k in range(-7, 7)] + [(k + 0.3) * s for k in range(-7, 7)], dtype=dtype)
+            around = torch.nextafter(x[:14].float(), torch.tensor(1e9)) if dtype == torch.float32 else x[:14]
+            rows.append(torch.cat([x, around.to(dtype)[:3], torch.tensor([7 * s], dtype=dtype)]))
+            rows.append(torch.cat([-x, -around.to(dtype)[3:6], torch.tensor([7 * s], dtype=dtype)]))
+        x = torch.stack(rows).view(247, 2, 32)
+        cache = Cache4(2, 32, 16, 17)
+        slots = torch.arange(247).cuda()
+        pk.write(x.cuda(), None, slots, cache.k, None, "int4", cache.ks, None)
+        codes, byte = quantise4(x.double().numpy())
+        assert np.array_equal(cache.ks.flatten(0, 1)[slots].cpu().numpy(), byte)
+        got = cache.k.flatten(0, 1)[slots].cpu().numpy()
+        assert np.array_equal(got & 15, codes[..., 0::2]) and np.array_equal(got >> 4, codes[..., 1::2])
 
 
 def test_odd_values_in_a_group():
