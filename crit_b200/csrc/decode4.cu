@@ -1,9 +1,9 @@
 // Split-K decode / speculative-verify attention over 4-bit pages (int4.cuh has the format).
 //
 // A block is a warp for each of HB kv heads (8, 4, 2 or 1: the most that divides the heads) and reads whole page rows, 16
-// positions of its HB heads a tile: one box of a tensor map with permuted dimensions, [dim / 2 bytes][slots][kv_heads], is
-// HB * dim / 2 contiguous bytes a position and lands head-major, swizzled as wide as a row is.  So the bytes asked of HBM
-// are long pieces although a row of one head is 64 bytes (dim 128).  The tile's scales come by a bulk copy onto the same
+// positions of its HB heads a tile: one box of a tensor map with permuted dimensions, [128 bytes][slots][rows of 128 a slot], is
+// HB * dim / 2 contiguous bytes a position and lands with a few heads' (two of dim 128) 16 positions together, swizzled.  So the
+// bytes asked of HBM are long pieces although a row of one head is 64 bytes (dim 128).  The tile's scales come by a bulk copy onto the same
 // mbarrier.  There is no producer warp (a ninth warp would take the registers of two blocks an SM): the warps take turns,
 // warp n mod HB refills the ring when it comes to tile n, with a tile S - 2 ahead and the page id it read a turn before.
 //
@@ -58,6 +58,7 @@ struct Decode4Launch {
     int ctiles;             // tiles of 8 NT query rows a window row takes at most
     int stages;             // of the ring
     int stage_bytes;
+    int row;                // bytes of a tensor map's row: 128, or what the block's heads fill of it
     int blocks;             // of an even launch; 0: splits
 };
 
@@ -142,13 +143,10 @@ __device__ __forceinline__ void scale_pairs(uint32_t a, uint32_t b, uint32_t (&p
     }
 }
 
-// Byte offset of 16-byte chunk c (a group of 32 codes) of row `row` of a tile, rows of D / 2 bytes with TMA's swizzle of
-// that width.
-template <int D>
-__device__ __forceinline__ int chunk4(int row, int c) {
-    if constexpr (D == 256) return row * 128 + ((c ^ (row & 7)) << 4);
-    else if constexpr (D == 128) return row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
-    else return row * 32 + ((c ^ ((row >> 2) & 1)) << 4);
+// Byte offset of 16-byte chunk c of row `row` of a tile, rows of `bytes` (128, 64 or 32) with TMA's swizzle of that width.
+__device__ __forceinline__ uint32_t chunk4(uint32_t row, uint32_t c, uint32_t bytes) {
+    const uint32_t turn = bytes == 128 ? row & 7 : (bytes == 64 ? (row >> 1) & 3 : (row >> 2) & 1);
+    return row * bytes + ((c ^ turn) << 4);
 }
 
 // A row of the launch: its tiles, and how many times they are read (head groups x tiles of query rows).
@@ -273,7 +271,7 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
 
     // -- refilling the ring (lane 0; a warp's turns are HB tiles apart) ------------------------------------------------------
     Place4 next = at;               // the tile of this warp's next turn, its page read ahead
-    int next_n = warp, next_page = 0, next_head = 0;
+    int next_n = warp, next_page = 0, next_row = 0;
     const int32_t* next_table = nullptr;
     auto step_to = [&](Place4& c, int by) {
         c.tile += by;
@@ -289,7 +287,7 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
     };
     auto read_row = [&]() {         // what stays the same from tile to tile
         next_table = p.tables + (int64_t)p.rows[next.r] * p.table_stride;
-        next_head = (u.blocks ? next.sub / (next.subs / HG) : next.sub / u.ctiles) * HB;
+        next_row = (u.blocks ? next.sub / (next.subs / HG) : next.sub / u.ctiles) * (HB * (D / 2) / u.row);
     };
     auto read_page = [&]() {
         const uint32_t tile = (uint32_t)next.tile;
@@ -304,9 +302,9 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
         const uint64_t scales0 = (uint64_t)slot0 * (uint32_t)row_scales;
         const uint32_t bar = full + stage * 8, to = ring + stage * u.stage_bytes;
         mbar_expect_tx(bar, (uint32_t)(2 * code_bytes + 2 * scale_bytes));
-        tma_load_3d(to, &kmap, 0, (int)slot0, next_head, bar);
+        tma_load_3d(to, &kmap, 0, (int)slot0, next_row, bar);
         bulk_load(to + 2 * code_bytes, (const char*)p.key_scales + scales0, scale_bytes, bar);
-        tma_load_3d(to + code_bytes, &vmap, 0, (int)slot0, next_head, bar);
+        tma_load_3d(to + code_bytes, &vmap, 0, (int)slot0, next_row, bar);
         bulk_load(to + 2 * code_bytes + scale_bytes, (const char*)p.value_scales + scales0, scale_bytes, bar);
     };
     auto turn_over = [&]() {        // to this warp's next turn
@@ -330,9 +328,10 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
     bool dead = false;
     int n = 0, stage = 0;           // tiles taken, the ring's place
     uint32_t phase = 0;
-    // ldmatrix rows: lanes 0-7 and 8-15 name positions 0-7 and 8-15 of chunk 2 i, lanes 16-31 the same of chunk 2 i + 1 (whose
-    // address is chunk lane / 16's with the bits of 2 i changed: a warp's part of a tile lies on a multiple of its swizzle)
-    const uint32_t lane_codes = ring + warp * (16 * (D / 2)) + chunk4<D>((lane & 7) + 8 * ((lane >> 3) & 1), lane >> 4);
+    // ldmatrix rows: lanes 0-7 and 8-15 name positions 0-7 and 8-15 of the head's chunk 2 i, lanes 16-31 the same of chunk 2 i + 1
+    // (whose address is that of chunk 0 or 1 with the bits of 2 i changed: a head's chunks begin at a multiple of their number)
+    const uint32_t heads_row = (uint32_t)u.row / (D / 2);
+    const uint32_t lane_codes = ring + chunk4(warp / heads_row * 16 + (lane & 7) + 8 * ((lane >> 3) & 1), warp % heads_row * NG + (lane >> 4), u.row);
 
     while (n < length) {
         // -- a unit: the tiles of one row, head group and query tile in this block -----------------------------------------
@@ -863,6 +862,7 @@ static int plan4(int q_heads, int kv_heads, int d, int columns, int n_rows, bool
     u.heads = decode4_heads(d, nt);
     while (kv_heads % u.heads) u.heads >>= 1;
     u.ctiles = (rows + 8 * nt - 1) / (8 * nt);
+    u.row = u.heads * d / 2 < 128 ? u.heads * d / 2 : 128;
     u.stage_bytes = (u.heads * 16 * d + 2 * 16 * kv_heads * (d / 32) + 1023) / 1024 * 1024;
     const int blocks = decode4_blocks(d, nt) * decode4_heads(d, nt) / u.heads;           // (the registers hold as many)
     const int room = (228 * 1024) / blocks - 1024 - 1024 - 4096;                          // (alignment, the driver's, the row lists)
@@ -904,8 +904,8 @@ int launch_decode4(const crit_b200_attend_params& p, cudaStream_t s) {
     if (int e = plan4(p, &plan)) return e;
     const Decode4Launch& u = plan.u;
     CUtensorMap kmap, vmap;
-    if (!rows4_map(&kmap, p.key_pages, p.head_dim, p.kv_heads, u.heads, p.slots) ||
-        !rows4_map(&vmap, p.value_pages, p.head_dim, p.kv_heads, u.heads, p.slots))
+    if (!rows4_map(&kmap, p.key_pages, p.head_dim, p.kv_heads, u.heads, u.row, p.slots) ||
+        !rows4_map(&vmap, p.value_pages, p.head_dim, p.kv_heads, u.heads, u.row, p.slots))
         return CRIT_B200_EUNSUPPORTED;
     cudaError_t ce = cudaFuncSetAttribute((const void*)plan.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, plan.smem);
     if (ce != cudaSuccess) return (int)ce;

@@ -56,18 +56,19 @@ inline bool page_rows_map(CUtensorMap* map, const void* pages, int dim, int kv_h
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// A 4-bit page tensor [slots][kv_heads][dim / 2 bytes] with the dimensions permuted, [dim / 2][slots][kv_heads]: a box is 16
-// slots of `heads` kv heads, heads * dim / 2 contiguous bytes a slot, and lands head-major, row 16 * head + slot, swizzled as
-// wide as a row is (32, 64 or 128 bytes), which is what ldmatrix reads without bank conflicts.
-inline bool rows4_map(CUtensorMap* map, const void* pages, int dim, int kv_heads, int heads, int64_t slots) {
+// A 4-bit page tensor [slots][kv_heads][dim / 2 bytes] as rows of `row` bytes (32, 64 or 128: one head or a few neighbours that
+// divide the heads), the dimensions permuted, [row][slots][rows a slot]: a box is 16 slots of `heads` kv heads, one contiguous
+// piece a slot, and lands row-major in (row of the slot, slot), swizzled as wide as a row is, which is what ldmatrix reads
+// without bank conflicts.
+inline bool rows4_map(CUtensorMap* map, const void* pages, int dim, int kv_heads, int heads, int row, int64_t slots) {
     encode_tiled_fn encode = encoder();
     if (!encode) return false;
-    const cuuint64_t row = (cuuint64_t)dim / 2;
-    const cuuint64_t dims[3] = {row, (cuuint64_t)slots, (cuuint64_t)kv_heads};
-    const cuuint64_t strides[2] = {row * kv_heads, row};
-    const cuuint32_t box[3] = {(cuuint32_t)row, 16, (cuuint32_t)heads};
+    const int per_slot = kv_heads * dim / 2;
+    const cuuint64_t dims[3] = {(cuuint64_t)row, (cuuint64_t)slots, (cuuint64_t)(per_slot / row)};
+    const cuuint64_t strides[2] = {(cuuint64_t)per_slot, (cuuint64_t)row};
+    const cuuint32_t box[3] = {(cuuint32_t)row, 16, (cuuint32_t)(heads * dim / 2 / row)};
     const cuuint32_t steps[3] = {1, 1, 1};
-    const CUtensorMapSwizzle swizzle = dim == 256 ? CU_TENSOR_MAP_SWIZZLE_128B : (dim == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
+    const CUtensorMapSwizzle swizzle = row == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : (row == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(pages), dims, strides, box, steps,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
