@@ -27,9 +27,8 @@
 // rows, the outputs of 256-wide heads), codes become n - 8 one add later.
 //
 // The queries become FP16 with an exponent of their own a row (the largest element between 2^13 and 2^14), so no bf16 query
-// overflows or vanishes.  Weights are 2^(x - ref) with ref at most 2 (in the exponent) above the running maximum and never
-// below it: a weight is at most 1, times a scale of at most 61,440 it stays an FP16 number, and the running reference moves
-// only when a score passes it.  Sums are FP32.
+// overflows or vanishes.  Weights are 2^(x - ref) with a reference that moves only when a score passes it (by 14 in the
+// exponent where the scales are on the codes): every weight and product stays an FP16 number.  Sums are FP32.
 //
 // Two ways to cut a launch.  By splits: a 3-D grid of (split of `chunk` positions, heads and query tiles, row), states in the
 // workspace as every other decode kernel leaves them: a column's bits do not depend on the launch.  Even
@@ -173,12 +172,14 @@ __global__ void __launch_bounds__(32 * decode4_heads(D, NT), decode4_blocks(D, N
 decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     constexpr int NG = D / 32;                // groups of a row
     constexpr int ROWS = 8 * NT;
-    constexpr int TPI = 2;                    // tiles an iteration takes
-    constexpr float AHEAD = 2.f;
+    constexpr int TPI = FAST && NT == 4 ? 1 : 2;        // tiles an iteration takes (the widest has products enough of its own)
     constexpr bool RAW_K = FAST && NT <= 2;                 // the 8 of the keys' codes through the accumulators' start
     constexpr bool RAW_V = FAST && NT == 1 && D <= 128;     // that of the values' through a product of its own
     constexpr bool SCALE_CODES = !FAST || NT > 1;           // the values' scales on the codes (an exact product), not on the weights:
                                                             // fewer products where a tile holds several columns of query rows
+    // A row's reference is set AHEAD above its maximum and moves when a score passes it by more than SLACK: weights on their
+    // way to a scale of up to 61,440 stay at 1 or below, weights beside scaled codes may grow to 2^14 first.
+    constexpr float AHEAD = SCALE_CODES ? 0.f : 2.f, SLACK = SCALE_CODES ? 14.f : 0.f;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     __shared__ __align__(8) uint64_t bars_mem[2 * D4_MAX_STAGES];
@@ -365,15 +366,20 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
                     raw[k] = *reinterpret_cast<const uint4*>((const char*)p.q + ((int64_t)(start + col) * p.q_stride_token +
                                                                                  (int64_t)(h * G + gq) * p.q_stride_head + k * 32 + t * 8) * 2);
             }
+            const bool bf16 = p.q_dtype == CRIT_B200_DTYPE_BF16;
             auto element = [&](int k, int i) {
                 const uint32_t w = (&raw[k].x)[i >> 1];
-                if (p.q_dtype == CRIT_B200_DTYPE_BF16) return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
+                if (bf16) return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
                 return __half2float(__ushort_as_half((unsigned short)(i & 1 ? w >> 16 : w)));
             };
+            {   // the largest magnitude: both types' bits without the sign are in the order of their values
+                uint32_t high = 0u;
 #pragma unroll
-            for (int k = 0; k < NG; ++k)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(element(k, i)));
+                for (int k = 0; k < NG; ++k)
+                    high = __vmaxu2(high, __vmaxu2(__vmaxu2(raw[k].x & 0x7fff7fffu, raw[k].y & 0x7fff7fffu), __vmaxu2(raw[k].z & 0x7fff7fffu, raw[k].w & 0x7fff7fffu)));
+                high = max(high >> 16, high & 0xffffu);
+                amax = bf16 ? __uint_as_float(high << 16) : __half2float(__ushort_as_half((unsigned short)high));
+            }
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
             int e = (int)((__float_as_uint(amax) >> 23) & 255u) - 127 - 13;
@@ -539,7 +545,7 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
                         mx[c & 1] = fmaxf(mx[c & 1], y);
                     }
                 top[nt][0] = mx[0] * mul[nt][0], top[nt][1] = mx[1] * mul[nt][1];
-                passed |= top[nt][0] > m_run[nt][0] || top[nt][1] > m_run[nt][1];
+                passed |= top[nt][0] > m_run[nt][0] + SLACK || top[nt][1] > m_run[nt][1] + SLACK;
             }
             // The reference of a row moves only when a score of it passes it; the lanes' maxima are compared across the warp, and
             // the sums brought to the new reference, only then.
@@ -553,7 +559,7 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
                         high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 4));
                         high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 8));
                         high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 16));
-                        const bool moved = high > m_run[nt][j];
+                        const bool moved = high > m_run[nt][j] + SLACK;
                         alpha[j] = moved ? ex2(m_run[nt][j] - (high + AHEAD)) : 1.f;
                         m_run[nt][j] = moved ? high + AHEAD : m_run[nt][j];
                         l_run[nt][j] *= alpha[j];
@@ -720,16 +726,14 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
 }
 
 // The fold of an even launch: a row's states are consecutive slots.  WARPS warps serve a (window token, query head), warp w the
-// slots w, w + WARPS, ..; first the slots' maximum, then sums with weights that are fixed by then, added in warp order.
+// slots w, w + WARPS, ..; the warps' sums are added in warp order.
 template <int D, int WARPS>
 __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) merge4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const int rows_tile) {
     constexpr int PER = D / 32;
-    __shared__ float part_l[WARPS], part_o[WARPS > 1 ? WARPS : 1][WARPS > 1 ? D : 1];
+    __shared__ float part_m[WARPS], part_l[WARPS], part_o[WARPS > 1 ? WARPS : 1][WARPS > 1 ? D : 1];
     const int lane = threadIdx.x & 31, warp = WARPS == 1 ? 0 : threadIdx.x >> 5;
-    const int64_t item = WARPS == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
-    if (item >= (int64_t)p.n_rows * p.columns * p.q_heads) return;
-    const int head = (int)(item % p.q_heads), rc = (int)(item / p.q_heads);
-    const int r = rc / p.columns, col = rc - r * p.columns;
+    const int head = WARPS == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x, col = blockIdx.y, r = blockIdx.z;
+    if (head >= p.q_heads) return;
     const int* info = reinterpret_cast<const int*>(p.workspace);
     const int run = info[0], first = info[1 + r];
     const int count = row_count4(p, r), start = p.starts[r];
@@ -745,51 +749,70 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) merge4_kernel(c
         if (n == 1 && !p.sinks) return;                              // written by the first launch
     }
     const float* space = p.workspace + (p.n_rows + 2 + 31) / 32 * 32;
-    const int64_t slots = (int64_t)u.blocks + (int64_t)p.n_rows * HG * u.ctiles, per = (int64_t)HB * rows_tile;
-    const int64_t state0 = ((int64_t)lo + ((int64_t)r * HG + hg) * u.ctiles + ct) * per + (int64_t)(h - hg * HB) * rows_tile + (flat - ct * rows_tile);
-    const float* pm = space + slots * per * D;
+    const int64_t slots = (int64_t)u.blocks + (int64_t)p.n_rows * HG * u.ctiles;
+    const int per = HB * rows_tile;
+    const int64_t state0 = ((int64_t)lo + ((int64_t)r * HG + hg) * u.ctiles + ct) * per + (h - hg * HB) * rows_tile + (flat - ct * rows_tile);
+    const float* pm = space + slots * per * D + state0;
     const float* pl = pm + slots * per;
-    float top = -INFINITY;
-    for (int s = lane; s < n; s += 32) top = fmaxf(top, pm[state0 + s * per]);
-    top = warp_max(top);
-    const float sub = top == -INFINITY ? 0.f : top;
-    float total = 0.f, acc[PER];
+    const float* po = space + state0 * D + lane * PER;
+    // a warp's states four at a time, everything of them asked for at once; the maximum and the sums go along
+    float top = -INFINITY, total = 0.f, acc[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-#pragma unroll 4
-    for (int s = warp; s < n; s += WARPS) {
-        const int64_t where = state0 + s * per;
-        const float w = ex2(pm[where] - sub);
-        total += pl[where] * w;
-        const float* o = space + where * D + lane * PER;
-        float v[PER];
-        if constexpr (PER == 2) {
-            const float2 a = *reinterpret_cast<const float2*>(o);
-            v[0] = a.x, v[1] = a.y;
-        } else {
+    for (int s0 = warp; s0 < n; s0 += 4 * WARPS) {
+        float m[4], l[4], v[4][PER];
 #pragma unroll
-            for (int i = 0; i < PER; i += 4) {
-                const float4 a = *reinterpret_cast<const float4*>(o + i);
-                v[i] = a.x, v[i + 1] = a.y, v[i + 2] = a.z, v[i + 3] = a.w;
+        for (int k = 0; k < 4; ++k) {
+            const int s = s0 + k * WARPS;
+            m[k] = -INFINITY, l[k] = 0.f;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) v[k][i] = 0.f;
+            if (s >= n) continue;
+            m[k] = pm[(int64_t)s * per], l[k] = pl[(int64_t)s * per];
+            const float* o = po + (int64_t)s * per * D;
+            if constexpr (PER == 2) {
+                const float2 a = *reinterpret_cast<const float2*>(o);
+                v[k][0] = a.x, v[k][1] = a.y;
+            } else {
+#pragma unroll
+                for (int i = 0; i < PER; i += 4) {
+                    const float4 a = *reinterpret_cast<const float4*>(o + i);
+                    v[k][i] = a.x, v[k][i + 1] = a.y, v[k][i + 2] = a.z, v[k][i + 3] = a.w;
+                }
             }
         }
+        const float up = fmaxf(fmaxf(top, fmaxf(m[0], m[1])), fmaxf(m[2], m[3])), sub = up == -INFINITY ? 0.f : up;
+        const float keep = ex2(top - sub);
+        total *= keep;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) acc[i] = fmaf(v[i], w, acc[i]);
+        for (int i = 0; i < PER; ++i) acc[i] *= keep;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float w = ex2(m[k] - sub);
+            total = fmaf(l[k], w, total);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) acc[i] = fmaf(v[k][i], w, acc[i]);
+        }
+        top = up;
     }
     if constexpr (WARPS > 1) {
-        if (lane == 0) part_l[warp] = total;
+        if (lane == 0) part_m[warp] = top, part_l[warp] = total;
 #pragma unroll
         for (int i = 0; i < PER; ++i) part_o[warp][lane * PER + i] = acc[i];
         __syncthreads();
         if (warp) return;
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w) top = fmaxf(top, part_m[w]);
+        const float sub = top == -INFINITY ? 0.f : top;
         total = 0.f;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) total += part_l[w];
+        for (int i = 0; i < PER; ++i) acc[i] = 0.f;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            acc[i] = 0.f;
+        for (int w = 0; w < WARPS; ++w) {
+            const float f = ex2(part_m[w] - sub);
+            total = fmaf(part_l[w], f, total);
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) acc[i] += part_o[w][lane * PER + i];
+            for (int i = 0; i < PER; ++i) acc[i] = fmaf(part_o[w][lane * PER + i], f, acc[i]);
         }
     }
     float shrink = 1.f;                     // the head's sink, last: one position more without a value
@@ -808,8 +831,7 @@ typedef void (*decode4_fn)(const crit_b200_attend_params, const Decode4Launch, c
 
 template <int D, int NT>
 static decode4_fn decode4_of(bool masks, bool fast) {
-    if constexpr (NT <= 2)
-        if (fast) return masks ? decode4_kernel<D, NT, true, true> : decode4_kernel<D, NT, false, true>;
+    if (fast) return masks ? decode4_kernel<D, NT, true, true> : decode4_kernel<D, NT, false, true>;
     return masks ? decode4_kernel<D, NT, true, false> : decode4_kernel<D, NT, false, false>;
 }
 
@@ -919,9 +941,9 @@ int launch_decode4(const crit_b200_attend_params& p, cudaStream_t s) {
 
 template <int D>
 static void launch_merge4_of(const crit_b200_attend_params& p, const Decode4Plan& plan, bool many, cudaStream_t s) {
-    const int64_t items = (int64_t)p.n_rows * p.columns * p.q_heads;
-    if (many) merge4_kernel<D, 8><<<(unsigned)items, 256, 0, s>>>(p, plan.u, 8 * plan.nt);
-    else merge4_kernel<D, 1><<<(unsigned)((items + 3) / 4), 128, 0, s>>>(p, plan.u, 8 * plan.nt);
+    const unsigned heads = (unsigned)p.q_heads, columns = (unsigned)p.columns, rows = (unsigned)p.n_rows;        // (rows <= D4_MAX_ROWS)
+    if (many) merge4_kernel<D, 8><<<dim3(heads, columns, rows), 256, 0, s>>>(p, plan.u, 8 * plan.nt);
+    else merge4_kernel<D, 1><<<dim3((heads + 3) / 4, columns, rows), 128, 0, s>>>(p, plan.u, 8 * plan.nt);
 }
 
 int launch_merge4(const crit_b200_attend_params& p, cudaStream_t s) {
