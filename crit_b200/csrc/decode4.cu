@@ -45,7 +45,7 @@ namespace crit_b200 {
 
 constexpr int D4_MAX_STAGES = 8;
 constexpr int D4_MAX_ROWS = 256;              // window rows an even launch lists
-constexpr int D4_MIN_RUN = 4;                 // tiles an even launch's block takes at least
+constexpr int D4_MIN_RUN = 2;                 // tiles an even launch's block takes at least
 
 // The most kv heads a block takes, and the blocks an SM is to hold: a warp's accumulators decide (the registers of 16 warps
 // are 128 a thread, of 8 warps 255).
@@ -663,7 +663,7 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
 
         // -- the state, or the row's output ------------------------------------------------------------------------------------
         bool whole, fits = true;
-        int64_t state0 = 0, state_row = 0, states = 0;          // an even launch: rows of states before this one's, their number
+        int64_t state0 = 0, states = 0;                         // an even launch: rows of states before this one's, their number
         int prow0 = 0, split = 0;
         if (u.blocks) {
             whole = ntiles == at.tiles && !p.sinks;
@@ -730,7 +730,7 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
 template <int D, int WARPS>
 __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) merge4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const int rows_tile) {
     constexpr int PER = D / 32;
-    __shared__ float part_m[WARPS], part_l[WARPS], part_o[WARPS > 1 ? WARPS : 1][WARPS > 1 ? D : 1];
+    __shared__ __align__(8) float part_m[WARPS], part_l[WARPS], part_o[WARPS > 1 ? WARPS : 1][WARPS > 1 ? D : 1];
     const int lane = threadIdx.x & 31, warp = WARPS == 1 ? 0 : threadIdx.x >> 5;
     const int head = WARPS == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x, col = blockIdx.y, r = blockIdx.z;
     if (head >= p.q_heads) return;
@@ -800,30 +800,30 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) merge4_kernel(c
 #pragma unroll
         for (int i = 0; i < PER; ++i) part_o[warp][lane * PER + i] = acc[i];
         __syncthreads();
-        if (warp) return;
+        if (threadIdx.x >= D / 2) return;                  // two columns a thread
+        top = -INFINITY;
 #pragma unroll
-        for (int w = 1; w < WARPS; ++w) top = fmaxf(top, part_m[w]);
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, part_m[w]);
         const float sub = top == -INFINITY ? 0.f : top;
-        total = 0.f;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+        total = acc[0] = acc[1] = 0.f;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
             const float f = ex2(part_m[w] - sub);
-            total = fmaf(part_l[w], f, total);
-#pragma unroll
-            for (int i = 0; i < PER; ++i) acc[i] = fmaf(part_o[w][lane * PER + i], f, acc[i]);
+            const float2 o = *reinterpret_cast<const float2*>(&part_o[w][2 * threadIdx.x]);
+            total = fmaf(part_l[w], f, total), acc[0] = fmaf(o.x, f, acc[0]), acc[1] = fmaf(o.y, f, acc[1]);
         }
     }
+    constexpr int MINE = WARPS > 1 ? 2 : PER;               // columns this thread writes, from `at`
+    const int at = WARPS > 1 ? 2 * threadIdx.x : lane * PER;
     float shrink = 1.f;                     // the head's sink, last: one position more without a value
     if (p.sinks) sink_fold(p.sinks[head], top, total, shrink);
     const float inv = total > 0.f ? shrink / total : (total == 0.f ? 0.f : total);         // (a NaN stays one)
-    const int64_t to = (int64_t)(start + col) * p.out_stride_token + (int64_t)head * p.out_stride_head + lane * PER;
+    const int64_t to = (int64_t)(start + col) * p.out_stride_token + (int64_t)head * p.out_stride_head + at;
 #pragma unroll
-    for (int i = 0; i < PER; i += 2)
+    for (int i = 0; i < MINE; i += 2)
         *reinterpret_cast<uint32_t*>((char*)p.out + (to + i) * 2) =
             p.q_dtype == CRIT_B200_DTYPE_BF16 ? pack2<true>(acc[i] * inv, acc[i + 1] * inv) : pack2<false>(acc[i] * inv, acc[i + 1] * inv);
-    if (p.lse && lane == 0) p.lse[(int64_t)(start + col) * p.q_heads + head] = total == 0.f ? -INFINITY : top * LN2 + logf(total);
+    if (p.lse && at == 0) p.lse[(int64_t)(start + col) * p.q_heads + head] = total == 0.f ? -INFINITY : top * LN2 + logf(total);
 }
 
 // -- host side --------------------------------------------------------------------------------------------------------------
@@ -942,7 +942,7 @@ int launch_decode4(const crit_b200_attend_params& p, cudaStream_t s) {
 template <int D>
 static void launch_merge4_of(const crit_b200_attend_params& p, const Decode4Plan& plan, bool many, cudaStream_t s) {
     const unsigned heads = (unsigned)p.q_heads, columns = (unsigned)p.columns, rows = (unsigned)p.n_rows;        // (rows <= D4_MAX_ROWS)
-    if (many) merge4_kernel<D, 8><<<dim3(heads, columns, rows), 256, 0, s>>>(p, plan.u, 8 * plan.nt);
+    if (many) merge4_kernel<D, 16><<<dim3(heads, columns, rows), 512, 0, s>>>(p, plan.u, 8 * plan.nt);
     else merge4_kernel<D, 1><<<dim3((heads + 3) / 4, columns, rows), 128, 0, s>>>(p, plan.u, 8 * plan.nt);
 }
 
