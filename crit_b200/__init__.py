@@ -35,6 +35,7 @@ __all__ = ["KINDS", "MAX_COLUMNS", "attend", "chunk_for", "gather", "merge_shard
 
 _STAGINGS = {None: 0, "cp.async": 1, "tma": 2}
 _ENGINES = {"tcgen05": 8, "mma.sync": 16, "tcgen05t": 64, "tcgen05p": 128, "even": 512}
+_PREFILL_ENGINES = {None: 0, "mma.sync": 1, "tcgen05": 2, "tcgen05:single": 2 | 4, "tcgen05:pair": 2 | 8}
 KINDS = {"bf16": 0, "fp16": 0, "fp8": 1, "fp8:row": 2, "int8": 3, "fp8:page": 4, "int4": 5}
 GROUP4 = 32                 # elements of an "int4" row that share a scale
 MAX_COLUMNS = 64            # columns of one row a launch reads
@@ -815,8 +816,8 @@ def prefill_serves(head_dim, value_dim, q_dtype, kind, page):
 
 # -- prompt chunks ------------------------------------------------------------------------------------------------------
 def _expanded(p, q, key_pages, value_pages, key_scales, value_scales, table, position, tokens, longest, page, workspace):
-    """4-bit pages as 16-bit ones of q's type in the workspace, one launch, in the order of the sequences' tables: (keys,
-    values, the table that reads them)."""
+    """4-bit pages as 16-bit ones of q's type in the workspace, one launch, in the order of the sequences' tables: the
+    addresses of the keys, the values and the table that reads them, its width, and the slots of the pages."""
     hkv, d = key_pages.shape[-2], q.shape[-1]
     place = q.get_device()
     if value_scales is None or _check4(key_pages, key_scales, "keys") != (hkv, d) or _check4(value_pages, value_scales, "values") != (hkv, d) or \
@@ -835,15 +836,23 @@ def _expanded(p, q, key_pages, value_pages, key_scales, value_scales, table, pos
     floats = 2 * half + pages
     # (a workspace that a launch outgrew is kept: large ones grow by powers of two)
     space = _workspace(q.device, floats if workspace is not None or floats < 1 << 24 else 1 << (floats - 1).bit_length(), workspace)
-    keys = space[:half].view(q.dtype).view(pages, page, hkv, d)
-    values = space[half:2 * half].view(q.dtype).view(pages, page, hkv, d)
-    found = space[2 * half:2 * half + pages].view(torch.int32).view(table.shape[:-1] + (width,))
-    on_device = p.positions if several else (position.data_ptr() if torch.is_tensor(position) else None)
-    e = _lib.block(_lib.ExpandParams, _ptr(key_pages), _ptr(value_pages), _ptr(key_scales), _ptr(value_scales), _ptr(table), on_device, p.starts,
-                   _ptr(keys), _ptr(values), _ptr(found), _ptr(_status_word(q.device)), int(position) if on_device is None else 0,
+    keys = space.data_ptr()
+    values, found = keys + 4 * half, keys + 8 * half
+    on_device = p.positions if several else _ptr(position) if torch.is_tensor(position) else None
+    e = _lib.block(_lib.ExpandParams, key_pages.data_ptr(), value_pages.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), table.data_ptr(),
+                   on_device, p.starts, keys, values, found, _ptr(_status_word(q.device)), 0 if on_device else int(position),
                    key_pages.numel() * 2 // (hkv * d), table.stride(0) if several else 0, sequences, width, tokens, hkv, d, page, _DTYPES[q.dtype])
     _run("crit_b200_expand", "crit_b200.prefill", q.device, e)
-    return keys, values, found
+    return keys, values, found, width, pages * page
+
+
+def _sent(numbers, dtype, device):
+    """A list on the device; the host does not wait for the device (the driver takes its copy of pageable memory at the
+    call).  A capture would record the address of the host's list instead: refused."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("crit_b200.prefill: under capture the positions are a tensor on the device and the starts are left out "
+                           "(a list of them is copied from the host)")
+    return torch.tensor(numbers, dtype=dtype).to(device, non_blocking=True)
 
 
 def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scales=None, value_scales=None,
@@ -885,7 +894,7 @@ def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scale
             if len(position) != S:
                 raise ValueError("one position a sequence")
             ahead = [int(x) for x in position]
-            position = torch.tensor(ahead, dtype=torch.int64, device=q.device)
+            position = _sent(ahead, torch.int64, q.device)
         if position.dtype != torch.int64 or position.numel() != S or not position.is_cuda or not position.is_contiguous():
             raise ValueError("the sequences' positions are an int64 tensor [S] on the device")
         if starts is None:
@@ -899,7 +908,7 @@ def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scale
                 raise ValueError("starts: S + 1 rising row numbers from 0 to the number of tokens")
             counts = [b - a for a, b in zip(starts, starts[1:])]
             most = max(counts)
-            starts = torch.tensor(starts, dtype=torch.int32, device=q.device)
+            starts = _sent(starts, torch.int32, q.device)
             p.starts = _ptr(starts)
         p.positions, p.sequences, p.table_stride = _ptr(position), S, table.stride(0)
         T, position, held = most, 0, position
@@ -908,28 +917,26 @@ def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scale
         raise ValueError("starts goes with a table of several sequences")
     if torch.is_tensor(position) and (position.dtype != torch.int64 or position.numel() != 1 or not position.is_cuda):
         raise ValueError("a position read on the device is a one-element int64 tensor there")
+    p.q, p.out, p.lse = q.data_ptr(), out.data_ptr(), _ptr(lse)
     if k_kind == 5:
-        key_pages, value_pages, table = _expanded(p, q, key_pages, value_pages, key_scales, value_scales, table, position, T, longest, int(page),
-                                                  workspace)
-        kind = "fp16" if q.dtype == torch.float16 else "bf16"
-        k_kind, key_scales, value_scales = 0, None, None
-        if p.sequences:
-            p.table_stride = table.stride(0)
-    p.q, p.out, p.lse = _ptr(q), _ptr(out), _ptr(lse)
-    p.key_pages, p.value_pages = _ptr(key_pages), _ptr(value_pages)
-    p.key_scales, p.value_scales = _ptr(key_scales), _ptr(value_scales)
-    p.table = _ptr(table)
+        p.key_pages, p.value_pages, p.table, width, p.slots = _expanded(p, q, key_pages, value_pages, key_scales, value_scales, table, position, T,
+                                                                        longest, int(page), workspace)
+        p.table_stride = width if p.sequences else 0
+        p.kind, p.page_dtype = 0, _DTYPES[q.dtype]
+    else:
+        p.key_pages, p.value_pages = _ptr(key_pages), _ptr(value_pages)
+        p.key_scales, p.value_scales = _ptr(key_scales), _ptr(value_scales)
+        p.table, p.slots = _ptr(table), key_pages.numel() // (hkv * d)
+        p.kind, p.page_dtype = k_kind, _page_dtype(kind, key_pages)
     if torch.is_tensor(position):
         p.position_ptr = _ptr(position)
     else:
         p.position = int(position)
-    p.q_stride_token, p.q_stride_head = q.stride(0), q.stride(1)
-    p.out_stride_token, p.out_stride_head = out.stride(0), out.stride(1)
-    p.slots = key_pages.numel() // (hkv * d)
-    p.flags = {None: 0, "mma.sync": 1, "tcgen05": 2, "tcgen05:single": 2 | 4, "tcgen05:pair": 2 | 8}[engine]
+    p.q_stride_token, p.q_stride_head, _ = q.stride()
+    p.out_stride_token, p.out_stride_head, _ = out.stride()
+    p.flags = _PREFILL_ENGINES[engine]
     p.status = _ptr(_status_word(q.device))
-    p.tokens, p.q_heads, p.kv_heads, p.head_dim, p.value_dim, p.page = T, hq, hkv, d, d, int(page)
-    p.kind, p.page_dtype, p.q_dtype = k_kind, _page_dtype(kind, key_pages), _DTYPES[q.dtype]
+    p.tokens, p.q_heads, p.kv_heads, p.head_dim, p.value_dim, p.page, p.q_dtype = T, hq, hkv, d, d, int(page), _DTYPES[q.dtype]
     p.scale = float(scale if scale is not None else d ** -0.5)
     p.key_multiplier, p.value_multiplier = float(multipliers[0]), float(multipliers[1])
     _run("crit_b200_prefill", "crit_b200.prefill", q.device, p)
