@@ -152,9 +152,12 @@ __device__ __forceinline__ uint32_t chunk4(uint32_t row, uint32_t c, uint32_t by
     return row * bytes + ((c ^ turn) << 4);
 }
 
-// A row of the launch: its tiles, and how many times they are read (head groups x tiles of query rows).
+// A row of the launch: its tiles.  -1 in an even launch whose plan is too small for the row (chunk * max_splits positions are
+// what a table row holds): the row is left out, its output as it was, and reported.  A launch cut into splits ends there by
+// its grid.
 __device__ __forceinline__ int row_tiles4(const crit_b200_attend_params& p, int r, int count) {
     const int64_t L = p.firsts[r] + ((p.flags & CRIT_B200_ATTEND_CONTEXT) ? 0 : count);
+    if ((p.flags & CRIT_B200_ATTEND_EVEN) && L > (int64_t)p.chunk * p.max_splits) return -1;
     return count > 0 && L > 0 ? (int)((L + 15) >> 4) : 0;
 }
 __device__ __forceinline__ int row_count4(const crit_b200_attend_params& p, int r) {
@@ -210,7 +213,8 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
                 int tiles = 0, subs = 0;
                 if (r < p.n_rows) {
                     const int count = row_count4(p, r);
-                    tiles = row_tiles4(p, r, count), subs = count > 0 ? HG * ((count * G + ROWS - 1) / ROWS) : 0;
+                    tiles = row_tiles4(p, r, count);
+                    tiles = tiles < 0 ? 0 : tiles, subs = count > 0 ? HG * ((count * G + ROWS - 1) / ROWS) : 0;
                 }
                 int scan = tiles * subs;
 #pragma unroll
@@ -743,6 +747,10 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) merge4_kernel(c
     const int count = row_count4(p, r), start = p.starts[r];
     const int tiles = row_tiles4(p, r, count);
     if (col >= count) return;
+    if (tiles < 0) {
+        if (lane == 0 && p.status) atomicExch(p.status, CRIT_B200_STATUS_PLAN);
+        return;
+    }
     const int G = p.q_heads / p.kv_heads, HB = u.heads, HG = p.kv_heads / HB;
     const int h = head / G, hg = h / HB, flat = col * G + head - h * G, ct = flat / rows_tile;
     const int ctiles = (count * G + rows_tile - 1) / rows_tile;
@@ -918,6 +926,8 @@ int64_t even_floats4(const crit_b200_attend_params& p) {
     Decode4Plan plan;
     if (p.kind != CRIT_B200_KIND_INT4 || p.head_dim != p.value_dim) return CRIT_B200_EUNSUPPORTED;
     if (int e = plan4(p, &plan)) return e;
+    // (the launch's tiles are counted in 32 bits)
+    if (((int64_t)p.chunk * p.max_splits / 16 + 1) * p.n_rows > 0x7fffffffLL / ((int64_t)p.kv_heads / plan.u.heads * plan.u.ctiles)) return CRIT_B200_EUNSUPPORTED;
     const int64_t slots = (int64_t)plan.u.blocks + (int64_t)p.n_rows * (p.kv_heads / plan.u.heads) * plan.u.ctiles;
     return (p.n_rows + 2 + 31) / 32 * 32 + slots * plan.u.heads * 8 * plan.nt * (p.head_dim + 2);
 }

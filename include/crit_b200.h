@@ -238,8 +238,9 @@ int crit_b200_compact_blocks(const crit_b200_compact_params* params, void* strea
                                         the m16n8k16 kernel's; both launches (decode and merge) carry the flag */
 #define CRIT_B200_ATTEND_EVEN 512    /* kind 5: the launch's tiles are dealt out in equal runs to the blocks the device holds at once
                                         (a column's bits then depend on the launch), at most 256 rows; a workspace of
-                                        crit_b200_attend_floats floats in a layout of its own (max_splits, partial_rows and offsets
-                                        are not read); both launches carry the flag */
+                                        crit_b200_attend_floats floats in a layout of its own (partial_rows and offsets are not
+                                        read; chunk * max_splits is the positions a table row holds at most: a row of more is left
+                                        out and reported); both launches carry the flag */
 #define CRIT_B200_ATTEND_PARTIALS 32 /* every row's split states go to the workspace, a row of one split too (the first launch
                                         writes nothing to out / lse): what crit_b200_merge_push sends, or what
                                         crit_b200_merge folds */
