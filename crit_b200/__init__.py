@@ -344,7 +344,7 @@ def _append_params(keys, values, slots, key_pages, value_pages, kind, key_scales
         value_at, (value_token, value_head, _), dv = values.data_ptr(), values.stride(), values.shape[-1]
     key_token, key_head, _ = keys.stride()
     p = _lib.block(_lib.AppendParams, keys.data_ptr(), value_at, slots.data_ptr(), key_pages.data_ptr(), _ptr(value_pages), _ptr(key_scales), _ptr(value_scales),
-                   _ptr(_status_word(keys.device)), T, key_pages.numel() // (hkv * key_pages.shape[-1]), key_token, key_head, value_token, value_head,
+                   _ptr(_status_word(keys.device)), T, key_pages.numel() * (2 if k_kind == 5 else 1) // (hkv * d), key_token, key_head, value_token, value_head,
                    hkv, d, dv, page, k_kind, in_dtype, _page_dtype(kind, key_pages), multipliers[0], multipliers[1])
     return p, (keys, values)
 
@@ -465,12 +465,18 @@ def norm_rope_write(q, keys, values, positions, frequencies, slots, key_pages, v
     """norm_rope with write() in the same launch: the queries and keys normed and turned, the keys and the values [tokens]
     [kv_heads][value_dim] (None: keys only) stored at their slots of one layer's pages -> the queries.  The keys go to the
     pages from their FP32 values, with no rounding to their type on the way (16-bit pages hold what norm_rope + write
-    would put there); keys_out takes them too when given.  "fp8:page" pages, whose scales are a page's rows together, take
+    would put there); keys_out takes them too when given (no output lies in the values' memory).  "fp8:page" pages, whose scales are a page's rows together, take
     two launches.  Arguments as norm_rope's and write's."""
     _cuda(q, "q")
     if keys is None:
         raise ValueError("norm_rope_write stores keys (and values): pass keys")
+    if values is not None and values.shape[:2] != keys.shape[:2]:
+        raise ValueError(f"values are a row a token and kv head, like the keys' {list(keys.shape[:2])}, not {list(values.shape[:2])}")
+    if values is not None and values.numel() and any(x is not None and x.data_ptr() == values.data_ptr() for x in (q_out, keys_out)):
+        raise ValueError("an output in the values' place would be stored as the values: pass values of their own")
     if kind == "fp8:page":
+        if keys.shape[0]:                      # (what write() would refuse, before the queries are turned)
+            _append_params(keys, values, slots, key_pages, value_pages, kind, key_scales, value_scales, multipliers)
         found, turned = norm_rope(q, keys, positions, frequencies, q_weight=q_weight, key_weight=key_weight, eps=eps, offset=offset,
                                   axes=axes, interleaved=interleaved, magnitude=magnitude, q_out=q_out, keys_out=keys_out)
         write(turned, values, slots, key_pages, value_pages, kind, key_scales, value_scales, multipliers)
@@ -511,12 +517,14 @@ def gather(pages, kind, page, *, table=None, slots=None, count=None, scales=None
         raise ValueError(f"gather's out is a contiguous bf16, fp16 or fp32 tensor of [{count}][{hkv}][{dim}] on the pages' device")
     elif out.shape != shape:
         out = out.view(shape)
+    if k_kind == 5 and (listed.dtype is not (torch.int32 if slots is None else torch.int64) or (slots is None and listed.numel() * page < count)):
+        raise ValueError(f"int4 rows are read through an int32 page table that holds the {count} positions, or at int64 slots")
     if count == 0:
         return out
     if not pages.is_contiguous():
         raise ValueError("pages are contiguous [slots][kv_heads][dim] storage")
     p = _lib.block(_lib.GatherParams, pages.data_ptr(), _ptr(scales), _ptr(table), _ptr(slots), out.data_ptr(), _ptr(_status_word(pages.device)), count,
-                   pages.numel() // (hkv * pages.shape[-1]), hkv, dim, page, k_kind, _page_dtype(kind, pages), _DTYPES[out.dtype], multiplier)
+                   pages.numel() // (hkv * pages.shape[-1]), hkv, dim, int(page), k_kind, _page_dtype(kind, pages), _DTYPES[out.dtype], multiplier)
     _run("crit_b200_gather", "crit_b200.gather", pages.device, p)
     return out
 
@@ -751,7 +759,7 @@ def attend(q, key_pages, value_pages, kind, tables, rows, starts, firsts, column
     flags = (_STAGINGS[staging] | (4 if persistent else 0) | _ENGINES[engine] | (32 if shards is not None else 0) | (256 if context else 0))
     p = _lib.block(_lib.AttendParams, _ptr(q), _ptr(out), _ptr(lse), _ptr(key_pages), _ptr(value_pages), _ptr(key_scales), _ptr(value_scales),
                    _ptr(tables), _ptr(rows), _ptr(starts), _ptr(counts), _ptr(firsts), _ptr(offsets), _ptr(space), _ptr(_status_word(device)),
-                   space.numel() if space is not None else 0, key_pages.numel() // (hkv * key_pages.shape[-1]), q.stride(0), q.stride(1),
+                   space.numel() if space is not None else 0, key_pages.numel() * (2 if k_kind == 5 else 1) // (hkv * d), q.stride(0), q.stride(1),
                    out.stride(0), out.stride(1), tables.stride(0), R, columns, partial_rows, hq, hkv, d, dv, page, k_kind,
                    _page_dtype(kind, key_pages), _DTYPES[q.dtype], chunk, splits, flags, float(scale if scale is not None else d ** -0.5),
                    float(multipliers[0]), float(multipliers[1]), _ptr(parents), _ptr(sinks), sliding,
@@ -887,6 +895,8 @@ def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scale
     if q.stride(-1) != 1 or out.stride(-1) != 1:
         raise ValueError("q and out have contiguous last dimensions")
     p = _lib.PrefillParams()
+    if k_kind == 5 and torch.is_tensor(position) and position.get_device() != q.get_device():
+        raise ValueError("positions read on the device are on q's device")
     longest = None if torch.is_tensor(position) or table.dim() == 2 else int(position) + T       # positions, where the host knows them
     if table.dim() == 2:             # several sequences, one launch
         S, ahead = table.shape[0], None

@@ -579,3 +579,115 @@ def _attend_with(cache, q, **kw):
     kw = {"key_scales": cache.ks, "value_scales": cache.vs, **kw}
     return pk.attend(q, cache.k, cache.v, "int4", cache.tables, torch.zeros(1, **i32), torch.zeros(1, **i32),
                      torch.tensor([5], device="cuda"), 1, 16, **kw)
+
+
+# -- at the borders of what a call says -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("engine", [None, "mma.sync"])
+def test_a_row_of_more_positions_than_its_table_is_reported_and_left_out(engine):
+    """Two rows, one of which says more positions than a table row holds: the other one is as it should be."""
+    cache = Cache4.filled(8, 128, 16, [100, 70], seed=221)
+    q = _queries(2, 32, 128, torch.bfloat16, 222)
+    before = pk._status[str(q.device)].clone()
+    out, lse = torch.full_like(q, float("nan")), torch.full((2, 32), float("nan"), device="cuda")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    if engine is None:                   # (launches cut into splits end with their grid)
+        firsts = torch.tensor([99, 1 << 40], device="cuda")
+        pk.attend(q, cache.k, cache.v, "int4", cache.tables, torch.arange(2, **i32), torch.arange(2, **i32), firsts, 1, 16, key_scales=cache.ks,
+                  value_scales=cache.vs, out=out, lse=lse)
+        assert pk.status() == 2 and out[1].isnan().all() and lse[1].isnan().all()
+        pk._status[str(q.device)].copy_(before)
+    else:
+        out[:1], lse[:1] = _attend(cache, q[:1], [0], [0], [99], 1, engine=engine)
+    _check(cache, q, out[:1], lse[:1], [0], [0], [99], [1])
+    assert pk.status() == int(before)
+
+
+@pytest.mark.parametrize("hq,hkv,dim,engine", [(32, 8, 128, None), (32, 8, 128, "mma.sync"), (32, 8, 128, "tcgen05:single"), (32, 8, 128, "tcgen05:pair"),
+                                               (8, 2, 64, None), (8, 2, 256, None)])
+def test_what_lies_in_a_prompts_workspace_does_not_matter(hq, hkv, dim, engine):
+    """NaN everywhere in the workspace, and in the pages behind the sequences' ends, against zeros."""
+    cache = Cache4.filled(hkv, dim, 16, [75, 33], seed=231, poison=True)
+    q = _queries(45, hq, dim, torch.bfloat16, 232)
+    found = []
+    for fill in (0.0, float("nan")):
+        space, lse = torch.full((4 << 20,), fill, device="cuda"), torch.empty(45, hq, device="cuda")
+        found.append((pk.prefill(q, cache.k, cache.v, "int4", cache.tables, [45, 18], 16, key_scales=cache.ks, value_scales=cache.vs, starts=[0, 30, 45],
+                                 workspace=space, lse=lse, engine=engine), lse))
+    assert found[0][0].isfinite().all() and torch.equal(found[0][0], found[1][0]) and torch.equal(found[0][1], found[1][1])
+    nothing = pk.prefill(q[:0], cache.k, cache.v, "int4", cache.tables[0], 0, 16, key_scales=cache.ks, value_scales=cache.vs)
+    assert nothing.shape == (0, hq, dim) and pk.status() == 0
+
+
+def test_two_streams_at_once_with_a_workspace_each():
+    """Steps of two owners on two streams, eager and as graphs, interleaved: each as alone."""
+    caches = [Cache4.filled(8, 128, 16, [3000, 500], seed=241), Cache4.filled(8, 128, 16, [1200], seed=242)]
+    queries = [_queries(2, 32, 128, torch.bfloat16, 243), _queries(6, 40, 128, torch.float16, 244)]
+    i32 = dict(dtype=torch.int32, device="cuda")
+    firsts = [torch.tensor([2999, 499], device="cuda"), torch.tensor([1194], device="cuda")]
+    rows = [torch.arange(2, **i32), torch.zeros(1, **i32)]
+    outs = [torch.empty_like(q) for q in queries]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+
+    def step(i, out):
+        c = caches[i]
+        pk.attend(queries[i], c.k, c.v, "int4", c.tables, rows[i], rows[i], firsts[i], 1 if i == 0 else 6, 16, key_scales=c.ks, value_scales=c.vs, out=out)
+        pk.prefill(queries[i][:1], c.k, c.v, "int4", c.tables[0], firsts[i][:1], 16, key_scales=c.ks, value_scales=c.vs)
+    want = [torch.empty_like(q) for q in queries]
+    for i in (0, 1):
+        step(i, want[i])
+    torch.cuda.synchronize()
+    graphs = []
+    for i in (0, 1):
+        with pk.owner(("stream", i)):
+            with torch.cuda.stream(streams[i]):
+                step(i, outs[i])
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=streams[i]):
+                step(i, outs[i])
+            graphs.append(graph)
+    for _ in range(20):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]), pk.owner(("stream", i)):
+                graphs[i].replay()
+                step(i, outs[i])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want)) and pk.status() == 0
+    del graphs
+    for i in (0, 1):
+        pk.release(("stream", i))
+
+
+def test_pages_as_any_view_of_their_storage():
+    """Pages of the other kinds given flat, which the slots' bound is counted from."""
+    keys = _queries(5, 4, 128, torch.bfloat16, 251)
+    slots = torch.tensor([0, 31, 16, 5, 63]).cuda()
+    for kind, store in (("bf16", torch.bfloat16), ("fp8", torch.float8_e4m3fn)):
+        shaped, flat = (torch.zeros(64, 4, 128, dtype=store, device="cuda") for _ in range(2))
+        pk.write(keys, None, slots, shaped, None, kind)
+        pk.write(keys, None, slots, flat.view(64, -1), None, kind)
+        assert torch.equal(shaped.view(torch.uint8), flat.view(torch.uint8)) and shaped.view(torch.uint8).any()
+    assert pk.status() == 0
+
+
+def test_lists_are_refused_under_capture_and_short_tables_always():
+    cache = Cache4.filled(8, 128, 16, [64, 64], seed=261)
+    q = _queries(10, 8, 128, torch.bfloat16, 262)
+    args, kw = (q, cache.k, cache.v, "int4", cache.tables), dict(key_scales=cache.ks, value_scales=cache.vs)
+    want, places = pk.prefill(*args, [3, 40], 16, starts=[0, 4, 10], **kw), torch.tensor([3, 40], device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="under capture"):
+            pk.prefill(*args, [3, 40], 16, **kw)
+        with pytest.raises(RuntimeError, match="under capture"):
+            pk.prefill(*args, places, 16, starts=[0, 4, 10], **kw)
+    assert torch.equal(pk.prefill(*args, [3, 40], 16, starts=[0, 4, 10], **kw), want)
+    with pytest.raises(ValueError, match="page table"):
+        pk.prefill(*args, [3, 1 << 30], 16, starts=[0, 4, 10], **kw)
+    with pytest.raises(ValueError, match="page table"):
+        pk.gather(cache.k, "int4", 16, table=cache.tables[0], count=cache.tables.shape[1] * 16 + 1, scales=cache.ks)
+    with pytest.raises(ValueError, match="page table"):
+        pk.gather(cache.k, "int4", 16, table=cache.tables[0].long(), count=4, scales=cache.ks)
+    with pytest.raises(ValueError, match="int64 slots"):
+        pk.gather(cache.k, "int4", 16, slots=torch.zeros(4, dtype=torch.int32, device="cuda"), scales=cache.ks)
+    assert pk.status() == 0

@@ -267,3 +267,21 @@ def test_what_the_entry_points_refuse():
     pk.norm_rope_write(q, keys, keys, positions, frequencies, torch.tensor([0, 1 << 40, 5]).cuda(), cache.k, cache.v, "int4", cache.ks, cache.vs)
     assert pk.status() == 3
     pk._status[str(q.device)].copy_(before)
+
+
+def test_a_refused_step_leaves_the_queries_as_they_were():
+    q, keys, qw, kw, positions, frequencies = inputs(3, 4, 2, 64, 64, torch.bfloat16, 10)
+    cache, slots, kept = Cache4(2, 64, 16, 2), torch.arange(3).cuda(), q.clone()
+    pages, scales = torch.zeros(2, 16, 2, 64, dtype=torch.float8_e4m3fn, device="cuda"), torch.zeros(2, 2, device="cuda")
+    values = keys.clone()
+    int4, fp8 = (cache.k, cache.v, "int4", cache.ks, cache.vs), (pages, pages.clone(), "fp8:page", scales, scales.clone())
+    for store, change, match in ((int4, {"values": values[:2]}, "a row a token"), (int4, {"values": values[:, :1]}, "a row a token"),
+                                 (int4, {"keys_out": values}, "values' place"), (int4, {"slots": slots[:2]}, "slots"), (fp8, {"slots": slots[:2]}, "slots"),
+                                 (fp8, {"slots": slots.int()}, "slots"), (int4, {"slots": slots.cpu()}, "slots")):
+        call = {"values": values, "slots": slots, "keys_out": None, **change}
+        with pytest.raises(ValueError, match=match):
+            pk.norm_rope_write(q, keys, call["values"], positions, frequencies, call["slots"], *store, q_weight=qw, key_weight=kw, q_out=q, keys_out=call["keys_out"])
+        assert torch.equal(q, kept)
+    # no tokens: nothing is launched, whatever the pages hold
+    none = pk.norm_rope_write(q[:0], keys[:0], values[:0], positions[:0], frequencies, slots[:0], *int4)
+    assert none.shape == (0, 4, 64) and not cache.k.any() and pk.status() == 0
