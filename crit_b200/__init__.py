@@ -56,7 +56,8 @@ def _check_kind(kind, key_scales):
 
 def _check4(pages, scales, what):
     """An "int4" page tensor [...][kv_heads][dim / 2] and its scales [...][kv_heads][dim / 32]: (kv_heads, dim)."""
-    hkv, half = pages.shape[-2:]
+    shape = pages.shape
+    hkv, half = shape[-2], shape[-1]
     if pages.dtype is not torch.uint8 or scales.dtype is not torch.uint8:
         raise ValueError(f"int4 pages and their scales are uint8 tensors: {what} are {pages.dtype} with scales of {scales.dtype}")
     if half % (GROUP4 // 2) or scales.numel() * (GROUP4 // 2) != pages.numel() or not scales.is_contiguous() or not pages.is_contiguous():
@@ -74,7 +75,7 @@ def _cuda(tensor, what):
 
 
 def _ptr(tensor):
-    return tensor.data_ptr() if tensor is not None else None
+    return tensor.data_ptr() if tensor is not None else 0
 
 
 # (the handle alone: a Stream object takes longer to make than a launch's other host work)
@@ -368,7 +369,12 @@ def rope_axes(sections, interleaved=False, device="cuda"):
 def _vectors_fit(x):
     """Whether rows are read or written in the kernel's vectors of four elements as they lie."""
     token, head, element = x.stride()
-    return element == 1 and not (token | head) % 4 and not x.data_ptr() % (4 * x.element_size())
+    return element == 1 and not (token | head) & 3 and not x.data_ptr() % (4 * x.element_size())
+
+
+def _like(x):
+    """An uninitialised contiguous tensor of x's shape, type and device."""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def _vectors(x):
@@ -388,9 +394,10 @@ def _norm_rope_params(q, keys, positions, frequencies, q_weight, key_weight, eps
         raise ValueError("q and keys are bf16, fp16 or fp32 tensors [tokens][heads][dim] of one dtype, width and device")
     if frequencies.dtype is not torch.float32 or frequencies.dim() != 1 or not frequencies.is_contiguous() or frequencies.get_device() != place:
         raise ValueError("frequencies are contiguous FP32 [rotary / 2] on the queries' device")
-    if positions.dim() == 2:
+    ways = positions.dim()
+    if ways == 2:
         n_axes, axis_stride = positions.shape[0], positions.stride(0)
-    if positions.dtype is not torch.int64 or positions.dim() not in (1, 2) or positions.shape[-1] != T or positions.get_device() != place or \
+    if positions.dtype is not torch.int64 or ways not in (1, 2) or positions.shape[-1] != T or positions.get_device() != place or \
             (T > 1 and positions.stride(-1) != 1):
         raise ValueError(f"positions are int64 [{T}], or [axes][{T}], on the queries' device")
     if axes is not None:
@@ -412,12 +419,12 @@ def _norm_rope_params(q, keys, positions, frequencies, q_weight, key_weight, eps
             continue
         read, into = _vectors(x), out
         if out is None and not (writes and what == "keys"):
-            out = into = torch.empty_like(x, memory_format=torch.contiguous_format)
+            out = into = _like(x)
         elif out is not None:
             if out.shape != x.shape or out.dtype != dtype or out.get_device() != place:
                 raise ValueError(f"the {what} output has the shape, dtype and device of {what}")
             if not _vectors_fit(out):                  # made beside it and copied
-                into = torch.empty_like(x, memory_format=torch.contiguous_format)
+                into = _like(x)
                 copies.append((out, into))
         reads.append(read), outs.append(out), at.append((read.data_ptr(), _ptr(into)))
         strides.append(read.stride() + (into.stride() if into is not None else (0, 0, 0)))
@@ -846,9 +853,9 @@ def _expanded(p, q, key_pages, value_pages, key_scales, value_scales, table, pos
     space = _workspace(q.device, floats if workspace is not None or floats < 1 << 24 else 1 << (floats - 1).bit_length(), workspace)
     keys = space.data_ptr()
     values, found = keys + 4 * half, keys + 8 * half
-    on_device = p.positions if several else _ptr(position) if torch.is_tensor(position) else None
+    on_device = p.positions if several else _ptr(position) if torch.is_tensor(position) else 0
     e = _lib.block(_lib.ExpandParams, key_pages.data_ptr(), value_pages.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), table.data_ptr(),
-                   on_device, p.starts, keys, values, found, _ptr(_status_word(q.device)), 0 if on_device else int(position),
+                   on_device or 0, p.starts or 0, keys, values, found, _ptr(_status_word(q.device)), 0 if on_device else int(position),
                    key_pages.numel() * 2 // (hkv * d), table.stride(0) if several else 0, sequences, width, tokens, hkv, d, page, _DTYPES[q.dtype])
     _run("crit_b200_expand", "crit_b200.prefill", q.device, e)
     return keys, values, found, width, pages * page

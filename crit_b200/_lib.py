@@ -113,9 +113,9 @@ _LAYOUTS = {kind: struct.Struct("@" + "".join(_CODES[field[1]] for field in kind
 
 
 def block(kind, *values):
-    """A parameter block from its fields' values in order (a pointer None is NULL): one pack, where a block filled field by
+    """A parameter block from its fields' values in order (a pointer 0 is NULL): one pack, where a block filled field by
     field costs a launch more host time than all its checks."""
-    return kind.from_buffer_copy(_LAYOUTS[kind].pack(*[0 if value is None else value for value in values]))
+    return kind.from_buffer_copy(_LAYOUTS[kind].pack(*values))
 
 
 # name -> (restype, argtypes): every symbol include/crit_b200.h declares
