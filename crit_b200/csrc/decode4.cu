@@ -51,10 +51,11 @@ constexpr int D4_SLACK = 3;
 constexpr int D4_MAX_ROWS = 256;              // window rows an even launch lists
 constexpr int D4_MIN_RUN = 2;                 // tiles an even launch's block takes at least
 
-// The most kv heads a block takes, and the blocks an SM is to hold: a warp's accumulators decide (the registers of 16 warps
-// are 128 a thread, of 8 warps 255).
-constexpr __host__ __device__ int decode4_heads(int d, int nt) { return d == 256 || nt == 4 ? 4 : 8; }
-constexpr __host__ __device__ int decode4_blocks(int d, int nt) { return (nt == 1 && d <= 128) || d == 256 || nt == 4 ? 2 : 1; }
+// The most kv heads a block takes: the pieces asked of HBM are its heads' bytes of a position (8 against 4: 64 sequences of 4,096
+// 81 us against 85, verify windows of 6 143 against 147).  The blocks of so many heads an SM is to hold: a warp's accumulators
+// decide (the registers of 16 warps are 128 a thread, of 8 warps 255).
+constexpr int D4_HEADS = 8;
+constexpr __host__ __device__ int decode4_blocks(int d, int nt) { return nt == 1 && d <= 128 ? 2 : 1; }
 
 struct Decode4Launch {
     int heads;              // kv heads a block takes (HB)
@@ -175,7 +176,7 @@ struct Place4 {
 // does the same arithmetic, n - 8 and the scales on the codes, so that a launch cut into splits gives a column the same bits
 // alone and in any window, and a weight is rounded once, which FP16 outputs' 11 bits ask for.
 template <int D, int NT, bool MASKS, bool FAST>
-__global__ void __launch_bounds__(32 * decode4_heads(D, NT), decode4_blocks(D, NT))
+__global__ void __launch_bounds__(32 * D4_HEADS, decode4_blocks(D, NT))
 decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     constexpr int NG = D / 32;                // groups of a row
     constexpr int ROWS = 8 * NT;
@@ -893,12 +894,12 @@ static int plan4(int q_heads, int kv_heads, int d, int columns, int n_rows, bool
     const int rows = columns * (q_heads / kv_heads);
     const int nt = rows <= 8 ? 1 : (rows <= 16 || d == 256 ? 2 : 4);
     Decode4Launch& u = out->u;
-    u.heads = decode4_heads(d, nt);
+    u.heads = D4_HEADS;
     while (kv_heads % u.heads) u.heads >>= 1;
     u.ctiles = (rows + 8 * nt - 1) / (8 * nt);
     u.row = u.heads * d / 2 < 128 ? u.heads * d / 2 : 128;
     u.stage_bytes = (u.heads * 16 * d + 2 * 16 * kv_heads * (d / 32) + 1023) / 1024 * 1024;
-    const int blocks = decode4_blocks(d, nt) * decode4_heads(d, nt) / u.heads;           // (the registers hold as many)
+    const int blocks = decode4_blocks(d, nt) * D4_HEADS / u.heads;           // (the registers hold as many)
     const int room = (228 * 1024) / blocks - 1024 - 1024 - 4096;                          // (alignment, the driver's, the row lists)
     const int stages = room / u.stage_bytes;
     u.stages = stages < 4 ? 4 : (stages > D4_MAX_STAGES ? D4_MAX_STAGES : stages);
