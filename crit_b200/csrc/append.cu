@@ -218,20 +218,17 @@ __device__ __forceinline__ void load8(const TIN* src, float (&x)[8]) {
     for (int i = 0; i < 8; ++i) x[i] = to_float<TIN>(src[i]);
 }
 
-// 4-bit rows.  Four lanes serve a group of 32 elements of one (token, kv head) of the keys or the values: 8 elements a
-// lane in one 16-byte load, the group's maximum by two shuffles, 8 codes in one 4-byte store.  A block takes 64 groups of a
+// 4-bit rows.  Two lanes serve a group of 32 elements of one (token, kv head) of the keys or the values: 16 elements a
+// lane in two 16-byte loads, the group's maximum by a shuffle, 16 codes in one 8-byte store.  A block takes 128 groups of a
 // token, or a few tokens of fewer groups (grid: tokens, parts of a token), so that no index needs a 64-bit division.  Every byte
 // is read and written once.
-// Measured: 8,192 tokens of 8 heads of 128, keys and values: 15 us with 42 MB moved, 2.8 TB/s; a step of 64 tokens 2 us.  Bound
-// by instructions (174 a warp and 32 groups' quarters, half of them the codes'; the issue slots half full under the loads'
-// latency).  Two tokens a thread with both loads in flight were 0.5 us slower, four 5 us: the registers cost warps.
 template <typename TIN>
 __global__ void __launch_bounds__(256) append4_kernel(const crit_b200_append_params p, const int key_groups, const int per_token, const int per_block,
                                                       const uint32_t magic_k, const uint32_t magic_v) {
-    const uint32_t item = threadIdx.x >> 2;                                      // a group of the block; some quads may have none
-    const int part = threadIdx.x & 3;
+    const uint32_t item = threadIdx.x >> 1;                                      // a group of the block; some pairs may have none
+    const int part = threadIdx.x & 1;
     const uint32_t tok = per_block > 1 ? item / (uint32_t)per_token : 0u;
-    int g = (int)(item - tok * (uint32_t)per_token) + blockIdx.y * 64;
+    int g = (int)(item - tok * (uint32_t)per_token) + blockIdx.y * 128;
     const int64_t t = (int64_t)blockIdx.x * per_block + tok;
     const bool live = (int)tok < per_block && g < per_token && t < p.tokens;
     const bool is_v = g >= key_groups;
@@ -240,19 +237,25 @@ __global__ void __launch_bounds__(256) append4_kernel(const crit_b200_append_par
     const int h = (int)(((uint32_t)g * (is_v ? magic_v : magic_k)) >> 16);      // g / groups
     const TIN* src = is_v ? (const TIN*)p.values + t * p.value_stride_token + (int64_t)h * p.value_stride_head
                           : (const TIN*)p.keys + t * p.key_stride_token + (int64_t)h * p.key_stride_head;
+    src += (g - h * groups) * 32 + part * 16;
     const int row = p.kv_heads * groups;                                        // groups of a slot
     int64_t slot = live ? p.slots[t] : -1;
+    float x[8], y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.f;
+    if (live) load8<TIN>(src, x), load8<TIN>(src + 8, y);                        // (the slot is on its way too)
     if (slot >= 0 && p.slots_total && slot >= p.slots_total) {                   // outside the page tensor: skipped and reported
         if (part == 0 && p.status) atomicExch(p.status, CRIT_B200_STATUS_BOUNDS);
         slot = -1;
     }
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (live) load8<TIN>(src + (g - h * groups) * 32 + part * 8, x);             // (the slot is on its way too)
-    uint32_t byte;
-    const uint32_t w = int4_quantise(x, byte);
+    int bits = max(int4_top(x), int4_top(y));
+    bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
+    const uint32_t byte = int4_scale_byte(__int_as_float(bits), bits > 0x7f800000);
+    const float s = int4_scale(byte);
+    const uint2 w = make_uint2(int4_codes(x, s, byte), int4_codes(y, s, byte));
     if (slot < 0) return;
     const int64_t at = slot * row + g;
-    reinterpret_cast<uint32_t*>(is_v ? p.value_pages : p.key_pages)[at * 4 + part] = w;
+    reinterpret_cast<uint2*>(is_v ? p.value_pages : p.key_pages)[at * 2 + part] = w;
     if (part == 0) reinterpret_cast<uint8_t*>(is_v ? p.value_scales : p.key_scales)[at] = (uint8_t)byte;
 }
 
@@ -260,7 +263,7 @@ template <typename TIN>
 static void launch_append4(const crit_b200_append_params& p, cudaStream_t s) {
     const int groups_k = p.head_dim >> 5, groups_v = p.values ? p.value_dim >> 5 : 1;
     const int key_groups = p.kv_heads * groups_k, per_token = key_groups + (p.values ? p.kv_heads * groups_v : 0);
-    const int per_block = per_token < 64 ? 64 / per_token : 1, parts = (per_token + 63) / 64;
+    const int per_block = per_token < 128 ? 128 / per_token : 1, parts = (per_token + 127) / 128;
     // g / groups as (g * ceil(2^16 / groups)) >> 16: exact for g below 2^13 (the excess is below 8 / 2^16 a unit)
     const uint32_t magic_k = (65536u + groups_k - 1) / groups_k, magic_v = (65536u + groups_v - 1) / groups_v;
     const int64_t blocks = (p.tokens + per_block - 1) / per_block;
@@ -274,7 +277,7 @@ int check_append(const crit_b200_append_params& p) {
     if (!width_ok(p.head_dim) || (p.values && !width_ok(p.value_dim))) return CRIT_B200_EUNSUPPORTED;
     if (p.kind < 0 || p.kind > CRIT_B200_KIND_INT4) return CRIT_B200_EUNSUPPORTED;
     if (p.kind == CRIT_B200_KIND_INT4 && (int64_t)p.kv_heads * (p.head_dim > p.value_dim ? p.head_dim : p.value_dim) >= 32 * 8192) return CRIT_B200_EUNSUPPORTED;
-    if (p.kind == CRIT_B200_KIND_INT4 && (!aligned(p.key_pages, 4) || (p.values && !aligned(p.value_pages, 4)))) return CRIT_B200_EALIGN;
+    if (p.kind == CRIT_B200_KIND_INT4 && (!aligned(p.key_pages, 8) || (p.values && !aligned(p.value_pages, 8)))) return CRIT_B200_EALIGN;
     if (p.kind >= CRIT_B200_KIND_FP8_ROW && (!p.key_scales || (p.values && !p.value_scales))) return CRIT_B200_EINVAL;
     if (p.kind == CRIT_B200_KIND_16BIT && p.page_dtype == CRIT_B200_DTYPE_FP32 && p.in_dtype != CRIT_B200_DTYPE_FP32)
         ;   // widening into FP32 pages is served too

@@ -42,54 +42,45 @@ __global__ void __launch_bounds__(128) gather_kernel(const crit_b200_gather_para
     }
 }
 
-// 4-bit rows back: a thread takes 8 codes (one 4-byte load) to 8 values, (code - 8) * scale in FP32 (exact), in one 16-byte
-// store for 16-bit types.  A block takes 256 words of a position, or a few positions of fewer words, and does so for
-// POSITIONS positions in turn, whose loads are in flight together.  Bound by the bytes it writes.
-template <typename TOUT, int POSITIONS>
-__global__ void __launch_bounds__(256) gather4_kernel(const crit_b200_gather_params p, const int words, const int per_block) {
-    const uint32_t tok = per_block > 1 ? threadIdx.x / (uint32_t)words : 0u;
-    const int w = (int)(threadIdx.x - tok * words) + blockIdx.y * 256;            // the word of 8 codes among the position's
-    if ((int)tok >= per_block || w >= words) return;
-    const int64_t n0 = (int64_t)blockIdx.x * (per_block * POSITIONS) + tok;
-    uint32_t codes[POSITIONS], byte[POSITIONS];
-#pragma unroll
-    for (int u = 0; u < POSITIONS; ++u) {
-        const int64_t n = n0 + u * per_block;
-        codes[u] = 0x88888888u, byte[u] = 0u;
-        if (n >= p.count) continue;
-        const int64_t slot = p.slots ? p.slots[n] : (int64_t)p.table[n / p.page] * p.page + n % p.page;
-        if (p.slots_total && (slot < 0 || slot >= p.slots_total)) {      // outside the page tensor: zeros, and reported
-            if (w == 0 && p.status) atomicExch(p.status, CRIT_B200_STATUS_BOUNDS);
-            continue;
-        }
-        const int64_t at = slot * words + w;
-        codes[u] = reinterpret_cast<const uint32_t*>(p.pages)[at];
-        byte[u] = reinterpret_cast<const uint8_t*>(p.scales)[at >> 2];
+// 4-bit rows back: a thread takes 16 codes (one 8-byte load) to 16 values, (code - 8) * scale in FP32 (exact), in 16-byte
+// stores.  A block takes 256 such pieces of a position, or a few positions of fewer.  Bound by the bytes it writes.
+template <typename TOUT>
+__global__ void __launch_bounds__(256) gather4_kernel(const crit_b200_gather_params p, const int pieces, const int per_block) {
+    const uint32_t tok = per_block > 1 ? threadIdx.x / (uint32_t)pieces : 0u;
+    const int w = (int)(threadIdx.x - tok * pieces) + blockIdx.y * 256;           // the piece of 16 codes among the position's
+    const int64_t n = (int64_t)blockIdx.x * per_block + tok;
+    if ((int)tok >= per_block || w >= pieces || n >= p.count) return;
+    const int64_t slot = p.slots ? p.slots[n] : (int64_t)p.table[n / p.page] * p.page + n % p.page;
+    uint2 codes = make_uint2(0x88888888u, 0x88888888u);
+    uint32_t byte = 0u;
+    if (p.slots_total && (slot < 0 || slot >= p.slots_total)) {              // outside the page tensor: zeros, and reported
+        if (w == 0 && p.status) atomicExch(p.status, CRIT_B200_STATUS_BOUNDS);
+    } else {
+        const int64_t at = slot * pieces + w;
+        codes = reinterpret_cast<const uint2*>(p.pages)[at];
+        byte = reinterpret_cast<const uint8_t*>(p.scales)[at >> 1];
     }
+    const float s = int4_scale(byte);
+    TOUT* dst = (TOUT*)p.out + (n * pieces + w) * 16;
 #pragma unroll
-    for (int u = 0; u < POSITIONS; ++u) {
-        const int64_t n = n0 + u * per_block;
-        if (n >= p.count) return;
+    for (int half = 0; half < 2; ++half) {
         float v[8];
-        int4_values(codes[u], int4_scale(byte[u]), v);
-        TOUT* dst = (TOUT*)p.out + (n * words + w) * 8;
+        int4_values(half ? codes.y : codes.x, s, v);
         if constexpr (sizeof(TOUT) == 2) {
             constexpr bool BF16 = std::is_same<TOUT, __nv_bfloat16>::value;
-            *reinterpret_cast<uint4*>(dst) = make_uint4(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]), pack2<BF16>(v[4], v[5]), pack2<BF16>(v[6], v[7]));
+            reinterpret_cast<uint4*>(dst)[half] = make_uint4(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]), pack2<BF16>(v[4], v[5]), pack2<BF16>(v[6], v[7]));
         } else {
-            *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
+            reinterpret_cast<float4*>(dst)[2 * half] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4*>(dst)[2 * half + 1] = make_float4(v[4], v[5], v[6], v[7]);
         }
     }
 }
 
 template <typename TOUT>
-static void launch_gather4(const crit_b200_gather_params& p, int words, cudaStream_t s) {
-    const int per_block = words < 256 ? 256 / words : 1;
-    const unsigned parts = (unsigned)((words + 255) / 256);
-    const int64_t blocks = (p.count + per_block - 1) / per_block;
-    if (blocks * parts >= 4096) gather4_kernel<TOUT, 4><<<dim3((unsigned)((blocks + 3) / 4), parts), 256, 0, s>>>(p, words, per_block);
-    else gather4_kernel<TOUT, 1><<<dim3((unsigned)blocks, parts), 256, 0, s>>>(p, words, per_block);
+static void launch_gather4(const crit_b200_gather_params& p, int pieces, cudaStream_t s) {
+    const int per_block = pieces < 256 ? 256 / pieces : 1;
+    const dim3 grid((unsigned)((p.count + per_block - 1) / per_block), (unsigned)((pieces + 255) / 256));
+    gather4_kernel<TOUT><<<grid, 256, 0, s>>>(p, pieces, per_block);
 }
 
 // The sequences' 4-bit pages as 16-bit ones, in the order of their tables: block = (page of the table, sequence, keys or
@@ -179,12 +170,12 @@ extern "C" __attribute__((visibility("default"))) int crit_b200_gather(const cri
     if (p.kind > CRIT_B200_KIND_INT4) return CRIT_B200_EUNSUPPORTED;
     if (p.kind == CRIT_B200_KIND_INT4) {
         if (p.dim % 32) return CRIT_B200_EUNSUPPORTED;
-        if (!aligned(p.pages, 4) || !aligned(p.out, 16)) return CRIT_B200_EALIGN;
-        const int words = p.kv_heads * (p.dim >> 3);
+        if (!aligned(p.pages, 8) || !aligned(p.out, 16)) return CRIT_B200_EALIGN;
+        const int pieces = p.kv_heads * (p.dim >> 4);
         switch (p.out_dtype) {
-            case CRIT_B200_DTYPE_BF16: launch_gather4<__nv_bfloat16>(p, words, (cudaStream_t)stream); break;
-            case CRIT_B200_DTYPE_FP16: launch_gather4<__half>(p, words, (cudaStream_t)stream); break;
-            case CRIT_B200_DTYPE_FP32: launch_gather4<float>(p, words, (cudaStream_t)stream); break;
+            case CRIT_B200_DTYPE_BF16: launch_gather4<__nv_bfloat16>(p, pieces, (cudaStream_t)stream); break;
+            case CRIT_B200_DTYPE_FP16: launch_gather4<__half>(p, pieces, (cudaStream_t)stream); break;
+            case CRIT_B200_DTYPE_FP32: launch_gather4<float>(p, pieces, (cudaStream_t)stream); break;
             default: return CRIT_B200_EINVAL;
         }
         CRIT_CHECK_LAUNCH();

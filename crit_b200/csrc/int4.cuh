@@ -97,12 +97,17 @@ __device__ __forceinline__ void int4_values(uint32_t codes, float s, float (&v)[
     for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(__fadd_rn(__uint_as_float(0x4b000000u | ((codes >> (4 * i)) & 15u)), -8388616.f), s);
 }
 
-// The four lanes that hold a group (8 elements each, lanes 4 k .. 4 k + 3) agree on its scale byte; the lane's code word.
-__device__ __forceinline__ uint32_t int4_quantise(float (&x)[8], uint32_t& byte) {
+// max |x| of eight elements, its bits: their order as integers is the floats', a NaN above infinity.
+__device__ __forceinline__ int int4_top(const float (&x)[8]) {
     float amax = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(amax) : "f"(fabsf(x[i])));
-    int bits = __float_as_int(amax) & 0x7fffffff;       // (their order as integers is the floats', a NaN above infinity)
+    return __float_as_int(amax) & 0x7fffffff;
+}
+
+// The four lanes that hold a group (8 elements each, lanes 4 k .. 4 k + 3) agree on its scale byte; the lane's code word.
+__device__ __forceinline__ uint32_t int4_quantise(float (&x)[8], uint32_t& byte) {
+    int bits = int4_top(x);
     bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
     bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 2));
     byte = int4_scale_byte(__int_as_float(bits), bits > 0x7f800000);
