@@ -222,6 +222,10 @@ __device__ __forceinline__ void load8(const TIN* src, float (&x)[8]) {
 // lane in two 16-byte loads, the group's maximum by a shuffle, 16 codes in one 8-byte store.  A block takes 128 groups of a
 // token, or a few tokens of fewer groups (grid: tokens, parts of a token), so that no index needs a 64-bit division.  Every byte
 // is read and written once.
+// Measured: 8,192 tokens of 8 heads of 128, keys and values, to scattered slots: 13.5 us for 42.5 MB, 3.1 TB/s (floor 6.5 us); a
+// step of 64 tokens 2.2 us, the launch.  Bound by instructions: with 8 elements a lane what a lane does once (address, scale,
+// reciprocal) was 130 of its 174 instructions, 17.6 us.  Several tokens a thread with their loads in flight together were
+// slower (two 0.5 us, four 5 us): their registers cost the warps that hide the loads.
 template <typename TIN>
 __global__ void __launch_bounds__(256) append4_kernel(const crit_b200_append_params p, const int key_groups, const int per_token, const int per_block,
                                                       const uint32_t magic_k, const uint32_t magic_v) {

@@ -3,9 +3,10 @@
 // A block is a warp for each of HB kv heads (8, 4, 2 or 1: the most that divides the heads) and reads whole page rows, 16
 // positions of its HB heads a tile: one box of a tensor map with permuted dimensions, [128 bytes][slots][rows of 128 a slot], is
 // HB * dim / 2 contiguous bytes a position and lands with a few heads' (two of dim 128) 16 positions together, swizzled.  So the
-// bytes asked of HBM are long pieces although a row of one head is 64 bytes (dim 128).  The tile's scales come by a bulk copy onto the same
-// mbarrier.  There is no producer warp (a ninth warp would take the registers of two blocks an SM): the warps take turns,
-// warp n mod HB refills the ring when it comes to tile n, with a tile S - 3 ahead and the page id it read a turn before.
+// bytes asked of HBM are long pieces although a row of one head is 64 bytes (dim 128).  The tile's scales come by a
+// bulk copy onto the same mbarrier.  There is no producer warp (a ninth warp would take the registers of two blocks an SM): the
+// warps take turns, warp n mod HB refills the ring when it comes to tile n, with a tile S - 3 ahead and the page id it read
+// a turn before.
 //
 // A warp attends its own head's query rows (up to 8 NT: the columns of a verify window times the heads of the kv head's
 // group) and waits for the others only through the ring.  Scores and outputs are m16n8k16 products, positions or value
@@ -23,8 +24,9 @@
 // where 1024 + n less 1032 takes an OR and an add more.  The factor 16 is undone in the queries (their odd elements are
 // divided by 16) and in the outputs' odd columns, 2^-24 in a constant.  The 8 that a code stands above its value comes off in
 // products of their own: the positions' scales with -8 * the sums of the groups' queries (a K of the groups' number, the sums
-// as two FP16 terms), and a constant matrix with P^T, which gathers -8 * the sum of the group's weights.  Where the accumulators for that do not fit the registers (wide tiles of query
-// rows, the outputs of 256-wide heads), codes become n - 8 one add later.
+// as two FP16 terms), and a constant matrix with P^T, which gathers -8 * the sum of the
+// group's weights.  Where the accumulators for that do not fit the registers (wide tiles of query rows, the outputs of
+// 256-wide heads), codes become n - 8 one add later.
 //
 // The queries become FP16 with an exponent of their own a row (the largest element between 2^13 and 2^14), so no bf16 query
 // overflows or vanishes.  Weights are 2^(x - ref) with a reference that moves only when a score passes it (by 14 in the
@@ -35,6 +37,15 @@
 // (CRIT_B200_ATTEND_EVEN): the launch's tiles, rows in order, are dealt out in equal runs to the blocks the device holds at
 // once; where a run and a row overlap there is one state, slot = block + row (both only grow along the tiles, so the sum
 // names the pair), and merge4_kernel folds a row's consecutive slots.  No block idles while another has two splits to go.
+//
+// Measured (B200, CUDA events around graphs; HBM's floor at the measured copy bandwidth beside it): 64 rows of 4,096 positions,
+// 64 query heads on 8 of 128: 81 us (44), 3.5 TB/s; one row of 200,000, 24 on 4 of 256: 67 us (33); 32 verify windows of 6 columns, 40
+// on 8 of 128, FP16: 143 us (27); one row of 777: 11 us, two launches' latency.  Bound by instructions at the registers' occupancy:
+// of the 64 rows' launch about 340 a warp and tile (V 100, K 60, scales and softmax the rest) fill 60% of the issue slots with
+// 16 warps an SM, the integer pipe 56%, the tensor pipe a quarter; of the verify windows' 720 a tile with 8 warps an SM fill
+// 45%, each warp waiting for its own last result.  The same tiles streamed without the products take about 60 us.
+// Slower: a block's queries in shared memory for 3 blocks an SM (104 us against 85), 3 blocks of 256-wide heads (75 against 70),
+// the shifts of the codes as multiplications (87 against 81).
 #include <mutex>
 #include <type_traits>
 
@@ -49,7 +60,6 @@ constexpr int D4_MAX_STAGES = 8;
 // 128: 80.6 us instead of 84.7; the other sizes 0 to 1%).
 constexpr int D4_SLACK = 3;
 constexpr int D4_MAX_ROWS = 256;              // window rows an even launch lists
-constexpr int D4_MIN_RUN = 2;                 // tiles an even launch's block takes at least
 
 // The most kv heads a block takes: the pieces asked of HBM are its heads' bytes of a position (8 against 4: 64 sequences of 4,096
 // 81 us against 85, verify windows of 6 143 against 147).  The blocks of so many heads an SM is to hold: a warp's accumulators
@@ -230,7 +240,7 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
         }
         __syncthreads();
         const int total = list_first[p.n_rows];
-        const int share = (total + u.blocks - 1) / u.blocks, run = share > D4_MIN_RUN ? share : D4_MIN_RUN;
+        const int share = (total + u.blocks - 1) / u.blocks, run = share > 1 ? share : 1;
         if (blockIdx.x == 0) {      // what the fold reads: the run, and where a row begins
             int* info = reinterpret_cast<int*>(p.workspace);
             for (int r = threadIdx.x; r <= p.n_rows; r += blockDim.x) info[1 + r] = list_first[r];
@@ -964,7 +974,8 @@ static void launch_merge4_of(const crit_b200_attend_params& p, const Decode4Plan
 int launch_merge4(const crit_b200_attend_params& p, cudaStream_t s) {
     Decode4Plan plan;
     if (int e = plan4(p, &plan)) return e;
-    // few rows share the blocks: a row may have a state in each, so a block folds it; many rows have a few states each
+    // Few rows share the blocks: a row may have a state in each, so 16 warps fold it; many rows have a few states each, a warp's
+    // work.  One row of 200,000: 67 us, with a warp 147; 64 rows of 4,096: 81 us, with 16 warps 115 (launch and fold together).
     const bool many = (int64_t)p.n_rows * (p.kv_heads / plan.u.heads) * plan.u.ctiles * 16 < plan.u.blocks;
     switch (p.head_dim) {
         case 64: launch_merge4_of<64>(p, plan, many, s); break;
