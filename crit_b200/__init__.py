@@ -22,6 +22,7 @@ tolerance, integer and byte results (slots, codes, scales) bit for bit.
 """
 import contextlib
 import ctypes
+import struct
 import math
 import threading
 
@@ -656,26 +657,26 @@ def attend(q, key_pages, value_pages, kind, tables, rows, starts, firsts, column
     k_kind = _check_kind(kind, key_scales)
     _cuda(q, "q")
     T, hq, d = q.shape
-    hkv, dv = key_pages.shape[-2], value_pages.shape[-1]
+    hkv, dv, place = key_pages.shape[-2], value_pages.shape[-1], q.get_device()
     if k_kind == 5:
         if value_scales is None:
             raise ValueError("int4 pages take scales beside their codes, keys and values alike")
         if _check4(key_pages, key_scales, "keys") != (hkv, d) or _check4(value_pages, value_scales, "values") != (hkv, d):
             raise ValueError(f"int4 pages hold keys and values of q's width, [...][kv_heads][{d // 2}]")
-        if key_pages.numel() != value_pages.numel() or key_pages.device != q.device or value_pages.device != q.device:
+        if key_pages.numel() != value_pages.numel() or key_pages.get_device() != place or value_pages.get_device() != place:
             raise ValueError("int4 keys and values are as many pages each, on q's device")
         dv = d
     R = int(starts.shape[0])
     if hq % hkv or not 1 <= columns <= MAX_COLUMNS or R == 0:
         raise ValueError("query heads a multiple of the KV heads, 1..64 columns a row, one row or more")
-    if q.stride(-1) != 1:
+    (q_token, q_head, q_element), q_dtype = q.stride(), q.dtype
+    if q_element != 1:
         raise ValueError("q's last dimension is contiguous")
-    if q.dtype not in (torch.bfloat16, torch.float16):
+    if q_dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("q is bf16 or fp16")
     if (offsets is None) != (tokens is None):
         raise ValueError("offsets come with the partial rows they take (tokens)")
     if k_kind == 5:
-        place = q.get_device()
         for x in (tables, rows, starts, firsts, counts, offsets, out, lse):
             if x is not None and x.get_device() != place:
                 raise ValueError("attend's tensors are on q's device")
@@ -685,7 +686,7 @@ def attend(q, key_pages, value_pages, kind, tables, rows, starts, firsts, column
     page = int(page)
     if page % TILE:
         raise ValueError(f"crit_b200 reads pages of a multiple of {TILE} positions, not {page}")
-    if not key_pages.is_contiguous() or not value_pages.is_contiguous():
+    if k_kind != 5 and (not key_pages.is_contiguous() or not value_pages.is_contiguous()):       # (int4: checked above)
         raise ValueError("pages are contiguous [slots][kv_heads][dim] storage")
     device = q.device
     positions = tables.shape[1] * page
@@ -750,8 +751,10 @@ def attend(q, key_pages, value_pages, kind, tables, rows, starts, firsts, column
         engine = "mma.sync"               # the caller's chunk is not one the chosen kernel takes
     splits = states_for(parts_for(positions, chunk), engine)
     partial_rows = R * columns if offsets is None else int(tokens)
-    out = torch.empty(T, hq, dv, dtype=q.dtype, device=device) if out is None else out
-    if out.dtype != q.dtype or out.stride(-1) != 1:
+    if out is None:
+        out = _like(q) if dv == d else torch.empty(T, hq, dv, dtype=q_dtype, device=device)
+    (out_token, out_head, out_element) = out.stride()
+    if out.dtype != q_dtype or out_element != 1:
         raise ValueError("out is in q's dtype, its last dimension contiguous")
     if engine == "even" and k_kind != 5:
         raise NotImplementedError("the even engine reads int4 pages")
@@ -764,16 +767,16 @@ def attend(q, key_pages, value_pages, kind, tables, rows, starts, firsts, column
         space = _workspace(device, workspace_floats(partial_rows, hq, splits, dv), workspace)
     columns = int(columns)
     flags = (_STAGINGS[staging] | (4 if persistent else 0) | _ENGINES[engine] | (32 if shards is not None else 0) | (256 if context else 0))
-    p = _lib.block(_lib.AttendParams, _ptr(q), _ptr(out), _ptr(lse), _ptr(key_pages), _ptr(value_pages), _ptr(key_scales), _ptr(value_scales),
-                   _ptr(tables), _ptr(rows), _ptr(starts), _ptr(counts), _ptr(firsts), _ptr(offsets), _ptr(space), _ptr(_status_word(device)),
-                   space.numel() if space is not None else 0, key_pages.numel() * (2 if k_kind == 5 else 1) // (hkv * d), q.stride(0), q.stride(1),
-                   out.stride(0), out.stride(1), tables.stride(0), R, columns, partial_rows, hq, hkv, d, dv, page, k_kind,
-                   _page_dtype(kind, key_pages), _DTYPES[q.dtype], chunk, splits, flags, float(scale if scale is not None else d ** -0.5),
+    p = _lib.block(_lib.AttendParams, q.data_ptr(), out.data_ptr(), _ptr(lse), key_pages.data_ptr(), value_pages.data_ptr(), _ptr(key_scales), _ptr(value_scales),
+                   tables.data_ptr(), rows.data_ptr(), starts.data_ptr(), _ptr(counts), firsts.data_ptr(), _ptr(offsets), _ptr(space), _ptr(_status_word(device)),
+                   space.numel() if space is not None else 0, key_pages.numel() * (2 if k_kind == 5 else 1) // (hkv * d), q_token, q_head,
+                   out_token, out_head, tables.stride(0), R, columns, partial_rows, hq, hkv, d, dv, page, k_kind,
+                   _page_dtype(kind, key_pages), _DTYPES[q_dtype], chunk, splits, flags, float(scale if scale is not None else d ** -0.5),
                    float(multipliers[0]), float(multipliers[1]), _ptr(parents), _ptr(sinks), sliding,
                    blocks.shape[1] if blocks is not None else 0, int(block_size) if blocks is not None else 0, _ptr(blocks))
     lib = _lib.load()
     if engine == "even":
-        key = (device.index, R, columns, hq, hkv, d, q.dtype, parents is not None or sliding > 0 or blocks is not None)
+        key = (place, R, columns, hq, hkv, d, q_dtype, parents is not None or sliding > 0 or blocks is not None)
         floats = _even_floats.get(key)
         if floats is None:
             with torch.cuda.device(device):
@@ -830,7 +833,7 @@ def prefill_serves(head_dim, value_dim, q_dtype, kind, page):
 
 
 # -- prompt chunks ------------------------------------------------------------------------------------------------------
-def _expanded(p, q, key_pages, value_pages, key_scales, value_scales, table, position, tokens, longest, page, workspace):
+def _expanded(positions_at, starts_at, q, key_pages, value_pages, key_scales, value_scales, table, position, tokens, longest, page, workspace):
     """4-bit pages as 16-bit ones of q's type in the workspace, one launch, in the order of the sequences' tables: the
     addresses of the keys, the values and the table that reads them, its width, and the slots of the pages."""
     hkv, d = key_pages.shape[-2], q.shape[-1]
@@ -853,21 +856,27 @@ def _expanded(p, q, key_pages, value_pages, key_scales, value_scales, table, pos
     space = _workspace(q.device, floats if workspace is not None or floats < 1 << 24 else 1 << (floats - 1).bit_length(), workspace)
     keys = space.data_ptr()
     values, found = keys + 4 * half, keys + 8 * half
-    on_device = p.positions if several else _ptr(position) if torch.is_tensor(position) else 0
+    on_device = positions_at if several else _ptr(position) if torch.is_tensor(position) else 0
     e = _lib.block(_lib.ExpandParams, key_pages.data_ptr(), value_pages.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), table.data_ptr(),
-                   on_device or 0, p.starts or 0, keys, values, found, _ptr(_status_word(q.device)), 0 if on_device else int(position),
+                   on_device, starts_at, keys, values, found, _ptr(_status_word(q.device)), 0 if on_device else int(position),
                    key_pages.numel() * 2 // (hkv * d), table.stride(0) if several else 0, sequences, width, tokens, hkv, d, page, _DTYPES[q.dtype])
     _run("crit_b200_expand", "crit_b200.prefill", q.device, e)
     return keys, values, found, width, pages * page
 
 
-def _sent(numbers, dtype, device):
-    """A list on the device; the host does not wait for the device (the driver takes its copy of pageable memory at the
-    call).  A capture would record the address of the host's list instead: refused."""
-    if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("crit_b200.prefill: under capture the positions are a tensor on the device and the starts are left out "
-                           "(a list of them is copied from the host)")
-    return torch.tensor(numbers, dtype=dtype).to(device, non_blocking=True)
+def _sent(positions, starts, device):
+    """Lists of positions (int64; None: none) and starts (int32; None: none) on the device: (the tensor that holds them, the
+    address of the starts).  They go as a small kernel's parameters, which wait for nothing and which a capture keeps; a copy
+    would leave a captured graph with the address of memory that is gone."""
+    numbers, odd = list(positions or ()), list(starts or ())
+    if len(odd) % 2:
+        odd.append(0)
+    at = len(numbers)
+    numbers += [a | b << 32 for a, b in zip(odd[::2], odd[1::2])]
+    held = torch.empty(len(numbers), dtype=torch.int64, device=device)
+    to = held.data_ptr()
+    _run("crit_b200_put", "crit_b200.prefill", device, to, struct.pack(f"{len(numbers)}q", *numbers), len(numbers))
+    return held, to + 8 * at
 
 
 def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scales=None, value_scales=None,
@@ -901,7 +910,7 @@ def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scale
         table = table.to(torch.int32).contiguous()       # (the reference's pool hands its tables over as int64 slices)
     if q.stride(-1) != 1 or out.stride(-1) != 1:
         raise ValueError("q and out have contiguous last dimensions")
-    p = _lib.PrefillParams()
+    positions_at = starts_at = sequences = table_stride = 0
     if k_kind == 5 and torch.is_tensor(position) and position.get_device() != q.get_device():
         raise ValueError("positions read on the device are on q's device")
     longest = None if torch.is_tensor(position) or table.dim() == 2 else int(position) + T       # positions, where the host knows them
@@ -911,8 +920,7 @@ def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scale
             if len(position) != S:
                 raise ValueError("one position a sequence")
             ahead = [int(x) for x in position]
-            position = _sent(ahead, torch.int64, q.device)
-        if position.dtype != torch.int64 or position.numel() != S or not position.is_cuda or not position.is_contiguous():
+        elif position.dtype != torch.int64 or position.numel() != S or not position.is_cuda or not position.is_contiguous():
             raise ValueError("the sequences' positions are an int64 tensor [S] on the device")
         if starts is None:
             if T % S:
@@ -925,36 +933,33 @@ def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scale
                 raise ValueError("starts: S + 1 rising row numbers from 0 to the number of tokens")
             counts = [b - a for a, b in zip(starts, starts[1:])]
             most = max(counts)
-            starts = _sent(starts, torch.int32, q.device)
-            p.starts = _ptr(starts)
-        p.positions, p.sequences, p.table_stride = _ptr(position), S, table.stride(0)
-        T, position, held = most, 0, position
+        held = position                      # (kept until both launches are made)
+        if ahead is not None or starts is not None:
+            held, at = _sent(ahead, starts, q.device)
+            starts_at = at if starts is not None else 0
+        positions_at, sequences, table_stride = (position if ahead is None else held).data_ptr(), S, table.stride(0)
+        T, position = most, 0
         longest = max((a + n for a, n in zip(ahead, counts)), default=0) if ahead is not None else None
     elif starts is not None:
         raise ValueError("starts goes with a table of several sequences")
     if torch.is_tensor(position) and (position.dtype != torch.int64 or position.numel() != 1 or not position.is_cuda):
         raise ValueError("a position read on the device is a one-element int64 tensor there")
-    p.q, p.out, p.lse = q.data_ptr(), out.data_ptr(), _ptr(lse)
+    page, q_code = int(page), _DTYPES[q.dtype]
     if k_kind == 5:
-        p.key_pages, p.value_pages, p.table, width, p.slots = _expanded(p, q, key_pages, value_pages, key_scales, value_scales, table, position, T,
-                                                                        longest, int(page), workspace)
-        p.table_stride = width if p.sequences else 0
-        p.kind, p.page_dtype = 0, _DTYPES[q.dtype]
+        keys_at, values_at, table_at, width, slots = _expanded(positions_at, starts_at, q, key_pages, value_pages, key_scales, value_scales, table, position,
+                                                               T, longest, page, workspace)
+        key_scales = value_scales = None
+        table_stride, k_kind, page_dtype = width if sequences else 0, 0, q_code
     else:
-        p.key_pages, p.value_pages = _ptr(key_pages), _ptr(value_pages)
-        p.key_scales, p.value_scales = _ptr(key_scales), _ptr(value_scales)
-        p.table, p.slots = _ptr(table), key_pages.numel() // (hkv * d)
-        p.kind, p.page_dtype = k_kind, _page_dtype(kind, key_pages)
-    if torch.is_tensor(position):
-        p.position_ptr = _ptr(position)
-    else:
-        p.position = int(position)
-    p.q_stride_token, p.q_stride_head, _ = q.stride()
-    p.out_stride_token, p.out_stride_head, _ = out.stride()
-    p.flags = _PREFILL_ENGINES[engine]
-    p.status = _ptr(_status_word(q.device))
-    p.tokens, p.q_heads, p.kv_heads, p.head_dim, p.value_dim, p.page, p.q_dtype = T, hq, hkv, d, d, int(page), _DTYPES[q.dtype]
-    p.scale = float(scale if scale is not None else d ** -0.5)
-    p.key_multiplier, p.value_multiplier = float(multipliers[0]), float(multipliers[1])
-    _run("crit_b200_prefill", "crit_b200.prefill", q.device, p)
+        keys_at, values_at, table_at, slots = key_pages.data_ptr(), value_pages.data_ptr(), table.data_ptr(), key_pages.numel() // (hkv * d)
+        page_dtype = _page_dtype(kind, key_pages)
+    device = q.device
+    position_at, position = (position.data_ptr(), 0) if torch.is_tensor(position) else (0, int(position))
+    q_token, q_head, _ = q.stride()
+    out_token, out_head, _ = out.stride()
+    p = _lib.block(_lib.PrefillParams, q.data_ptr(), out.data_ptr(), _ptr(lse), keys_at, values_at, _ptr(key_scales), _ptr(value_scales), table_at, position_at,
+                   _ptr(_status_word(device)), position, slots, q_token, q_head, out_token, out_head, T, hq, hkv, d, d, page, k_kind, page_dtype, q_code,
+                   _PREFILL_ENGINES[engine], float(scale if scale is not None else d ** -0.5), float(multipliers[0]), float(multipliers[1]),
+                   starts_at, positions_at, sequences, table_stride)
+    _run("crit_b200_prefill", "crit_b200.prefill", device, p)
     return out

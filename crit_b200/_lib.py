@@ -132,6 +132,7 @@ SYMBOLS = {
     "crit_b200_merge_shards": (c_int, [POINTER(MergeShardsParams), c_void_p]),
     "crit_b200_move_rows": (c_int, [POINTER(MoveParams), c_void_p]),
     "crit_b200_compact_blocks": (c_int, [POINTER(CompactParams), c_void_p]),
+    "crit_b200_put": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
     "crit_b200_expand": (c_int, [POINTER(ExpandParams), c_void_p]),
     "crit_b200_norm_rope": (c_int, [POINTER(NormRopeParams), POINTER(AppendParams), c_void_p]),
     "crit_b200_prefill": (c_int, [POINTER(PrefillParams), c_void_p]),

@@ -1,4 +1,5 @@
 // Block-table page gather with dequantisation, slot mapping on the device, and the merge of shards' partials.
+#include <cstring>
 #include <type_traits>
 
 #include "int4.cuh"
@@ -116,6 +117,18 @@ __global__ void __launch_bounds__(256) expand4_kernel(const crit_b200_expand_par
         }
         out[i] = make_uint4(pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3]), pack2<BF16>(v[4], v[5]), pack2<BF16>(v[6], v[7]));
     }
+}
+
+// A few numbers from the host: a launch's parameters are taken at the call and kept by a capture, where a copy of pageable
+// memory would be neither quick nor the capture's own.
+constexpr int PUT_NUMBERS = 256;
+struct PutNumbers {
+    int64_t* to;
+    int n;
+    int64_t numbers[PUT_NUMBERS];
+};
+__global__ void __launch_bounds__(PUT_NUMBERS) put_kernel(const __grid_constant__ PutNumbers p) {
+    if ((int)threadIdx.x < p.n) p.to[threadIdx.x] = p.numbers[threadIdx.x];
 }
 
 // Reference: pages.py:653-660 (_slots_at) and :721-722 (_slot).
@@ -289,6 +302,20 @@ __global__ void __launch_bounds__(128) compact_blocks_kernel(const crit_b200_com
 }
 
 }  // namespace crit_b200
+
+extern "C" __attribute__((visibility("default"))) int crit_b200_put(int64_t* to, const int64_t* numbers, int64_t n, void* stream) {
+    if (n < 0 || (n && (!to || !numbers))) return CRIT_B200_EINVAL;
+    if (!crit_b200::aligned(to, 8)) return CRIT_B200_EALIGN;
+    for (int64_t i = 0; i < n; i += crit_b200::PUT_NUMBERS) {
+        crit_b200::PutNumbers p;
+        p.to = to + i;
+        p.n = (int)(n - i < crit_b200::PUT_NUMBERS ? n - i : crit_b200::PUT_NUMBERS);
+        memcpy(p.numbers, numbers + i, p.n * sizeof(int64_t));
+        crit_b200::put_kernel<<<1, crit_b200::PUT_NUMBERS, 0, (cudaStream_t)stream>>>(p);
+        CRIT_CHECK_LAUNCH();
+    }
+    return 0;
+}
 
 extern "C" __attribute__((visibility("default"))) int crit_b200_expand(const crit_b200_expand_params* params, void* stream) {
     if (!params) return CRIT_B200_EINVAL;

@@ -122,6 +122,9 @@ typedef struct crit_b200_expand_params {
     int32_t sequences, width, tokens, kv_heads, dim, page, out_dtype;
 } crit_b200_expand_params;
 
+/* n numbers of host memory (read at the call) to `to` on the device, in stream order: as launch parameters, 256 a launch, so that
+ * a capture keeps them.  What a step's few positions and starts take. */
+int crit_b200_put(int64_t* to, const int64_t* numbers, int64_t n, void* stream);
 int crit_b200_expand(const crit_b200_expand_params* params, void* stream);
 
 /* -- norm and rotation of queries and keys, with the append ------------------------------------------------------------

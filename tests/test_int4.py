@@ -139,3 +139,11 @@ def test_bad_blocks_of_expand_and_norm_rope_are_refused_before_any_launch(lib):
         setattr(a, field, before)
     n.tokens = 0
     assert lib.crit_b200_norm_rope(ctypes.byref(n), None, None) == 0                   # no tokens: no launch
+
+
+def test_numbers_for_the_device_are_checked(lib):
+    numbers = (ctypes.c_int64 * 2)(1, 2)
+    assert lib.crit_b200_put(None, None, 0, None) == 0
+    for to, n, code in ((None, 2, -1), (4096, -1, -1), (4100, 2, -4)):
+        assert lib.crit_b200_put(to, numbers, n, None) == code
+    assert lib.crit_b200_put(4096, None, 2, None) == -1

@@ -670,18 +670,24 @@ def test_pages_as_any_view_of_their_storage():
     assert pk.status() == 0
 
 
-def test_lists_are_refused_under_capture_and_short_tables_always():
+def test_lists_are_kept_by_a_capture_and_short_tables_refused():
     cache = Cache4.filled(8, 128, 16, [64, 64], seed=261)
     q = _queries(10, 8, 128, torch.bfloat16, 262)
     args, kw = (q, cache.k, cache.v, "int4", cache.tables), dict(key_scales=cache.ks, value_scales=cache.vs)
-    want, places = pk.prefill(*args, [3, 40], 16, starts=[0, 4, 10], **kw), torch.tensor([3, 40], device="cuda")
-    graph = torch.cuda.CUDAGraph()
+    want = pk.prefill(*args, [3, 40], 16, starts=[0, 4, 10], **kw)
+    out, graph, firsts = torch.empty_like(q), torch.cuda.CUDAGraph(), [3, 40]
     with torch.cuda.graph(graph):
-        with pytest.raises(RuntimeError, match="under capture"):
-            pk.prefill(*args, [3, 40], 16, **kw)
-        with pytest.raises(RuntimeError, match="under capture"):
-            pk.prefill(*args, places, 16, starts=[0, 4, 10], **kw)
-    assert torch.equal(pk.prefill(*args, [3, 40], 16, starts=[0, 4, 10], **kw), want)
+        pk.prefill(*args, firsts, 16, starts=[0, 4, 10], out=out, **kw)
+    firsts[0] = 9
+    other = [torch.full((64,), -1, device="cuda") for _ in range(8)]       # (memory that a freed list would have been given to)
+    for _ in range(2):
+        out.fill_(float("nan"))
+        graph.replay()
+        assert torch.equal(out, want)
+    del other
+    assert torch.equal(pk.prefill(*args, torch.tensor([3, 40], device="cuda"), 16, starts=[0, 4, 10], **kw), want)
+    assert torch.equal(pk.prefill(q[:8], *args[1:], [3, 40], 16, **kw),                # equal counts: no starts
+                       pk.prefill(q[:8], *args[1:], [3, 40], 16, starts=[0, 4, 8], **kw))
     with pytest.raises(ValueError, match="page table"):
         pk.prefill(*args, [3, 1 << 30], 16, starts=[0, 4, 10], **kw)
     with pytest.raises(ValueError, match="page table"):
