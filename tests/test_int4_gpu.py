@@ -697,3 +697,28 @@ def test_lists_are_kept_by_a_capture_and_short_tables_refused():
     with pytest.raises(ValueError, match="int64 slots"):
         pk.gather(cache.k, "int4", 16, slots=torch.zeros(4, dtype=torch.int32, device="cuda"), scales=cache.ks)
     assert pk.status() == 0
+
+
+@pytest.mark.parametrize("columns,chunk", [(1, 64), (6, 128), (3, 1024)])
+def test_states_that_stay_in_the_workspace_fold_to_the_same_bits(columns, chunk, monkeypatch):
+    """The flag a sharded context's launches carry: every row's states kept, a row of one split too, and folded by the merge."""
+    import ctypes
+    from crit_b200 import _lib
+    cache = Cache4.filled(8, 128, 16, [700 + columns, 40 + columns], seed=271)
+    q, space = _queries(2 * columns, 32, 128, torch.bfloat16, 272), torch.full((1 << 21,), float("nan"), device="cuda")
+    blocks, run = [], pk._run
+    monkeypatch.setattr(pk, "_run", lambda name, what, device, *params: (blocks.extend(params), run(name, what, device, *params)))
+    want, want_lse = _attend(cache, q, [0, 1], [0, columns], [700, 40], columns, chunk=chunk, engine="mma.sync", workspace=space)
+    out, lse, p = torch.full_like(q, float("nan")), torch.full((2 * columns, 32), float("nan"), device="cuda"), blocks[-1]
+    tensors = [torch.tensor(x, dtype=t, device="cuda") for x, t in (([0, 1], torch.int32), ([0, columns], torch.int32), ([700, 40], torch.int64))]
+    p.rows, p.starts, p.firsts, p.counts = [x.data_ptr() for x in tensors] + [0]
+    p.out, p.lse, p.workspace, p.workspace_floats, p.flags = out.data_ptr(), lse.data_ptr(), space.data_ptr(), space.numel(), p.flags | 32
+    stream, lib = torch.cuda.current_stream().cuda_stream, _lib.load()
+    assert lib.crit_b200_decode(ctypes.byref(p), stream) == 0
+    assert out.isnan().all() and lse.isnan().all()
+    assert lib.crit_b200_merge(ctypes.byref(p), stream) == 0
+    if chunk < 700:
+        assert torch.equal(out[:columns], want[:columns])                  # a row of several splits: the same states, the same fold
+    # (a row of one split is divided by its sum in the fold instead: two FP32 roundings apart, one step of bf16 at most)
+    assert ((out.float() - want.float()).abs() <= 2.0 ** -7 * want.float().abs()).all()
+    assert (lse - want_lse).abs().max() <= 1e-5 and pk.status() == 0
