@@ -305,7 +305,32 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32, 4) norm_rope_kernel(const cri
     }
 
     // -- the values' rows go to their pages as they are ----------------------------------------------------------------------
-    if (WRITE && v0 < v1 && slot >= 0) {
+    if (WRITE && v0 < v1 && slot >= 0 && a.kind == CRIT_B200_KIND_INT4) {       // 16 elements a lane, as crit_b200_append takes them
+        const int vpart = lane % (LANES / 2), vsub = lane / (LANES / 2);
+        const bool held = vpart * 16 < a.value_dim;
+        const T* v_row = (const T*)a.values + t * a.value_stride_token + (int64_t)(v0 + vsub) * a.value_stride_head + vpart * 16;
+        for (int h = v0; h < v1; h += 2 * ROWS) {
+            float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            const bool live = held && h + vsub < v1;
+            if (live) {
+                Raw4<T> v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i].load(v_row + 4 * i);
+                v[0].floats(reinterpret_cast<float(&)[4]>(y[0])), v[1].floats(reinterpret_cast<float(&)[4]>(y[4]));
+                v[2].floats(reinterpret_cast<float(&)[4]>(z[0])), v[3].floats(reinterpret_cast<float(&)[4]>(z[4]));
+            }
+            v_row += 2 * ROWS * a.value_stride_head;
+            int bits = max(int4_top(y), int4_top(z));
+            bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
+            const uint32_t byte = int4_scale_byte(__int_as_float(bits), bits > 0x7f800000);
+            const float s = int4_scale(byte);
+            const uint2 w = make_uint2(int4_codes(y, s, byte), int4_codes(z, s, byte));
+            if (!live) continue;
+            const int64_t row = slot * a.kv_heads + h + vsub;
+            reinterpret_cast<uint2*>(a.value_pages)[row * (a.value_dim >> 4) + vpart] = w;
+            if ((vpart & 1) == 0) reinterpret_cast<uint8_t*>(a.value_scales)[row * (a.value_dim >> 5) + (vpart >> 1)] = (uint8_t)byte;
+        }
+    } else if (WRITE && v0 < v1 && slot >= 0) {
         const bool held = part * 8 < a.value_dim;
         const T* v_row = (const T*)a.values + t * a.value_stride_token + (int64_t)(v0 + sub) * a.value_stride_head + part * 8;
         for (int h = v0; h < v1; h += ROWS) {
