@@ -16,8 +16,9 @@
 // crit_b200_append encodes rows (16-bit pages, E4M3, INT8 and 4-bit codes).
 // All sums are FP32; a result is rounded once.  Every element is read and written once.
 // Measured: 8,192 tokens of 32 + 8 heads of 128, bf16: 35.9 us, 168 MB at 4.7 TB/s (floor 25.6 us); keys and values to 4-bit pages
-// in the same pass: 50 us for 177 MB (floor 27), 70% of the issue slots full, so the codes' instructions bound it; a step of 64 tokens
-// of 64 + 8 heads: 4.1 us, with the append 4.8, the launch and one row's latency.
+// in the same pass: 46.6 us for 177 MB (floor 27), bound by the codes' instructions (70% of the issue slots full; the values at 8
+// elements a lane 50 us, the keys at 16 by way of two turns' rows in shared memory no faster); a step of 64 tokens of 64 + 8 heads:
+// 4.1 us, with the append 4.8, the launch and one row's latency.
 #include <type_traits>
 
 #include "int4.cuh"
@@ -26,8 +27,8 @@ namespace crit_b200 {
 
 constexpr int ROPE_WARPS = 8;
 // Warps an SM that a launch of few tokens is to have: a token's heads are dealt to more warps until then, each of which makes the
-// token's sines again.  8,192 tokens with the append and two reads back: 65 us with 32 (and 16), 75 with 64; 64 tokens: 8.6 us with 32,
-// 9.3 with 16.
+// token's sines again.  8,192 tokens with the append and two reads back: 65 us with 32 (and 16), 75 with 64; 64 tokens: 8.6 us
+// with 32, 9.3 with 16.
 constexpr int ROPE_FILL = 32;
 
 template <typename T>
