@@ -223,9 +223,9 @@ __device__ __forceinline__ void load8(const TIN* src, float (&x)[8]) {
 // token, or a few tokens of fewer groups (grid: tokens, parts of a token), so that no index needs a 64-bit division.  Every byte
 // is read and written once.
 // Measured: 8,192 tokens of 8 heads of 128, keys and values, to scattered slots: 13.5 us for 42.5 MB, 3.1 TB/s (floor 6.5 us); a
-// step of 64 tokens 2.2 us, the launch.  Bound by instructions: with 8 elements a lane what a lane does once (address, scale,
-// reciprocal) was 130 of its 174 instructions, 17.6 us.  Several tokens a thread with their loads in flight together were
-// slower (two 0.5 us, four 5 us): their registers cost the warps that hide the loads.
+// step of 64 tokens 2.2 us, the launch.  Bound by instructions: 295 a lane and 16 elements, 75% of the issue slots full; 8
+// elements a lane were 174 instructions, 17.6 us.  Several tokens a thread with their loads in flight together were slower
+// (of 8 elements each, two 0.5 us, four 5 us): their registers cost the warps that hide the loads.
 template <typename TIN>
 __global__ void __launch_bounds__(256) append4_kernel(const crit_b200_append_params p, const int key_groups, const int per_token, const int per_block,
                                                       const uint32_t magic_k, const uint32_t magic_v) {
