@@ -13,24 +13,31 @@
 // columns on the instruction's 16 rows, query rows on its 8 columns:
 //   S^T[16 positions][8 query rows] = K Q^T    one accumulator a group of 32: a group's scale is one number a position,
 //                                              so x = sum over groups of scale[position][group] * S_group, in FP32
-//   O^T[32 values][8 query rows] += V^T P^T    the values' scales multiply the probabilities (a group at a time), or the
-//                                              codes
+//   O^T[32 values][8 query rows] += V^T P^T    the values' scales multiply the codes
 // The codes never pass through a thread one by one: ldmatrix hands a thread the 8 codes of a position and group that its
 // fragments want (K), or, transposed, 4 codes each of two neighbouring positions (V).  The head dimension is consumed in the
 // order the nibbles come, the queries laid out to match.
 //
 // Codes as FP16 operands.  The nibbles 0 and 4 of a word under the mask 0x000f000f ARE two FP16 numbers, n * 2^-24 (subnormal;
 // the tensor cores take them as they are), the nibbles 1 and 5 under 0x00f000f0 are 16 n * 2^-24: one AND makes two operands,
-// where 1024 + n less 1032 takes an OR and an add more.  The factor 16 is undone in the queries (their odd elements are
-// divided by 16) and in the outputs' odd columns, 2^-24 in a constant.  The 8 that a code stands above its value comes off in
-// products of their own: the positions' scales with -8 * the sums of the groups' queries (a K of the groups' number, the sums
-// as two FP16 terms), and a constant matrix with P^T, which gathers -8 * the sum of the
-// group's weights.  Where the accumulators for that do not fit the registers (wide tiles of query rows, the outputs of
-// 256-wide heads), codes become n - 8 one add later.
+// where 1024 + n less 1032 takes an OR and an add more.  The keys are taken so: the factor 16 is undone in the queries (their
+// odd elements are divided by 16), 2^-24 in a constant, and the 8 that a code stands above its value comes off in a product of
+// its own, the positions' scales with -8 * the sums of the groups' queries (a K of the groups' number, the sums as two FP16
+// terms).  Where the accumulators for that do not fit the registers (wide tiles of query rows), codes become n - 8 one add
+// later.  The values become (n - 8) * s with s the scale over 128, exactly: 8 significant bits, from 2^-24 up to 3,840.  The
+// nibbles 1 and 5 in one FMA: under 0x5400 they are 64 + n, and (64 + n) * s - 72 * s has no rounding (72 * s: 8 bits too); the
+// nibbles 0 and 4 as n - 8, then times s.  (All of them by the FMA take more shifts, which wait for the integer pipe: 64 rows of
+// 4,096 88.3 us against 86.8; all of them as n - 8 first 88.1.)
 //
 // The queries become FP16 with an exponent of their own a row (the largest element between 2^13 and 2^14), so no bf16 query
-// overflows or vanishes.  Weights are 2^(x - ref) with a reference that moves only when a score passes it (by 14 in the
-// exponent where the scales are on the codes): every weight and product stays an FP16 number.  Sums are FP32.
+// overflows or vanishes; an element is rounded only where it is below 2^-24 of its row's largest.
+// Weights are rounded to FP16, 2^-12 of each at the most (a product takes both operands in one type, and the scaled codes are
+// exact in FP16 with 3 bits to spare; bf16 weights would be 8 times coarser), while their sum is of the FP32 ones.  They are
+// 2^(x - ref + 11) with a reference that moves when a score passes it by 4 in the exponent: high in FP16's range, so that a weight
+// keeps its 11 bits down to 2^-25 of its row's largest, and what is left out below that is 2^-36 of it at the most.  (A reference
+// that moves at 1 would reach 2^-28, but moves so often that verify windows take 160 us instead of 143.  Scales on the weights
+// would take fewer instructions, 64 rows of 4,096 81 us, but round the product again, and lose it where a dominant position
+// meets small values: no better than 2^-20 of the largest at scales of 2^-3.)  Sums are FP32.
 //
 // Two ways to cut a launch.  By splits: a 3-D grid of (split of `chunk` positions, heads and query tiles, row), states in the
 // workspace as every other decode kernel leaves them: a column's bits do not depend on the launch.  Even
@@ -39,7 +46,7 @@
 // names the pair), and merge4_kernel folds a row's consecutive slots.  No block idles while another has two splits to go.
 //
 // Measured (B200, CUDA events around graphs; HBM's floor at the measured copy bandwidth beside it): 64 rows of 4,096 positions,
-// 64 query heads on 8 of 128: 81 us (44), 3.5 TB/s; one row of 200,000, 24 on 4 of 256: 67 us (33); 32 verify windows of 6 columns, 40
+// 64 query heads on 8 of 128: 87 us (44), 3.3 TB/s; one row of 200,000, 24 on 4 of 256: 70 us (33); 32 verify windows of 6 columns, 40
 // on 8 of 128, FP16: 143 us (27); one row of 777: 11 us, two launches' latency.  Bound by instructions at the registers' occupancy:
 // of the 64 rows' launch about 340 a warp and tile (V 100, K 60, scales and softmax the rest) fill 60% of the issue slots with
 // 16 warps an SM, the integer pipe 56%, the tensor pipe a quarter; of the verify windows' 720 a tile with 8 warps an SM fill
@@ -91,19 +98,25 @@ __device__ __forceinline__ uint32_t codes_high(uint32_t w) {
     return *reinterpret_cast<uint32_t*>(&h);
 }
 template <bool RAW>
-__device__ __forceinline__ void four_operands(uint32_t lo, uint32_t hi, uint32_t (&a1)[4], uint32_t (&a2)[4], int i1, int i2) {
-    // words lo and hi -> operands 0 and i1 of the low nibbles, i2 and 3 of the high ones; a2 from the words' upper bytes
-    a1[0] = RAW ? raw_low(lo) : codes_low(lo), a1[i1] = RAW ? raw_low(hi) : codes_low(hi);
-    a1[i2] = RAW ? raw_high(lo) : codes_high(lo), a1[3] = RAW ? raw_high(hi) : codes_high(hi);
+__device__ __forceinline__ void key_operands(uint32_t lo, uint32_t hi, uint32_t (&a1)[4], uint32_t (&a2)[4]) {
+    // words lo and hi -> operands 0 and 1 of the low nibbles, 2 and 3 of the high ones; a2 from the words' upper bytes
+    a1[0] = RAW ? raw_low(lo) : codes_low(lo), a1[1] = RAW ? raw_low(hi) : codes_low(hi);
+    a1[2] = RAW ? raw_high(lo) : codes_high(lo), a1[3] = RAW ? raw_high(hi) : codes_high(hi);
     lo >>= 8, hi >>= 8;
-    a2[0] = RAW ? raw_low(lo) : codes_low(lo), a2[i1] = RAW ? raw_low(hi) : codes_low(hi);
-    a2[i2] = RAW ? raw_high(lo) : codes_high(lo), a2[3] = RAW ? raw_high(hi) : codes_high(hi);
+    a2[0] = RAW ? raw_low(lo) : codes_low(lo), a2[1] = RAW ? raw_low(hi) : codes_low(hi);
+    a2[2] = RAW ? raw_high(lo) : codes_high(lo), a2[3] = RAW ? raw_high(hi) : codes_high(hi);
 }
 
 __device__ __forceinline__ uint32_t hmul2_bits(uint32_t a, uint32_t b) {
     __half2 h = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
     return *reinterpret_cast<uint32_t*>(&h);
 }
+__device__ __forceinline__ uint32_t hfma2_bits(uint32_t a, uint32_t b, uint32_t c) {
+    __half2 h = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b), *reinterpret_cast<__half2*>(&c));
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+// The nibbles 1 and 5 of a word as (n - 8) * scale / 128, `scale` a pair over 128 and `less` -72 times that.
+__device__ __forceinline__ uint32_t scaled_codes(uint32_t w, uint32_t scale, uint32_t less) { return hfma2_bits((w & 0x00f000f0u) | 0x54005400u, scale, less); }
 // D = A * B, and D += A * B (FP16 operands, FP32 sums; not volatile: nothing but the registers is touched, and the compiler
 // may place them between the loads and the conversions).
 __device__ __forceinline__ void mma16816_new(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -182,9 +195,8 @@ struct Place4 {
 };
 
 // MASKS: draft trees, sliding windows and block lists (else a column sees every position up to its own).
-// FAST: the fewest instructions for the tile's width (raw codes, scales on the weights where NT is 1).  Otherwise every width
-// does the same arithmetic, n - 8 and the scales on the codes, so that a launch cut into splits gives a column the same bits
-// alone and in any window, and a weight is rounded once, which FP16 outputs' 11 bits ask for.
+// FAST: the fewest instructions for the tile's width (the keys' raw codes).  Otherwise every width does the same arithmetic, so
+// that a launch cut into splits gives a column the same bits alone and in any window.
 template <int D, int NT, bool MASKS, bool FAST>
 __global__ void __launch_bounds__(32 * D4_HEADS, decode4_blocks(D, NT))
 decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
@@ -192,12 +204,9 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
     constexpr int ROWS = 8 * NT;
     constexpr int TPI = FAST && NT == 4 ? 1 : 2;        // tiles an iteration takes (the widest has products enough of its own)
     constexpr bool RAW_K = FAST && NT <= 2;                 // the 8 of the keys' codes through the accumulators' start
-    constexpr bool RAW_V = FAST && NT == 1 && D <= 128;     // that of the values' through a product of its own
-    constexpr bool SCALE_CODES = !FAST || NT > 1;           // the values' scales on the codes (an exact product), not on the weights:
-                                                            // fewer products where a tile holds several columns of query rows
-    // A row's reference is set AHEAD above its maximum and moves when a score passes it by more than SLACK: weights on their
-    // way to a scale of up to 61,440 stay at 1 or below, weights beside scaled codes may grow to 2^14 first.
-    constexpr float AHEAD = SCALE_CODES ? 0.f : 2.f, SLACK = SCALE_CODES ? 14.f : 0.f;
+    // A row's m_run is set TOP below its maximum, so that the largest weight is 2^TOP, and moves when a weight passes 2^SLACK
+    // (FAST: with it every row of the tile whose weights passed 2^TOP, so that fewer iterations stop for it).
+    constexpr float TOP = 11.f, SLACK = 15.f;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     __shared__ __align__(8) uint64_t bars_mem[2 * D4_MAX_STAGES];
@@ -341,10 +350,6 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
         turn_over();
     }
 
-    // -8 (rows of the low nibbles) and -8 * 16 (of the high ones), in the raw codes' units; made so that they stay in registers
-    uint32_t eight[4];
-    asm volatile("mov.b32 %0, 0x80088008;\n\tmov.b32 %1, 0x80808080;\n\tmov.b32 %2, 0x80088008;\n\tmov.b32 %3, 0x80808080;"
-                 : "=r"(eight[0]), "=r"(eight[1]), "=r"(eight[2]), "=r"(eight[3]));
     bool dead = false;
     int n = 0, stage = 0;           // tiles taken, the ring's place
     uint32_t phase = 0;
@@ -448,11 +453,7 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
             }
         }
 
-        float acc[NG][2][NT][4], acc8[RAW_V ? NG : 1][4], m_run[NT][2], l_run[NT][2];
-#pragma unroll
-        for (int k = 0; k < (RAW_V ? NG : 1); ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc8[k][i] = 0.f;
+        float acc[NG][2][NT][4], m_run[NT][2], l_run[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -516,7 +517,7 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
                     for (int o = 0; o < 2; ++o) {
                         const float2 s = __half22float2(*reinterpret_cast<__half2*>(&pair[k + o]));
                         uint32_t a1[4], a2[4];
-                        four_operands<RAW_K>(w[2 * o], w[2 * o + 1], a1, a2, 1, 2);
+                        key_operands<RAW_K>(w[2 * o], w[2 * o + 1], a1, a2);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             float c[4];
@@ -566,8 +567,8 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
                 top[nt][0] = mx[0] * mul[nt][0], top[nt][1] = mx[1] * mul[nt][1];
                 passed |= top[nt][0] > m_run[nt][0] + SLACK || top[nt][1] > m_run[nt][1] + SLACK;
             }
-            // The reference of a row moves only when a score of it passes it; the lanes' maxima are compared across the warp, and
-            // the sums brought to the new reference, only then.
+            // The reference of a row moves only when a score passes it; the lanes' maxima are compared across the warp, and the
+            // sums brought to the new reference, only then.
             if (__any_sync(0xffffffffu, passed)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -578,21 +579,15 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
                         high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 4));
                         high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 8));
                         high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 16));
-                        const bool moved = high > m_run[nt][j] + SLACK;
-                        alpha[j] = moved ? ex2(m_run[nt][j] - (high + AHEAD)) : 1.f;
-                        m_run[nt][j] = moved ? high + AHEAD : m_run[nt][j];
+                        const bool moved = high > m_run[nt][j] + (FAST ? TOP : SLACK);
+                        alpha[j] = moved ? ex2(m_run[nt][j] - (high - TOP)) : 1.f;
+                        m_run[nt][j] = moved ? high - TOP : m_run[nt][j];
                         l_run[nt][j] *= alpha[j];
                     }
 #pragma unroll
                     for (int k = 0; k < NG; ++k)
 #pragma unroll
                         for (int c = 0; c < 8; ++c) acc[k][c >> 2][nt][c & 3] *= alpha[c & 1];
-                    if constexpr (RAW_V) {
-#pragma unroll
-                        for (int k = 0; k < NG; ++k)
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) acc8[k][c] *= alpha[c & 1];
-                    }
                 }
             }
             uint32_t pb[TPI][NT][2];
@@ -621,7 +616,7 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
                 uint32_t pair[2][NG];                    // scales of positions 2 t, 2 t + 1 and of 2 t + 8, 2 t + 9
                 scale_pairs<NG>(lane_vscales + from, lane_vscales + from + row_scales, pair[0]);
                 scale_pairs<NG>(lane_vscales + from + 8 * row_scales, lane_vscales + from + 9 * row_scales, pair[1]);
-                if constexpr (SCALE_CODES && GENERAL) {
+                if constexpr (GENERAL) {
                     // A position that a query row does not take may have any scale, a NaN too: the scale becomes 0, and the
                     // weights of the rows that do take the position a NaN.
 #pragma unroll
@@ -643,26 +638,16 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
 #pragma unroll
                     for (int o = 0; o < 2; ++o) {
                         // words of positions 0-7 and 8-15: values 4 g .. 4 g + 3 of the group
-                        uint32_t a1[4], a2[4];
-                        four_operands<RAW_V>(w[2 * o], w[2 * o + 1], a1, a2, 2, 1);
-                        if constexpr (SCALE_CODES) {
-                            // the scale over 8 (exact), so that the product stays in FP16's range; the state takes the 8 back
-                            const uint32_t s0 = hmul2_bits(pair[0][k + o], 0x30003000u), s1 = hmul2_bits(pair[1][k + o], 0x30003000u);
-                            a1[0] = hmul2_bits(a1[0], s0), a1[1] = hmul2_bits(a1[1], s0), a1[2] = hmul2_bits(a1[2], s1), a1[3] = hmul2_bits(a1[3], s1);
-                            a2[0] = hmul2_bits(a2[0], s0), a2[1] = hmul2_bits(a2[1], s0), a2[2] = hmul2_bits(a2[2], s1), a2[3] = hmul2_bits(a2[3], s1);
-                        }
+                        const uint32_t s0 = hmul2_bits(pair[0][k + o], 0x20002000u), s1 = hmul2_bits(pair[1][k + o], 0x20002000u);        // / 128
+                        const uint32_t c0 = hmul2_bits(pair[0][k + o], 0xb880b880u), c1 = hmul2_bits(pair[1][k + o], 0xb880b880u);        // * -72 / 128
+                        const uint32_t lo = w[2 * o], hi = w[2 * o + 1];
+                        const uint32_t lo8 = lo >> 8, hi8 = hi >> 8;
+                        const uint32_t a1[4] = {hmul2_bits(codes_low(lo), s0), scaled_codes(lo, s0, c0), hmul2_bits(codes_low(hi), s1), scaled_codes(hi, s1, c1)};
+                        const uint32_t a2[4] = {hmul2_bits(codes_low(lo8), s0), scaled_codes(lo8, s0, c0), hmul2_bits(codes_low(hi8), s1), scaled_codes(hi8, s1, c1)};
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            uint32_t b0 = pb[v][nt][0], b1 = pb[v][nt][1];
-                            if constexpr (!SCALE_CODES) {
-                                b0 = hmul2_bits(b0, pair[0][k + o]), b1 = hmul2_bits(b1, pair[1][k + o]);
-                                if constexpr (GENERAL) b0 &= nonzero2(pb[v][nt][0]), b1 &= nonzero2(pb[v][nt][1]);
-                            }
-                            mma16816_add(acc[k + o][0][nt], a1, b0, b1);
-                            mma16816_add(acc[k + o][1][nt], a2, b0, b1);
-                            if constexpr (RAW_V) {
-                                mma16816_add(acc8[k + o], eight, b0, b1);
-                            }
+                            mma16816_add(acc[k + o][0][nt], a1, pb[v][nt][0], pb[v][nt][1]);
+                            mma16816_add(acc[k + o][1][nt], a2, pb[v][nt][0], pb[v][nt][1]);
                         }
                     }
                 }
@@ -711,9 +696,7 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
                 const int token = start + col, head = h * G + gq;
                 const float inv = whole ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;          // (a NaN stays one)
                 auto value = [&](int k, int e) {                 // element 32 k + 4 g + e
-                    float o = acc[k][e >> 1][nt][(e & 1) * 2 + j];
-                    if constexpr (RAW_V) return (o + acc8[k][(e & 1) * 2 + j]) * ((e & 1 ? 0x1p20f : 0x1p24f) * inv);
-                    else return o * (SCALE_CODES ? 8.f * inv : inv);
+                    return acc[k][e >> 1][nt][(e & 1) * 2 + j] * (128.f * inv);
                 };
                 if (whole) {
                     char* dst = (char*)p.out + ((int64_t)token * p.out_stride_token + (int64_t)head * p.out_stride_head + 4 * g) * 2;
