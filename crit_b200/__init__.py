@@ -208,6 +208,7 @@ def tcgen05p_serves(kind, head_dim, value_dim, heads, kv_heads, columns, chunk, 
 # whole-page-rows kernel deals whole splits to its blocks, and a small launch has too few to fill the device.
 PAGE_ROWS_FROM = 1 << 16
 EVEN_ROWS = 256             # window rows an even launch takes (decode4.cu, D4_MAX_ROWS)
+_LISTED_ROWS = {"even": EVEN_ROWS, "tcgen05": 256, "tcgen05p": 256, "tcgen05t": 128}      # window rows the kernels take that list them
 
 
 def engine_for(kind, head_dim, value_dim, heads, kv_heads, columns, rows=1, positions=None, engine=None):
@@ -710,6 +711,8 @@ def attend(q, key_pages, value_pages, kind, tables, rows, starts, firsts, column
             # (built on the device), so the launch reads those blocks and nothing else, on whichever kernel serves it
             out = torch.empty(T, hq, dv, dtype=q.dtype, device=q.device) if out is None else out
             listed = _listed_rows(tables, rows, starts, counts, firsts, blocks, int(block_size), page, int(columns), out, lse)
+            if engine in _LISTED_ROWS and listed[2].numel() > _LISTED_ROWS[engine]:
+                engine = "mma.sync"           # (named for the caller's rows; the tokens are more than it lists)
             return attend(q, key_pages, value_pages, kind, listed[0], listed[1], listed[2], listed[3], 1, page,
                           counts=listed[4], key_scales=key_scales, value_scales=value_scales, multipliers=multipliers,
                           scale=scale, partitions=partitions, out=out, lse=lse, workspace=workspace, chunk=chunk,

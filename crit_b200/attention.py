@@ -169,7 +169,8 @@ class DeviceAttention:
         named = kernels.engine_for(*geometry, len(meta), positions, None if self.window_engine == "auto" else self.window_engine)
         sinks, sliding = getattr(self, "_sinks", None), getattr(self, "_sliding", 0)
         listed = getattr(self, "_blocks", None)
-        sparse = listed is not None and listed[1] % pool.page == 0           # the lists as page tables of their own: any kernel
+        # the lists as page tables of their own, on any kernel (rows with packed partials read them as a mask)
+        sparse = listed is not None and listed[1] % pool.page == 0 and meta.offsets is None
         if (parents is not None or sinks is not None or sliding or (listed is not None and not sparse)) and named != "even":
             named = "mma.sync"             # draft trees, sinks, sliding windows and lists as masks are the m16n8k16 kernels'
         if named == "even" and (self.partial_bytes or self.partitions or self.chunk or len(meta) > kernels.EVEN_ROWS):

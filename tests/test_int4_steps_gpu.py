@@ -1,0 +1,95 @@
+"""Steps over "int4" pages at the borders of what the plugin's objects and the entry points let through."""
+from types import SimpleNamespace
+
+import numpy as np
+import pytest
+import torch
+
+import crit_b200 as pk
+from crit_b200.attention import DeviceAttention
+from crit_b200.batch import StepBatch
+from crit_b200.pool import KVPool
+from int4_oracle import Cache4, attention4, bounds4
+
+pytestmark = pytest.mark.gpu
+
+
+def _filled_pool(kind, rows, length, columns, hkv, dim, seed, **kw):
+    """A pool of `rows` sequences of `length` positions, and the step that adds `columns` more to each: (pool, batch)."""
+    pool = KVPool([0], hkv, dim, rows * (length + columns + 16), "cuda", kind, sequences=rows, **kw)
+    g = torch.Generator().manual_seed(seed)
+    for first, count in ((0, length), (length, columns)):
+        if first == 0:
+            for r in range(rows):
+                pool.open(r)
+        batch = StepBatch.build([(r, first, count) for r in range(rows)], "cuda")
+        slots = pool.reserve(batch)
+        make = lambda: torch.randn(batch.tokens, hkv, dim, generator=g).bfloat16().cuda()
+        pool.write(0, slots, make(), make())
+    return pool, batch
+
+
+def _as_cache(pool):
+    cache = Cache4.__new__(Cache4)
+    cache.heads, cache.dim, cache.page = pool.kv_heads, pool.head_dim, pool.page
+    cache.k, cache.v, cache.ks, cache.vs = pool.layer_pages(0)
+    pool._flush()
+    cache.tables = torch.stack([pool.block_tables[pool.row_of[r]] for r in pool.tables])
+    return cache
+
+
+def _round(rows, columns, length):
+    """The same step as a captured round has it: sequences in round slots, a width for all."""
+    return SimpleNamespace(round=True, prompt=False, rows=rows, width=columns - 1, tokens=rows * columns, slots_t=torch.arange(rows, device="cuda"),
+                           starts_t=torch.arange(rows, dtype=torch.int32, device="cuda") * columns,
+                           frontier_t=torch.full((rows,), length, device="cuda"))
+
+
+def _lists(rows, columns, length, block, seed):
+    """Lists of four blocks a token: its own, two of its context's, and none."""
+    g = torch.Generator().manual_seed(seed)
+    own = (length + torch.arange(columns)) // block
+    picks = torch.randint(0, length // block, (rows * columns, 2), generator=g)
+    return torch.cat([own.repeat(rows)[:, None], picks, torch.full((rows * columns, 1), -1)], 1).to(torch.int32).cuda()
+
+
+@pytest.mark.parametrize("rows,columns", [(64, 6), (43, 6), (257, 1)])
+def test_lists_of_whole_pages_over_more_tokens_than_an_even_launch_has_rows(rows, columns):
+    length = 70
+    pool, batch = _filled_pool("int4", rows, length, columns, 2, 64, 1, round_rows=256)
+    q = torch.randn(rows * columns, 4, 64, generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+    blocks = _lists(rows, columns, length, 32, 3)
+    cache = _as_cache(pool)
+    found = [DeviceAttention().forward(0, q, pool, batch, blocks=blocks, block_size=32, lse=True)]         # (as a mask)
+    if rows <= 256:
+        for r in range(rows):
+            pool.bind(r, r, length + columns)
+        found.append(DeviceAttention().forward(0, q, pool, _round(rows, columns, length), blocks=blocks, block_size=32, lse=True))
+    for r in (0, rows // 2, rows - 1):
+        for c in range(columns):
+            t = r * columns + c
+            want, want_lse, room = attention4(cache, q[t], r, length, c, columns, t, blocks=blocks, block_size=32)
+            for out, lse in found:
+                assert (np.abs(out[t].double().cpu().numpy() - want) <= bounds4(want, room, length + columns, q.dtype)).all()
+                assert (np.abs(lse[t].double().cpu().numpy() - want_lse) <= 3e-4).all()
+    args = (q, *pool.layer_pages(0)[:2], "int4", pool.block_tables, torch.arange(rows, dtype=torch.int32, device="cuda"),
+            torch.arange(rows, dtype=torch.int32, device="cuda") * columns, torch.full((rows,), length, device="cuda"), columns, pool.page)
+    kw = dict(key_scales=cache.ks, value_scales=cache.vs, blocks=blocks, block_size=32)
+    named = pk.attend(*args, engine="even" if rows <= 256 else "mma.sync", **kw)                # named for the caller's rows
+    chosen = pk.attend(*args, **kw)
+    assert torch.equal(named, chosen) and pk.status() == 0
+
+
+def test_lists_over_many_tokens_of_fp8_pages_read_by_whole_rows():
+    """The same rule for the other kernels that list their rows."""
+    rows, columns, length = 64, 6, 70
+    pool, batch = _filled_pool("fp8:page", rows, length, columns, 8, 128, 4, round_rows=rows)
+    for r in range(rows):
+        pool.bind(r, r, length + columns)
+    q = torch.randn(rows * columns, 8, 128, generator=torch.Generator().manual_seed(5)).bfloat16().cuda()
+    assert pk.engine_for("fp8:page", 128, 128, 8, 8, columns, rows, pool.block_tables.shape[1] * pool.page) == "tcgen05p"
+    blocks = _lists(rows, columns, length, 32, 6)
+    for step in (_round(rows, columns, length), batch):
+        out, lse = DeviceAttention().forward(0, q, pool, step, blocks=blocks, block_size=32, lse=True)
+        want, want_lse = DeviceAttention(window_engine="mma.sync").forward(0, q, pool, step, blocks=blocks, block_size=32, lse=True)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse) and pk.status() == 0
