@@ -776,7 +776,8 @@ def attend(q, key_pages, value_pages, kind, tables, rows, starts, firsts, column
                    out_token, out_head, tables.stride(0), R, columns, partial_rows, hq, hkv, d, dv, page, k_kind,
                    _page_dtype(kind, key_pages), _DTYPES[q_dtype], chunk, splits, flags, float(scale if scale is not None else d ** -0.5),
                    float(multipliers[0]), float(multipliers[1]), _ptr(parents), _ptr(sinks), sliding,
-                   blocks.shape[1] if blocks is not None else 0, int(block_size) if blocks is not None else 0, _ptr(blocks))
+                   blocks.shape[1] if blocks is not None else 0, int(block_size) if blocks is not None else 0, tables.shape[1] if k_kind == 5 else 0,
+                   _ptr(blocks))
     lib = _lib.load()
     if engine == "even":
         key = (place, R, columns, hq, hkv, d, q_dtype, parents is not None or sliding > 0 or blocks is not None)

@@ -6,7 +6,7 @@ from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int6
 from pathlib import Path
 
 LIBRARY = Path(__file__).resolve().parent / "_native" / "libcrit_b200.so"
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 KIND_16BIT, KIND_FP8, KIND_FP8_ROW, KIND_INT8, KIND_FP8_PAGE, KIND_INT4 = range(6)
 DTYPE_BF16, DTYPE_FP16, DTYPE_FP32 = range(3)
@@ -61,7 +61,7 @@ class AttendParams(Structure):
                 ("chunk", c_int32), ("max_splits", c_int32), ("flags", c_int32),
                 ("scale", c_float), ("key_multiplier", c_float), ("value_multiplier", c_float),
                 ("parents", c_void_p), ("sinks", c_void_p), ("sliding", c_int32),
-                ("blocks_k", c_int32), ("block_size", c_int32), ("blocks", c_void_p)]
+                ("blocks_k", c_int32), ("block_size", c_int32), ("table_pages", c_int32), ("blocks", c_void_p)]
 
 
 class MergeShardsParams(Structure):

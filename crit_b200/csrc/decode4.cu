@@ -176,12 +176,19 @@ __device__ __forceinline__ uint32_t chunk4(uint32_t row, uint32_t c, uint32_t by
     return row * bytes + ((c ^ turn) << 4);
 }
 
-// A row of the launch: its tiles.  -1 in an even launch whose plan is too small for the row (chunk * max_splits positions are
-// what a table row holds): the row is left out, its output as it was, and reported.  A launch cut into splits ends there by
-// its grid.
+// The positions that a row's page table holds.
+__device__ __forceinline__ int64_t table_positions4(const crit_b200_attend_params& p) {
+    return p.table_pages > 0 ? (int64_t)p.table_pages * p.page : (int64_t)p.chunk * p.max_splits;
+}
+// Whether a row begins past its page table: nothing it says can be right.  It is reported; an even launch leaves it out, its
+// output as it was, a launch cut into splits reads what the table holds.
+__device__ __forceinline__ bool past_table4(const crit_b200_attend_params& p, int r, int count) {
+    return count > 0 && p.firsts[r] >= table_positions4(p) + ((p.flags & CRIT_B200_ATTEND_CONTEXT) ? 1 : 0);
+}
+// A row of the launch: its tiles, as far as its page table goes (a row may end past it where a captured step is padded).
 __device__ __forceinline__ int row_tiles4(const crit_b200_attend_params& p, int r, int count) {
-    const int64_t L = p.firsts[r] + ((p.flags & CRIT_B200_ATTEND_CONTEXT) ? 0 : count);
-    if ((p.flags & CRIT_B200_ATTEND_EVEN) && L > (int64_t)p.chunk * p.max_splits) return -1;
+    const int64_t end = p.firsts[r] + ((p.flags & CRIT_B200_ATTEND_CONTEXT) ? 0 : count), holds = table_positions4(p), L = end < holds ? end : holds;
+    if ((p.flags & CRIT_B200_ATTEND_EVEN) && past_table4(p, r, count)) return 0;
     return count > 0 && L > 0 ? (int)((L + 15) >> 4) : 0;
 }
 __device__ __forceinline__ int row_count4(const crit_b200_attend_params& p, int r) {
@@ -233,8 +240,7 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
                 int tiles = 0, subs = 0;
                 if (r < p.n_rows) {
                     const int count = row_count4(p, r);
-                    tiles = row_tiles4(p, r, count);
-                    tiles = tiles < 0 ? 0 : tiles, subs = count > 0 ? HG * ((count * G + ROWS - 1) / ROWS) : 0;
+                    tiles = row_tiles4(p, r, count), subs = count > 0 ? HG * ((count * G + ROWS - 1) / ROWS) : 0;
                 }
                 int scan = tiles * subs;
 #pragma unroll
@@ -272,6 +278,7 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
         const int r = blockIdx.z, count = row_count4(p, r);
         const int hg = blockIdx.y / u.ctiles, ct = blockIdx.y - hg * u.ctiles;
         if (count <= 0 || ct * ROWS >= count * G) return;
+        if (blockIdx.x == 0 && threadIdx.x == 0 && p.status && past_table4(p, r, count)) atomicExch(p.status, CRIT_B200_STATUS_PLAN);
         at.r = r, at.tiles = row_tiles4(p, r, count), at.subs = 0x7fffffff;
         at.sub = blockIdx.y, at.tile = blockIdx.x * (p.chunk >> 4);
         length = at.tiles - at.tile < (p.chunk >> 4) ? at.tiles - at.tile : (p.chunk >> 4);
@@ -361,7 +368,7 @@ decode4_kernel(const crit_b200_attend_params p, const Decode4Launch u, const __g
     while (n < length) {
         // -- a unit: the tiles of one row, head group and query tile in this block -----------------------------------------
         const int r = at.r, count = row_count4(p, r);
-        const int64_t first = p.firsts[r];
+        const int64_t holds = table_positions4(p), first = p.firsts[r] < holds ? p.firsts[r] : holds;
         const int first32 = (int)first;
         const int per_hg = u.blocks ? at.subs / HG : u.ctiles;
         const int hg = at.sub / per_hg, ct = at.sub - hg * per_hg;
@@ -741,7 +748,7 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) merge4_kernel(c
     const int count = row_count4(p, r), start = p.starts[r];
     const int tiles = row_tiles4(p, r, count);
     if (col >= count) return;
-    if (tiles < 0) {
+    if (past_table4(p, r, count)) {
         if (lane == 0 && p.status) atomicExch(p.status, CRIT_B200_STATUS_PLAN);
         return;
     }
@@ -921,7 +928,8 @@ int64_t even_floats4(const crit_b200_attend_params& p) {
     if (p.kind != CRIT_B200_KIND_INT4 || p.head_dim != p.value_dim) return CRIT_B200_EUNSUPPORTED;
     if (int e = plan4(p, &plan)) return e;
     // (the launch's tiles are counted in 32 bits)
-    if (((int64_t)p.chunk * p.max_splits / 16 + 1) * p.n_rows > 0x7fffffffLL / ((int64_t)p.kv_heads / plan.u.heads * plan.u.ctiles)) return CRIT_B200_EUNSUPPORTED;
+    const int64_t holds = p.table_pages > 0 ? (int64_t)p.table_pages * p.page : (int64_t)p.chunk * p.max_splits;
+    if (holds > 0x7fffffffLL || (holds / 16 + 1) * p.n_rows > 0x7fffffffLL / ((int64_t)p.kv_heads / plan.u.heads * plan.u.ctiles)) return CRIT_B200_EUNSUPPORTED;
     const int64_t slots = (int64_t)plan.u.blocks + (int64_t)p.n_rows * (p.kv_heads / plan.u.heads) * plan.u.ctiles;
     return (p.n_rows + 2 + 31) / 32 * 32 + slots * plan.u.heads * 8 * plan.nt * (p.head_dim + 2);
 }
@@ -930,6 +938,9 @@ int launch_decode4(const crit_b200_attend_params& p, cudaStream_t s) {
     if (p.flags & (CRIT_B200_ATTEND_TCGEN05 | CRIT_B200_ATTEND_TCGEN05P | CRIT_B200_ATTEND_TCGEN05T)) return CRIT_B200_EUNSUPPORTED;
     if (p.head_dim != p.value_dim || p.slots < 16 || p.slots > 0x7fffffffLL || p.slots < p.page) return CRIT_B200_EUNSUPPORTED;
     if (!aligned(p.key_scales, 16) || !aligned(p.value_scales, 16)) return CRIT_B200_EALIGN;
+    // (positions are 32 bits in the kernel; splits wholly past the table would leave no state for the fold)
+    if (p.table_pages < 0 || (int64_t)p.table_pages * p.page > 0x7fffffffLL) return CRIT_B200_EUNSUPPORTED;
+    if (!(p.flags & CRIT_B200_ATTEND_EVEN) && p.table_pages > 0 && (int64_t)p.chunk * (p.max_splits - 1) >= (int64_t)p.table_pages * p.page) return CRIT_B200_EINVAL;
     Decode4Plan plan;
     if (int e = plan4(p, &plan)) return e;
     const Decode4Launch& u = plan.u;

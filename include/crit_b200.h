@@ -21,7 +21,7 @@
 extern "C" {
 #endif
 
-#define CRIT_B200_ABI_VERSION 4
+#define CRIT_B200_ABI_VERSION 5
 
 /* Page kinds (the reference's KINDS, paged_kv_attention/__init__.py:78, plus the per-page FP8 scale). */
 #define CRIT_B200_KIND_16BIT    0   /* bf16 or fp16 pages (page_dtype says which) */
@@ -242,8 +242,8 @@ int crit_b200_compact_blocks(const crit_b200_compact_params* params, void* strea
 #define CRIT_B200_ATTEND_EVEN 512    /* kind 5: the launch's tiles are dealt out in equal runs to the blocks the device holds at once
                                         (a column's bits then depend on the launch), at most 256 rows; a workspace of
                                         crit_b200_attend_floats floats in a layout of its own (partial_rows and offsets are not
-                                        read; chunk * max_splits is the positions a table row holds at most: a row of more is left
-                                        out and reported); both launches carry the flag */
+                                        read; chunk * max_splits is the positions a row has at most, table_pages the exact
+                                        number where given); both launches carry the flag */
 #define CRIT_B200_ATTEND_PARTIALS 32 /* every row's split states go to the workspace, a row of one split too (the first launch
                                         writes nothing to out / lse): what crit_b200_merge_push sends, or what
                                         crit_b200_merge folds */
@@ -295,6 +295,10 @@ typedef struct crit_b200_attend_params {
     int32_t sliding;             /* 0, or the positions a column sees up to its own (a sliding window): positions at or
                                     below its own minus `sliding` are masked (_kernels.py:332-333); m16n8k16 kernel only */
     int32_t blocks_k, block_size;/* with `blocks`: ids a token lists, positions a block holds */
+    int32_t table_pages;         /* kind 5: pages a row of `tables` holds, or 0: chunk * max_splits positions.  Nothing past them is
+                                    read: of a row that ends past them the columns there see the table's positions only (the
+                                    padding of a captured step); a row that begins past them is reported as
+                                    CRIT_B200_STATUS_PLAN, and left out by an even launch */
     const int32_t* blocks;       /* NULL, or [tokens of q][blocks_k] KV block ids, -1 for none: of what the other rules
                                     leave, a token sees only the positions of its listed blocks (block-sparse lists,
                                     _kernels.py:481-555; here as a mask: every position is still read); m16n8k16 kernel only */

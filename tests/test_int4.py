@@ -147,3 +147,19 @@ def test_numbers_for_the_device_are_checked(lib):
     for to, n, code in ((None, 2, -1), (4096, -1, -1), (4100, 2, -4)):
         assert lib.crit_b200_put(to, numbers, n, None) == code
     assert lib.crit_b200_put(4096, None, 2, None) == -1
+
+
+def test_splits_past_a_page_table_and_tables_past_32_bits_are_refused(lib):
+    from crit_b200 import _lib
+    p = _lib.AttendParams()
+    p.q = p.out = p.key_pages = p.value_pages = p.key_scales = p.value_scales = p.tables = p.rows = p.starts = p.firsts = p.workspace = 4096
+    p.n_rows = p.columns = p.partial_rows = 1
+    p.q_heads, p.kv_heads, p.head_dim, p.value_dim, p.page, p.kind, p.chunk, p.slots = 8, 8, 128, 128, 16, _lib.KIND_INT4, 64, 64
+    p.workspace_floats, p.table_pages = 1 << 20, 5
+    for splits in (3, 100):                                                      # the table's 80 positions are two splits of 64
+        p.max_splits = splits
+        assert lib.crit_b200_attend(ctypes.byref(p), None) == -1
+    p.max_splits, p.flags = 1, 512
+    for pages in (-1, 1 << 28):
+        p.table_pages = pages
+        assert lib.crit_b200_attend(ctypes.byref(p), None) == -2

@@ -9,6 +9,7 @@ import crit_b200 as pk
 from crit_b200.attention import DeviceAttention
 from crit_b200.batch import StepBatch
 from crit_b200.pool import KVPool
+from test_int4_gpu import _attend, _queries
 from int4_oracle import Cache4, attention4, bounds4
 
 pytestmark = pytest.mark.gpu
@@ -93,3 +94,49 @@ def test_lists_over_many_tokens_of_fp8_pages_read_by_whole_rows():
         out, lse = DeviceAttention().forward(0, q, pool, step, blocks=blocks, block_size=32, lse=True)
         want, want_lse = DeviceAttention(window_engine="mma.sync").forward(0, q, pool, step, blocks=blocks, block_size=32, lse=True)
         assert torch.equal(out, want) and torch.equal(lse, want_lse) and pk.status() == 0
+
+
+@pytest.mark.parametrize("engine", [None, "mma.sync", 64])
+@pytest.mark.parametrize("columns", [1, 4])
+def test_rows_that_end_or_begin_past_their_page_table(engine, columns):
+    """A table of 7 pages of 16 (no multiple of a split), the last row of its tensor, with ids behind it that are no pages: a row
+    that ends past it reads nothing there, its columns within it are as they should be; a row that begins past it is reported."""
+    page, width = 16, 7
+    holds = page * width
+    cache = Cache4.filled(8, 128, page, [holds, holds], seed=301)
+    behind = torch.full((3, width), 1 << 20, dtype=torch.int32, device="cuda")
+    behind[:2] = cache.tables
+    cache.tables = behind[:2]
+    q = _queries(2 * columns, 16, 128, torch.bfloat16, 302)
+    first = holds - (1 if columns == 1 else 2)
+    kw = {} if engine is None else {"engine": "mma.sync", "chunk": engine if isinstance(engine, int) else None}
+    out, lse = _attend(cache, q, [0, 1], [0, columns], [50, first], columns, **kw)               # (reports nothing)
+    _as_many = [columns, holds - first]
+    for r, (at, n) in enumerate(zip((50, first), _as_many)):
+        for c in range(n):
+            t = r * columns + c
+            want, want_lse, room = attention4(cache, q[t], r, at, c, n, t)
+            assert (np.abs(out[t].double().cpu().numpy() - want) <= bounds4(want, room, at + n, q.dtype)).all()
+            assert (np.abs(lse[t].double().cpu().numpy() - want_lse) <= 3e-4).all()
+    assert out.isfinite().all()
+    before = pk._status[str(q.device)].clone()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    for beyond in (holds, holds + 500, 1 << 40):
+        out = torch.full_like(q, float("nan"))
+        pk.attend(q, cache.k, cache.v, "int4", cache.tables, torch.arange(2, **i32), torch.arange(2, **i32) * columns, torch.tensor([50, beyond], device="cuda"), columns,
+                  page, key_scales=cache.ks, value_scales=cache.vs, out=out, **kw)
+        assert pk.status() == 2
+        pk._status[str(q.device)].copy_(before)
+        for c in range(columns):
+            want, _, room = attention4(cache, q[c], 0, 50, c, columns, c)
+            assert (np.abs(out[c].double().cpu().numpy() - want) <= bounds4(want, room, 50 + columns, q.dtype)).all()
+        assert engine is not None or out[columns:].isnan().all()
+    # context rows: one that sees the whole table, and one that says more
+    out, lse = _attend(cache, q[:columns], [1], [0], [holds], columns, context=True, **kw)
+    for c in range(columns):
+        want, _, room = attention4(cache, q[c], 1, holds, c, columns, c, context=True)
+        assert (np.abs(out[c].double().cpu().numpy() - want) <= bounds4(want, room, holds, q.dtype)).all()
+    pk.attend(q[:columns], cache.k, cache.v, "int4", cache.tables, torch.ones(1, **i32), torch.zeros(1, **i32), torch.tensor([holds + 1], device="cuda"), columns, page,
+              key_scales=cache.ks, value_scales=cache.vs, context=True, **kw)
+    assert pk.status() == 2
+    pk._status[str(q.device)].copy_(before)
