@@ -22,6 +22,7 @@ tolerance, integer and byte results (slots, codes, scales) bit for bit.
 """
 import contextlib
 import ctypes
+import itertools
 import struct
 import math
 import threading
@@ -837,9 +838,27 @@ def prefill_serves(head_dim, value_dim, q_dtype, kind, page):
 
 
 # -- prompt chunks ------------------------------------------------------------------------------------------------------
-def _expanded(positions_at, starts_at, q, key_pages, value_pages, key_scales, value_scales, table, position, tokens, longest, page, workspace):
-    """4-bit pages as 16-bit ones of q's type in the workspace, one launch, in the order of the sequences' tables: the
-    addresses of the keys, the values and the table that reads them, its width, and the slots of the pages."""
+def _expansion(device, size, given, steady):
+    """`size` bytes for a prompt launch's own use (16-byte aligned): `given`, or memory of the launch's stream that goes back to
+    torch's allocator when the call returns.  steady: calls of this size repeat; else a prompt grows chunk by chunk, and sizes of
+    powers of two are few, so that the allocator's blocks are found again."""
+    if given is not None:
+        if given.dtype != torch.float32 or 4 * given.numel() < size or not given.is_contiguous() or given.device != device:
+            raise ValueError(f"prefill's workspace holds {given.numel()} floats; this launch needs {-(-size // 4)} contiguous FP32 ones on q's device")
+        return given
+    if not steady and not torch.cuda.is_current_stream_capturing():
+        try:
+            return torch.empty(1 << (size - 1).bit_length(), dtype=torch.uint8, device=device)
+        except torch.OutOfMemoryError:
+            pass
+    return torch.empty(size, dtype=torch.uint8, device=device)
+
+
+def _expanded(positions_at, starts_at, bases_at, q, key_pages, value_pages, key_scales, value_scales, table, position, tokens, pages, width, page, workspace):
+    """4-bit pages as 16-bit ones of q's type in memory of the launch's own, one launch: (that memory, the addresses of the keys,
+    the values, the table that reads them and the positions, the slots of the pages).  pages: how many the sequences take
+    together, at the bases, where the host knows; None: positions on the device, room for every page the tables (of `width`) may
+    name, or for the pool's where those are fewer."""
     hkv, d = key_pages.shape[-2], q.shape[-1]
     place = q.get_device()
     if value_scales is None or _check4(key_pages, key_scales, "keys") != (hkv, d) or _check4(value_pages, value_scales, "values") != (hkv, d) or \
@@ -848,24 +867,34 @@ def _expanded(positions_at, starts_at, q, key_pages, value_pages, key_scales, va
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("q is bf16 or fp16")
     several = table.dim() == 2
-    sequences, width = table.shape if several else (1, table.shape[0])
-    if longest is not None:
-        if longest > width * page:
-            raise ValueError(f"a chunk's positions go up to {longest}; its page table holds {width * page}")
-        width = -(-longest // page)
-    pages = sequences * width
-    half = pages * page * hkv * d // 2                                 # floats of the keys, or the values
-    floats = 2 * half + pages
-    # (a workspace that a launch outgrew is kept: large ones grow by powers of two)
-    space = _workspace(q.device, floats if workspace is not None or floats < 1 << 24 else 1 << (floats - 1).bit_length(), workspace)
-    keys = space.data_ptr()
-    values, found = keys + 4 * half, keys + 8 * half
+    sequences, slots = table.shape[0] if several else 1, key_pages.numel() * 2 // (hkv * d)
+    steady = pages is None                                             # (the same room whatever the positions are)
+    keep_ids = steady and slots // page < sequences * width
+    if steady:
+        pages = slots // page if keep_ids else sequences * width
+    side = pages * page * hkv * d * 2                                  # bytes of the keys, or the values
+    held = _expansion(q.device, 2 * side + 8 * sequences + 4 * sequences * width + 16, workspace, steady)
+    keys = held.data_ptr()
+    values, found = keys + side, keys + 2 * side                       # then the positions, then the table
     on_device = positions_at if several else _ptr(position) if torch.is_tensor(position) else 0
     e = _lib.block(_lib.ExpandParams, key_pages.data_ptr(), value_pages.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), table.data_ptr(),
-                   on_device, starts_at, keys, values, found, _ptr(_status_word(q.device)), 0 if on_device else int(position),
-                   key_pages.numel() * 2 // (hkv * d), table.stride(0) if several else 0, sequences, width, tokens, hkv, d, page, _DTYPES[q.dtype])
+                   on_device, starts_at, bases_at, keys, values, found + 8 * sequences, found, _ptr(_status_word(q.device)), 0 if on_device else int(position),
+                   slots, table.stride(0) if several else 0, sequences, width, tokens, hkv, d, page, _DTYPES[q.dtype], keep_ids)
     _run("crit_b200_expand", "crit_b200.prefill", q.device, e)
-    return keys, values, found, width, pages * page
+    return held, keys, values, found + 8 * sequences, found if on_device else 0, pages * page
+
+
+def _pages_of(positions, ends, tokens, width, page):
+    """The pages of tables of `width` that the sequences of a prompt launch over 4-bit pages take, or None: positions on the
+    device.  What lies outside the tables is refused here."""
+    longest = tokens if positions is None else max(ends, default=0)
+    if longest > width * page:
+        raise ValueError(f"a chunk's positions go up to {longest}; its page table holds {width * page}")
+    if positions is None:
+        return None
+    if min(positions, default=0) < 0:
+        raise ValueError("positions are not negative")
+    return [-(-end // page) for end in ends]
 
 
 def _sent(positions, starts, device):
@@ -894,9 +923,10 @@ def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scale
     (tcgen05.mma tiles with TMEM accumulators for 16-bit pages of 128-wide heads, m16n8k16 tiles otherwise), "mma.sync"
     or "tcgen05" (refused where not served); "tcgen05:single" / "tcgen05:pair" also name the block shape (128 query rows
     two blocks an SM / 256 rows over one ring of key and value tiles, which "tcgen05" picks by the launch's size).
-    "int4" pages are first made 16-bit ones of q's type in the workspace (exact: no second rounding), positions * kv_heads *
-    dim floats a sequence and a few, the workspace of `owner` or `workspace` (FP32) when given: run a launch of that size
-    once before capturing it.
+    "int4" pages are first made 16-bit ones of q's type (exact: no second rounding) in memory of the launch's own: the sequences'
+    positions * kv_heads * dim * 4 bytes (with positions on the device those that the tables or the pool hold, whichever are
+    fewer) and a few, of the current stream and given back when the call returns (a capture keeps its own), or `workspace` (FP32,
+    read and written until the launch is through: not for two launches at once).
     Reference: paged_kv_attention/__init__.py:1245-1332."""
     _refuse(int8_qk=int8_qk, fresh=fresh, sinks=sinks, sliding=sliding, derive=derive)
     k_kind = _check_kind(kind, key_scales)
@@ -917,7 +947,7 @@ def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scale
     positions_at = starts_at = sequences = table_stride = 0
     if k_kind == 5 and torch.is_tensor(position) and position.get_device() != q.get_device():
         raise ValueError("positions read on the device are on q's device")
-    longest = None if torch.is_tensor(position) or table.dim() == 2 else int(position) + T       # positions, where the host knows them
+    bases_at, width = 0, table.shape[-1]
     if table.dim() == 2:             # several sequences, one launch
         S, ahead = table.shape[0], None
         if not torch.is_tensor(position):
@@ -937,28 +967,39 @@ def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scale
                 raise ValueError("starts: S + 1 rising row numbers from 0 to the number of tokens")
             counts = [b - a for a, b in zip(starts, starts[1:])]
             most = max(counts)
-        held = position                      # (kept until both launches are made)
-        if ahead is not None or starts is not None:
-            held, at = _sent(ahead, starts, q.device)
-            starts_at = at if starts is not None else 0
+        ends = None if ahead is None else [a + n for a, n in zip(ahead, counts)]
+        numbers, held = starts or [], position                   # (held: kept until both launches are made)
+        if k_kind == 5:
+            taken = _pages_of(ahead, ends, most, width, int(page))
+            numbers = numbers + [0, *itertools.accumulate(taken)][:S] if taken else numbers             # (the bases)
+        if ahead is not None or numbers:
+            held, at = _sent(ahead, numbers, q.device)
+            starts_at, bases_at = at if starts is not None else 0, at + 4 * len(starts or ()) if k_kind == 5 and ahead is not None else 0
         positions_at, sequences, table_stride = (position if ahead is None else held).data_ptr(), S, table.stride(0)
         T, position = most, 0
-        longest = max((a + n for a, n in zip(ahead, counts)), default=0) if ahead is not None else None
     elif starts is not None:
         raise ValueError("starts goes with a table of several sequences")
     if torch.is_tensor(position) and (position.dtype != torch.int64 or position.numel() != 1 or not position.is_cuda):
         raise ValueError("a position read on the device is a one-element int64 tensor there")
     page, q_code = int(page), _DTYPES[q.dtype]
     if k_kind == 5:
-        keys_at, values_at, table_at, width, slots = _expanded(positions_at, starts_at, q, key_pages, value_pages, key_scales, value_scales, table, position,
-                                                               T, longest, page, workspace)
+        if not sequences:
+            taken = _pages_of(*((None, None) if torch.is_tensor(position) else ([int(position)], [int(position) + T])), T, width, page)
+        width = max(taken, default=0) if taken is not None else width
+        own, keys_at, values_at, table_at, at, slots = _expanded(positions_at, starts_at, bases_at, q, key_pages, value_pages, key_scales, value_scales, table,
+                                                                 position, T, None if taken is None else sum(taken), width, page, workspace)
         key_scales = value_scales = None
         table_stride, k_kind, page_dtype = width if sequences else 0, 0, q_code
+        if sequences:
+            positions_at = at
     else:
         keys_at, values_at, table_at, slots = key_pages.data_ptr(), value_pages.data_ptr(), table.data_ptr(), key_pages.numel() // (hkv * d)
         page_dtype = _page_dtype(kind, key_pages)
     device = q.device
-    position_at, position = (position.data_ptr(), 0) if torch.is_tensor(position) else (0, int(position))
+    if torch.is_tensor(position):
+        position_at, position = at if kind == "int4" else position.data_ptr(), 0
+    else:
+        position_at, position = 0, int(position)
     q_token, q_head, _ = q.stride()
     out_token, out_head, _ = out.stride()
     p = _lib.block(_lib.PrefillParams, q.data_ptr(), out.data_ptr(), _ptr(lse), keys_at, values_at, _ptr(key_scales), _ptr(value_scales), table_at, position_at,

@@ -88,10 +88,10 @@ class ExchangeParams(Structure):
 
 class ExpandParams(Structure):
     _fields_ = [("key_pages", c_void_p), ("value_pages", c_void_p), ("key_scales", c_void_p), ("value_scales", c_void_p),
-                ("tables", c_void_p), ("positions", c_void_p), ("starts", c_void_p), ("out_keys", c_void_p), ("out_values", c_void_p),
-                ("out_tables", c_void_p), ("status", c_void_p), ("position", c_int64), ("slots_total", c_int64), ("table_stride", c_int64),
+                ("tables", c_void_p), ("positions", c_void_p), ("starts", c_void_p), ("bases", c_void_p), ("out_keys", c_void_p),
+                ("out_values", c_void_p), ("out_tables", c_void_p), ("out_positions", c_void_p), ("status", c_void_p), ("position", c_int64), ("slots_total", c_int64), ("table_stride", c_int64),
                 ("sequences", c_int32), ("width", c_int32), ("tokens", c_int32), ("kv_heads", c_int32), ("dim", c_int32),
-                ("page", c_int32), ("out_dtype", c_int32)]
+                ("page", c_int32), ("out_dtype", c_int32), ("keep_ids", c_int32)]
 
 
 class NormRopeParams(Structure):

@@ -92,16 +92,25 @@ template <bool BF16>
 __global__ void __launch_bounds__(256) expand4_kernel(const crit_b200_expand_params p, const int words) {
     const int j = blockIdx.x, s = blockIdx.y, is_v = blockIdx.z;
     const int tokens = p.starts ? p.starts[s + 1] - p.starts[s] : p.tokens;
-    const int64_t length = (p.positions ? p.positions[s] : p.position) + tokens;
-    const int64_t to = (int64_t)s * p.width + j;
-    if (!is_v && threadIdx.x == 0) p.out_tables[to] = (int32_t)to;
-    if ((int64_t)j * p.page >= length) return;
+    const int64_t said = p.positions ? p.positions[s] : p.position, room = (int64_t)p.width * p.page - tokens;
+    const int64_t position = said > room ? (room > 0 ? room : 0) : (said > 0 ? said : 0), length = position + tokens;
+    if (j == 0 && !is_v && threadIdx.x == 0) {
+        if (p.out_positions) p.out_positions[s] = position;
+        if ((said != position || room < 0) && p.status) atomicExch(p.status, CRIT_B200_STATUS_PLAN);
+    }
+    int32_t* const entry = p.out_tables + (int64_t)s * p.width + j;
+    if ((int64_t)j * p.page >= length) {
+        if (!is_v && threadIdx.x == 0) *entry = 0;                   // (not read)
+        return;
+    }
     const uint32_t pages_total = (uint32_t)(p.slots_total / p.page);
     uint32_t pg = (uint32_t)p.tables[(int64_t)s * p.table_stride + j];
     if (pg >= pages_total) {                       // outside the page tensor: its last page instead, and reported
         if (threadIdx.x == 0 && p.status) atomicExch(p.status, CRIT_B200_STATUS_BOUNDS);
         pg = pages_total - 1;
     }
+    const int64_t to = p.keep_ids ? (int64_t)pg : (p.bases ? (int64_t)p.bases[s] : (int64_t)s * p.width) + j;
+    if (!is_v && threadIdx.x == 0) *entry = (int32_t)to;
     const uint32_t* codes = reinterpret_cast<const uint32_t*>(is_v ? p.value_pages : p.key_pages) + (int64_t)pg * words;
     const uint8_t* scales = reinterpret_cast<const uint8_t*>(is_v ? p.value_scales : p.key_scales) + (int64_t)pg * (words >> 2);
     uint4* out = reinterpret_cast<uint4*>(is_v ? p.out_values : p.out_keys) + to * words;

@@ -99,11 +99,12 @@ typedef struct crit_b200_gather_params {
 
 int crit_b200_gather(const crit_b200_gather_params* params, void* stream);
 
-/* 4-bit pages (kind 5) as 16-bit ones: page j of each sequence's table goes to page s * width + j of out_keys and out_values
+/* 4-bit pages (kind 5) as 16-bit ones: page j of each sequence's table goes to page bases[s] + j of out_keys and out_values
  * (bf16 or FP16; every value is exact there, FP16 up to its range), as far as the sequence's positions go (its first new
- * position + its tokens); out_tables gets the page ids s * width + j, the table that reads them.  What crit_b200_prefill
- * reads a 4-bit cache through: its chunks read every page once a 256 query rows, so one pass over the codes costs little
- * and the tcgen05 tiles take the values without a second rounding. */
+ * position + its tokens); out_tables gets those page ids, the table that reads them.  With keep_ids a page goes to the page
+ * of its own id instead (pages that sequences share are written by each, the same bytes): the outputs hold the pool's pages then,
+ * however many the tables name.  What crit_b200_prefill reads a 4-bit cache through: its chunks read every page once a 256 query
+ * rows, so one pass over the codes costs little and the tcgen05 tiles take the values without a second rounding. */
 typedef struct crit_b200_expand_params {
     const void* key_pages;       /* kind 5 */
     const void* value_pages;
@@ -112,14 +113,17 @@ typedef struct crit_b200_expand_params {
     const int32_t* tables;       /* [sequences][table_stride] page ids */
     const int64_t* positions;    /* [sequences] on the device, or NULL: `position` (one sequence) */
     const int32_t* starts;       /* [sequences + 1] on the device, or NULL: `tokens` a sequence */
-    void* out_keys;              /* [sequences * width][page][kv_heads][dim] 16-bit */
+    const int32_t* bases;        /* [sequences] on the device: the first page of each sequence in the outputs; NULL: s * width */
+    void* out_keys;              /* [pages][page][kv_heads][dim] 16-bit */
     void* out_values;
     int32_t* out_tables;         /* [sequences][width] */
-    int32_t* status;             /* or NULL: CRIT_B200_STATUS_BOUNDS for a page id outside the page tensors */
+    int64_t* out_positions;      /* [sequences], or NULL: the positions, brought within what a table of `width` pages holds */
+    int32_t* status;             /* or NULL: CRIT_B200_STATUS_BOUNDS for a page id outside the page tensors, CRIT_B200_STATUS_PLAN for
+                                    a position outside the table */
     int64_t position;
     int64_t slots_total;         /* slots each page tensor stores */
     int64_t table_stride;
-    int32_t sequences, width, tokens, kv_heads, dim, page, out_dtype;
+    int32_t sequences, width, tokens, kv_heads, dim, page, out_dtype, keep_ids;
 } crit_b200_expand_params;
 
 /* n numbers of host memory (read at the call) to `to` on the device, in stream order: as launch parameters, 256 a launch, so that

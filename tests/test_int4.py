@@ -163,3 +163,12 @@ def test_splits_past_a_page_table_and_tables_past_32_bits_are_refused(lib):
     for pages in (-1, 1 << 28):
         p.table_pages = pages
         assert lib.crit_b200_attend(ctypes.byref(p), None) == -2
+
+
+def test_the_pages_of_prompt_chunks():
+    import crit_b200 as pk
+    assert pk._pages_of([0, 5, 16, 7], [1, 21, 16, 7], 9, 4, 16) == [1, 2, 1, 1]
+    assert pk._pages_of(None, None, 64, 4, 16) is None
+    for positions, ends, tokens in (([0], [65], 65), (None, None, 65), ([-1], [3], 4), ([3, -5], [5, 2], 7)):
+        with pytest.raises(ValueError):
+            pk._pages_of(positions, ends, tokens, 4, 16)
