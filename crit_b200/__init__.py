@@ -473,13 +473,14 @@ def norm_rope_write(q, keys, values, positions, frequencies, slots, key_pages, v
                     multipliers=(1.0, 1.0), q_weight=None, key_weight=None, eps=1e-6, offset=0.0, axes=None, interleaved=False,
                     magnitude=1.0, q_out=None, keys_out=None):
     """norm_rope with write() in the same launch: the queries and keys normed and turned, the keys and the values [tokens]
-    [kv_heads][value_dim] (None: keys only) stored at their slots of one layer's pages -> the queries.  The keys go to the
-    pages from their FP32 values, with no rounding to their type on the way (16-bit pages hold what norm_rope + write
-    would put there); keys_out takes them too when given (no output lies in the values' memory).  "fp8:page" pages, whose scales are a page's rows together, take
-    two launches.  Arguments as norm_rope's and write's."""
-    _cuda(q, "q")
+    [kv_heads][value_dim] (None: keys only) stored at their slots of one layer's pages -> the queries (q None: None).  The keys go
+    to the pages from their FP32 values, with no rounding to their type on the way (16-bit pages of that type hold what
+    norm_rope + write would put there); keys_out takes them too when given (no output lies in the values' memory).  "fp8:page"
+    pages, whose scales are a page's rows together, take two launches, the keys rounded to their type between them.  Arguments
+    as norm_rope's and write's."""
     if keys is None:
         raise ValueError("norm_rope_write stores keys (and values): pass keys")
+    _cuda(q if q is not None else keys, "q")
     if values is not None and values.shape[:2] != keys.shape[:2]:
         raise ValueError(f"values are a row a token and kv head, like the keys' {list(keys.shape[:2])}, not {list(values.shape[:2])}")
     if values is not None and values.numel() and any(x is not None and x.data_ptr() == values.data_ptr() for x in (q_out, keys_out)):
