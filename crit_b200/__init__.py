@@ -328,11 +328,13 @@ def _append_params(keys, values, slots, key_pages, value_pages, kind, key_scales
         values = values.contiguous()
     if slots.dtype is not torch.int64 or not slots.is_contiguous() or slots.numel() != T or slots.get_device() != place:
         raise ValueError(f"slots are contiguous int64 [{T}] on the keys' device")
+    if key_pages is None or (values is not None and value_pages is None and k_kind != 5):
+        raise ValueError("write stores rows in pages: pass them beside the rows")
     if not key_pages.is_contiguous() or (value_pages is not None and not value_pages.is_contiguous()):
         raise ValueError("pages are contiguous [slots][kv_heads][dim] storage")
     page, dv = 1, d
     if k_kind == 5:
-        if key_pages is None or (hkv, d) != _check4(key_pages, key_scales, "keys") or key_pages.get_device() != place:
+        if (hkv, d) != _check4(key_pages, key_scales, "keys") or key_pages.get_device() != place:
             raise ValueError(f"int4 keys [{T}][{hkv}][{d}] go to pages [...][{hkv}][{d // 2}] on their device")
         if values is not None:
             if value_pages is None or value_scales is None:
@@ -346,11 +348,34 @@ def _append_params(keys, values, slots, key_pages, value_pages, kind, key_scales
     value_at = value_token = value_head = 0
     if values is not None:
         value_at, (value_token, value_head, _), dv = values.data_ptr(), values.stride(), values.shape[-1]
+    if k_kind == 5:                              # (checked above)
+        held = key_pages.numel() * 2 // (hkv * d)
+        if values is not None:
+            held = min(held, value_pages.numel() * 2 // (hkv * dv))
+    else:
+        held = _slots_held(key_pages, key_scales, k_kind, hkv, d, page, place)
+        if values is not None:
+            if values.shape[0] < T or values.shape[1] != hkv or values.get_device() != place:
+                raise ValueError(f"values are [{T}][{hkv}][value_dim] on the keys' device, not {list(values.shape)}")
+            held = min(held, _slots_held(value_pages, value_scales, k_kind, hkv, dv, page, place))
+    if T and held < 1:
+        raise ValueError("the pages (and their scales) hold no slot")
     key_token, key_head, _ = keys.stride()
     p = _lib.block(_lib.AppendParams, keys.data_ptr(), value_at, slots.data_ptr(), key_pages.data_ptr(), _ptr(value_pages), _ptr(key_scales), _ptr(value_scales),
-                   _ptr(_status_word(keys.device)), T, key_pages.numel() * (2 if k_kind == 5 else 1) // (hkv * d), key_token, key_head, value_token, value_head,
+                   _ptr(_status_word(keys.device)), T, held, key_token, key_head, value_token, value_head,
                    hkv, d, dv, page, k_kind, in_dtype, _page_dtype(kind, key_pages), multipliers[0], multipliers[1])
     return p, (keys, values)
+
+
+def _slots_held(pages, scales, k_kind, heads, dim, page, place):
+    """The slots that a page tensor (of another kind than "int4") and its scales have room for: the append writes to none beyond."""
+    if pages.get_device() != place:
+        raise ValueError("pages are on the keys' device")
+    if k_kind < 2:
+        return pages.numel() // (heads * dim)
+    if scales is None or scales.dtype is not torch.float32 or not scales.is_contiguous() or scales.get_device() != place:
+        raise ValueError("scales are contiguous FP32 on the keys' device, a tensor beside each of the page tensors")
+    return min(pages.numel() // (heads * dim), scales.numel() // heads * (page if k_kind == 4 else 1))
 
 
 # -- norm and rotation ----------------------------------------------------------------------------------------------------
