@@ -410,6 +410,20 @@ def _vectors(x):
     return x if _vectors_fit(x) else x.clone(memory_format=torch.contiguous_format)
 
 
+def _bytes(x):
+    """The addresses a tensor lies between."""
+    at = x.data_ptr()
+    return at, at + (sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1) * x.element_size() if x.numel() else at
+
+
+def _in_place(out, x):
+    """Whether rows may be written to `out` as they are made of x's: its own place, or memory apart from it."""
+    if out.data_ptr() == x.data_ptr() and out.stride() == x.stride():
+        return True
+    (a, b), (c, d) = _bytes(out), _bytes(x)
+    return b <= c or d <= a
+
+
 def _norm_rope_params(q, keys, positions, frequencies, q_weight, key_weight, eps, offset, axes, interleaved, magnitude, q_out, keys_out, writes):
     """norm_rope's arguments checked: (parameter block, [q, keys] as they are read, [q, keys] outputs, outputs to copy)."""
     given = q if q is not None else keys
@@ -451,11 +465,17 @@ def _norm_rope_params(q, keys, positions, frequencies, q_weight, key_weight, eps
         elif out is not None:
             if out.shape != x.shape or out.dtype != dtype or out.get_device() != place:
                 raise ValueError(f"the {what} output has the shape, dtype and device of {what}")
-            if not _vectors_fit(out):                  # made beside it and copied
+            if out.numel() and any(n > 1 and not s for n, s in zip(out.shape, out.stride())):
+                raise ValueError(f"the {what} output's rows lie apart from one another")
+            if not _vectors_fit(out) or not _in_place(out, x):         # made beside it and copied
                 into = _like(x)
                 copies.append((out, into))
         reads.append(read), outs.append(out), at.append((read.data_ptr(), _ptr(into)))
         strides.append(read.stride() + (into.stride() if into is not None else (0, 0, 0)))
+    # (the launch's warps read one tensor's rows while others write the other's)
+    if T and q is not None and keys is not None and ((q_out is not None and (q_out.data_ptr() == keys.data_ptr() or keys_out is not None and
+            q_out.data_ptr() == keys_out.data_ptr())) or (keys_out is not None and keys_out.data_ptr() == q.data_ptr())):
+        raise ValueError("the queries' and the keys' outputs are in each other's or the other input's place")
     (q_at, q_to), (k_at, k_to) = at
     a, b = strides
     p = _lib.block(_lib.NormRopeParams, q_at, k_at, q_to, k_to, positions.data_ptr(), frequencies.data_ptr(), _ptr(axes), _ptr(q_weight), _ptr(key_weight),
@@ -475,7 +495,7 @@ def norm_rope(q, keys, positions, frequencies, *, q_weight=None, key_weight=None
     (i, rotary / 2 + i), or (2 i, 2 i + 1) with interleaved.  The angle of pair i is position * frequencies[i], made in FP64;
     positions int64 [tokens], or [axes][tokens] with axes int32 [rotary / 2] naming the axis each pair turns with
     (rope_axes).  Sums are FP32, a result is rounded once.  q_out / keys_out: where to put them (q and keys themselves for
-    in place).  Heads of 32..256 in steps of 32."""
+    in place; in no other argument's memory).  Heads of 32..256 in steps of 32."""
     if q is None and keys is None:
         raise ValueError("norm_rope takes q, keys or both")
     _cuda(q if q is not None else keys, "q")

@@ -58,3 +58,32 @@ def test_values_of_fewer_pages_bound_the_slots():
             assert pk.status() == 3
             pk._status[str(q.device)].copy_(before)
             assert k.view(torch.uint8).flatten(0, 1)[5].any() and not k.view(torch.uint8).flatten(0, 1)[70].any()
+
+
+def test_outputs_that_meet_their_inputs_in_memory():
+    q, keys, qw, kw, positions, frequencies = inputs(40, 4, 4, 64, 64, torch.bfloat16, 4)
+    norm = dict(q_weight=qw, key_weight=kw)
+    want = pk.norm_rope(q, keys, positions, frequencies, **norm)
+    buffer = torch.zeros(41, 4, 64, dtype=q.dtype, device="cuda")
+    for shift in (0, 1):                                                  # a token further on, and a token back
+        buffer[1 - shift:41 - shift] = q
+        pk.norm_rope(buffer[1 - shift:41 - shift], None, positions, frequencies, q_weight=qw, q_out=buffer[shift:40 + shift])
+        assert torch.equal(buffer[shift:40 + shift], want[0])
+    square = torch.empty(8, 8, 64, dtype=q.dtype, device="cuda")          # the same memory, the other way about
+    square.copy_(torch.cat([q[:8], q[8:16]], 1))
+    turned, p8 = square.transpose(0, 1), positions[:8]
+    right = pk.norm_rope(square.clone(), None, p8, frequencies, q_weight=qw)[0]
+    pk.norm_rope(square, None, p8, frequencies, q_weight=qw, q_out=turned)
+    assert torch.equal(turned, right)
+    packed = torch.cat([q, keys], 1)                                      # a packed projection, in place
+    views = packed[:, :4], packed[:, 4:]
+    pk.norm_rope(*views, positions, frequencies, q_out=views[0], keys_out=views[1], **norm)
+    assert torch.equal(views[0], want[0]) and torch.equal(views[1], want[1])
+    out = torch.empty_like(q)
+    for bad in (dict(q_out=keys), dict(keys_out=q), dict(q_out=out, keys_out=out), dict(q_out=keys, keys_out=q)):
+        with pytest.raises(ValueError, match="place"):
+            pk.norm_rope(q, keys, positions, frequencies, **norm, **bad)
+    for bad in (out[:1].expand(40, 4, 64), out[:, :1].expand(40, 4, 64)):
+        with pytest.raises(ValueError, match="apart"):
+            pk.norm_rope(q, keys, positions, frequencies, q_out=bad, **norm)
+    assert pk.status() == 0
