@@ -132,9 +132,9 @@ def release(key):
 
 def _workspace(device, floats, given):
     if given is not None:
-        if given.dtype != torch.float32 or given.numel() < floats or not given.is_contiguous():
-            raise ValueError(f"attend's workspace holds {given.numel()} floats; this launch needs {floats} "
-                             "(workspace_floats)")
+        if given.dtype != torch.float32 or given.numel() < floats or not given.is_contiguous() or given.device != device:
+            raise ValueError(f"attend's workspace holds {given.numel()} floats on {given.device}; this launch needs {floats} "
+                             f"contiguous FP32 ones on {device} (workspace_floats)")
         return given
     at = (device.index, getattr(_owner, "key", None))
     found = _workspaces.get(at)
@@ -728,6 +728,15 @@ def attend(q, key_pages, value_pages, kind, tables, rows, starts, firsts, column
         for x in (tables, rows, starts, firsts, counts, offsets, out, lse):
             if x is not None and x.get_device() != place:
                 raise ValueError("attend's tensors are on q's device")
+        for x in (rows, starts, firsts, counts, offsets):
+            if x is not None and (x.numel() < R or not x.is_contiguous()):
+                raise ValueError(f"rows, starts, firsts, counts and offsets are contiguous, an entry each of the {R} rows")
+        if workspace is not None and workspace.get_device() != place:
+            raise ValueError("attend's workspace is on q's device")
+        if any(x is not None and x.dtype is not torch.int32 for x in (counts, offsets)):
+            raise ValueError("counts and offsets are int32")
+        if out is not None and out.shape != q.shape:
+            raise ValueError(f"out is [{T}][{hq}][{d}], as q")
     if tables.dtype != torch.int32 or tables.stride(-1) != 1 or rows.dtype != torch.int32 or \
             starts.dtype != torch.int32 or firsts.dtype != torch.int64:
         raise ValueError("tables, rows and starts are int32, firsts int64")
@@ -983,13 +992,18 @@ def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scale
         raise ValueError("prompt chunks read keys and values of one width")
     if not key_pages.is_contiguous() or not value_pages.is_contiguous():
         raise ValueError("pages are contiguous [slots][kv_heads][dim] storage")
-    out = torch.empty_like(q) if out is None else out
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != q.get_device():
+        raise ValueError(f"out is [{T}][{hq}][{d}] in q's dtype, on its device")
     if table.dtype not in (torch.int32, torch.int64) or table.dim() not in (1, 2):
         raise ValueError("table is the sequence's page ids, int32 (read in place) or int64 (converted)")
     if table.dtype != torch.int32 or not table.is_contiguous():
         table = table.to(torch.int32).contiguous()       # (the reference's pool hands its tables over as int64 slices)
     if q.stride(-1) != 1 or out.stride(-1) != 1:
         raise ValueError("q and out have contiguous last dimensions")
+    if lse is not None and (lse.dtype is not torch.float32 or lse.shape != (T, hq) or not lse.is_contiguous() or lse.get_device() != q.get_device()):
+        raise ValueError(f"lse is contiguous FP32 [{T}][{hq}] on q's device")
     positions_at = starts_at = sequences = table_stride = 0
     if k_kind == 5 and torch.is_tensor(position) and position.get_device() != q.get_device():
         raise ValueError("positions read on the device are on q's device")

@@ -140,3 +140,34 @@ def test_rows_that_end_or_begin_past_their_page_table(engine, columns):
               key_scales=cache.ks, value_scales=cache.vs, context=True, **kw)
     assert pk.status() == 2
     pk._status[str(q.device)].copy_(before)
+
+
+def test_arguments_that_a_launch_would_read_or_write_past():
+    cache = Cache4.filled(2, 128, 16, [40, 50, 60], seed=311)
+    q = _queries(3, 8, 128, torch.bfloat16, 312)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    rows, firsts = torch.arange(3, **i32), torch.tensor([39, 49, 59], device="cuda")
+    ok = dict(tables=cache.tables, rows=rows, starts=rows, firsts=firsts, counts=torch.ones(3, **i32), out=torch.empty_like(q))
+
+    def attend(**change):
+        a = {**ok, **change}
+        return pk.attend(q, cache.k, cache.v, "int4", a.pop("tables"), a.pop("rows"), a.pop("starts"), a.pop("firsts"), 1, 16, key_scales=cache.ks,
+                         value_scales=cache.vs, **a)
+    attend()
+    wide = torch.zeros(3, 2, **i32)
+    space = torch.empty(1 << 20)
+    for change, match in ((dict(rows=rows[:2]), "an entry each"), (dict(firsts=firsts[:2]), "an entry each"), (dict(counts=torch.ones(2, **i32)), "an entry each"),
+                          (dict(rows=wide[:, 0]), "contiguous"), (dict(firsts=firsts.repeat(2).view(3, 2)[:, 0]), "contiguous"),
+                          (dict(counts=torch.ones(3, dtype=torch.int64, device="cuda")), "int32"), (dict(out=torch.empty_like(q)[:2]), "as q"),
+                          (dict(out=torch.empty(3, 8, 64, dtype=q.dtype, device="cuda")), "as q"), (dict(workspace=space), "workspace"),
+                          (dict(workspace=space, engine="even"), "workspace"), (dict(workspace=space, chunk=16), "workspace")):
+        with pytest.raises(ValueError, match=match):
+            attend(**change)
+    chunk = lambda **kw: pk.prefill(q, cache.k, cache.v, "int4", cache.tables[2], 50, 16, key_scales=cache.ks, value_scales=cache.vs, **kw)
+    chunk()
+    for kw, match in ((dict(out=torch.empty_like(q)[:2]), "out is"), (dict(out=torch.empty(3, 8, 128, device="cuda")), "out is"), (dict(out=torch.empty_like(q).cpu()), "out is"),
+                      (dict(lse=torch.empty(2, 8, device="cuda")), "lse is"), (dict(lse=torch.empty(8, 3, device="cuda").T), "lse is"),
+                      (dict(lse=torch.empty(3, 8, dtype=torch.float64, device="cuda")), "lse is"), (dict(lse=torch.empty(3, 8)), "lse is")):
+        with pytest.raises(ValueError, match=match):
+            chunk(**kw)
+    assert pk.status() == 0
