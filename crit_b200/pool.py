@@ -134,8 +134,9 @@ class KVPool:
         self.value_dim = head_dim if value_dim is None else int(value_dim)
         self.page, self.device, self.dtype = page, torch.device(device), dtype
         self.storage = {"bf16": torch.bfloat16, "fp16": torch.float16, "int8": torch.int8, "int4": torch.uint8}.get(dtype, torch.float8_e4m3fn)
-        if dtype == "int4" and (head_dim % 32 or self.value_dim % 32):
-            raise ValueError(f"int4 pages hold heads of a multiple of 32 elements, not {head_dim} and {self.value_dim}")
+        if dtype == "int4" and (head_dim % 32 or self.value_dim != head_dim):
+            raise ValueError(f"int4 pools hold keys and values of one width (as attention reads them), a multiple of 32 elements, "
+                             f"not {head_dim} and {self.value_dim}")
         packed = 2 if dtype == "int4" else 1                # elements a stored one holds
         self.compute = torch.float16 if dtype == "fp16" else torch.bfloat16
         self.pages = math.ceil(tokens / page)
@@ -420,23 +421,25 @@ class KVPool:
                            self.v[i] if self.value_dim else None, self.dtype, self.k_scales[i] if scaled else None,
                            self.v_scales[i] if scaled and self.value_dim else None, multipliers=self.scale_values[i])
 
-    def norm_rope_write(self, layer, slots, queries, keys, values, positions, frequencies, **rotation):
+    def norm_rope_write(self, layer, slots, queries, keys, values, positions, frequencies, *, keys_out=None, **rotation):
         """A step's queries and keys normed and turned, and the keys and values stored at their slots, in one launch
-        (crit_b200.norm_rope_write, whose keyword arguments these are) -> the queries.  A prompt step of a pool with a
-        fresh buffer keeps the turned keys and the values there, as write() does."""
+        (crit_b200.norm_rope_write, whose keyword arguments these are, but for the pages' multipliers) -> the queries.  A prompt
+        step of a pool with a fresh buffer keeps the turned keys and the values there, as write() does."""
         self._on_gpu("norm_rope_write")
         i, tokens = self.layers[layer], keys.shape[0]
         scaled = self.dtype in SCALED
         fresh = self.fresh_k is not None and self._staging and tokens <= self.fresh_tokens
-        turned = None
+        turned = keys_out
         if fresh:
-            turned = self.fresh_k[:tokens] if keys.dtype == self.compute else keys.new_empty(keys.shape)
+            self._fresh_buffer.tag = None           # (what it holds is being replaced)
+            if turned is None:
+                turned = self.fresh_k[:tokens] if keys.dtype == self.compute else keys.new_empty(keys.shape)
         found = self.kernels.norm_rope_write(queries, keys, values if self.value_dim else None, positions, frequencies, slots, self.k[i],
                                              self.v[i] if self.value_dim else None, self.dtype, self.k_scales[i] if scaled else None,
                                              self.v_scales[i] if scaled and self.value_dim else None, multipliers=self.scale_values[i],
                                              keys_out=turned, **rotation)
         if fresh:
-            if keys.dtype != self.compute:
+            if turned.data_ptr() != self.fresh_k.data_ptr():
                 self.fresh_k[:tokens].copy_(turned)
             self.fresh_v[:tokens].copy_(values)
             self._fresh_buffer.tag = (id(self), layer, tokens, self._reserves)

@@ -87,3 +87,26 @@ def test_outputs_that_meet_their_inputs_in_memory():
         with pytest.raises(ValueError, match="apart"):
             pk.norm_rope(q, keys, positions, frequencies, q_out=bad, **norm)
     assert pk.status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_pools_step_gives_the_turned_keys_too(dtype):
+    """keys_out through the pool, with a fresh buffer and without; a refused step leaves no fresh rows behind."""
+    from crit_b200.batch import StepBatch
+    from crit_b200.pool import FreshBuffer, KVPool
+    q, keys, qw, kw, positions, frequencies = inputs(40, 8, 2, 64, 64, dtype, 5)
+    values, positions = torch.randn_like(keys), torch.arange(40, device="cuda")
+    want = pk.norm_rope(q, keys, positions, frequencies, q_weight=qw, key_weight=kw)
+    for fresh in (None, FreshBuffer(torch.zeros(1 << 20, dtype=torch.uint8, device="cuda"))):
+        pool = KVPool([0], 2, 64, 256, "cuda", "int4", window=16, fresh=fresh)
+        pool.open("a")
+        slots, turned = pool.reserve(StepBatch.build([("a", 0, 40)], "cuda")), torch.empty_like(keys)
+        found = pool.norm_rope_write(0, slots, q, keys, values, positions, frequencies, q_weight=qw, key_weight=kw, keys_out=turned)
+        assert torch.equal(found, want[0]) and torch.equal(turned, want[1])
+        if fresh is not None:
+            rows = pool.fresh_rows(0, 40)
+            assert torch.equal(rows[0], want[1].bfloat16()) and torch.equal(rows[1], values.bfloat16())
+            with pytest.raises(ValueError):
+                pool.norm_rope_write(0, slots[:3], q, keys, values, positions, frequencies, q_weight=qw, key_weight=kw)
+            assert pool.fresh_rows(0, 40) is None
+    assert pk.status() == 0

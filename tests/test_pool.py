@@ -139,3 +139,11 @@ def test_the_native_page_allocator_takes_the_lowest_free_page():
     assert (pages, short) == ([1, 2, 3], False) and pager.floor() == 4
     pages, short = pager.grow([0, 0], [3, 3])                                         # 4 free, 6 wanted
     assert (pages, short) == ([4, 5, 6, 7], True) and pager.free() == 0 and pager.take() == -1
+
+
+def test_an_int4_pool_holds_keys_and_values_of_one_width():
+    from crit_b200.pool import KVPool
+    assert KVPool([0], 1, 64, 64, "cpu", "int4").k.shape == (1, 5, 16, 1, 32)
+    for head, value in ((64, 128), (64, 0), (128, 64), (48, 48)):
+        with pytest.raises(ValueError, match="int4"):
+            KVPool([0], 1, head, 64, "cpu", "int4", value_dim=value)
