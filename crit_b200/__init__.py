@@ -733,7 +733,7 @@ def attend(q, key_pages, value_pages, kind, tables, rows, starts, firsts, column
                 raise ValueError(f"rows, starts, firsts, counts and offsets are contiguous, an entry each of the {R} rows")
         if workspace is not None and workspace.get_device() != place:
             raise ValueError("attend's workspace is on q's device")
-        if any(x is not None and x.dtype is not torch.int32 for x in (counts, offsets)):
+        if (counts is not None and counts.dtype is not torch.int32) or (offsets is not None and offsets.dtype is not torch.int32):
             raise ValueError("counts and offsets are int32")
         if out is not None and out.shape != q.shape:
             raise ValueError(f"out is [{T}][{hq}][{d}], as q")
@@ -903,17 +903,17 @@ def _expansion(device, size, given, steady):
         return given
     if not steady and not torch.cuda.is_current_stream_capturing():
         try:
-            return torch.empty(1 << (size - 1).bit_length(), dtype=torch.uint8, device=device)
+            return torch.empty(1 << max(size - 1, 15).bit_length(), dtype=torch.uint8, device=device)
         except torch.OutOfMemoryError:
             pass
-    return torch.empty(size, dtype=torch.uint8, device=device)
+    return torch.empty(max(size, 16), dtype=torch.uint8, device=device)
 
 
-def _expanded(positions_at, starts_at, bases_at, q, key_pages, value_pages, key_scales, value_scales, table, position, tokens, pages, width, page, workspace):
+def _expanded(q, key_pages, value_pages, key_scales, value_scales, table, position, ahead, starts, tokens, taken, width, page, workspace):
     """4-bit pages as 16-bit ones of q's type in memory of the launch's own, one launch: (that memory, the addresses of the keys,
-    the values, the table that reads them and the positions, the slots of the pages).  pages: how many the sequences take
-    together, at the bases, where the host knows; None: positions on the device, room for every page the tables (of `width`) may
-    name, or for the pool's where those are fewer."""
+    the values, the table that reads them, the positions and the starts, the slots of the pages).  taken: the pages of each
+    sequence, one sequence's after another's, where the host knows; None: positions on the device, room for every page that the
+    tables (of `width`) may name, or for the pool's where those are fewer."""
     hkv, d = key_pages.shape[-2], q.shape[-1]
     place = q.get_device()
     if value_scales is None or _check4(key_pages, key_scales, "keys") != (hkv, d) or _check4(value_pages, value_scales, "values") != (hkv, d) or \
@@ -923,20 +923,26 @@ def _expanded(positions_at, starts_at, bases_at, q, key_pages, value_pages, key_
         raise ValueError("q is bf16 or fp16")
     several = table.dim() == 2
     sequences, slots = table.shape[0] if several else 1, key_pages.numel() * 2 // (hkv * d)
-    steady = pages is None                                             # (the same room whatever the positions are)
-    keep_ids = steady and slots // page < sequences * width
-    if steady:
-        pages = slots // page if keep_ids else sequences * width
+    keep_ids = taken is None and slots // page < sequences * width
+    pages = sum(taken) if taken is not None else slots // page if keep_ids else sequences * width
+    bases = [0, *itertools.accumulate(taken)][:sequences] if several and taken is not None else []
+    numbers, ints = _packed(ahead, (starts or []) + bases)
     side = pages * page * hkv * d * 2                                  # bytes of the keys, or the values
-    held = _expansion(q.device, 2 * side + 8 * sequences + 4 * sequences * width + 16, workspace, steady)
+    read = taken is None                                               # (positions that the device reads)
+    held = _expansion(q.device, 2 * side + 8 * len(numbers) + 8 * read * sequences + 4 * sequences * width, workspace, read)
     keys = held.data_ptr()
-    values, found = keys + side, keys + 2 * side                       # then the positions, then the table
-    on_device = positions_at if several else _ptr(position) if torch.is_tensor(position) else 0
+    sent = keys + 2 * side                                             # the lists; the positions read, brought within the tables; the table
+    found = sent + 8 * len(numbers)
+    if numbers:
+        _send(numbers, sent, q.device)
+    starts_at, bases_at = sent + 8 * ints if starts else 0, sent + 8 * ints + 4 * len(starts or ()) if bases else 0
+    said, at = (position.data_ptr(), found) if read else (sent, sent) if ahead else (0, 0)
+    tables_at = found + 8 * read * sequences
     e = _lib.block(_lib.ExpandParams, key_pages.data_ptr(), value_pages.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), table.data_ptr(),
-                   on_device, starts_at, bases_at, keys, values, found + 8 * sequences, found, _ptr(_status_word(q.device)), 0 if on_device else int(position),
+                   said, starts_at, bases_at, keys, keys + side, tables_at, found if read else 0, _ptr(_status_word(q.device)), 0 if said else int(position),
                    slots, table.stride(0) if several else 0, sequences, width, tokens, hkv, d, page, _DTYPES[q.dtype], keep_ids)
     _run("crit_b200_expand", "crit_b200.prefill", q.device, e)
-    return held, keys, values, found + 8 * sequences, found if on_device else 0, pages * page
+    return held, keys, keys + side, tables_at, at, starts_at, pages * page
 
 
 def _pages_of(positions, ends, tokens, width, page):
@@ -952,19 +958,18 @@ def _pages_of(positions, ends, tokens, width, page):
     return [-(-end // page) for end in ends]
 
 
-def _sent(positions, starts, device):
-    """Lists of positions (int64; None: none) and starts (int32; None: none) on the device: (the tensor that holds them, the
-    address of the starts).  They go as a small kernel's parameters, which wait for nothing and which a capture keeps; a copy
-    would leave a captured graph with the address of memory that is gone."""
-    numbers, odd = list(positions or ()), list(starts or ())
+def _packed(positions, ints):
+    """Lists of positions (int64; None: none) and of int32 numbers as int64 ones: (them, where the int32 ones begin)."""
+    numbers, odd = list(positions or ()), list(ints or ())
     if len(odd) % 2:
         odd.append(0)
-    at = len(numbers)
-    numbers += [a | b << 32 for a, b in zip(odd[::2], odd[1::2])]
-    held = torch.empty(len(numbers), dtype=torch.int64, device=device)
-    to = held.data_ptr()
+    return numbers + [a | b << 32 for a, b in zip(odd[::2], odd[1::2])], len(numbers)
+
+
+def _send(numbers, to, device):
+    """Numbers to the device as a small kernel's parameters, which wait for nothing and which a capture keeps; a copy would leave
+    a captured graph with the address of memory that is gone."""
     _run("crit_b200_put", "crit_b200.prefill", device, to, struct.pack(f"{len(numbers)}q", *numbers), len(numbers))
-    return held, to + 8 * at
 
 
 def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scales=None, value_scales=None,
@@ -1007,9 +1012,9 @@ def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scale
     positions_at = starts_at = sequences = table_stride = 0
     if k_kind == 5 and torch.is_tensor(position) and position.get_device() != q.get_device():
         raise ValueError("positions read on the device are on q's device")
-    bases_at, width = 0, table.shape[-1]
+    ahead = held = None                                # (held: kept until every launch is made)
     if table.dim() == 2:             # several sequences, one launch
-        S, ahead = table.shape[0], None
+        S = table.shape[0]
         if not torch.is_tensor(position):
             if len(position) != S:
                 raise ValueError("one position a sequence")
@@ -1027,27 +1032,30 @@ def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scale
                 raise ValueError("starts: S + 1 rising row numbers from 0 to the number of tokens")
             counts = [b - a for a, b in zip(starts, starts[1:])]
             most = max(counts)
-        ends = None if ahead is None else [a + n for a, n in zip(ahead, counts)]
-        numbers, held = starts or [], position                   # (held: kept until both launches are made)
         if k_kind == 5:
-            taken = _pages_of(ahead, ends, most, width, int(page))
-            numbers = numbers + [0, *itertools.accumulate(taken)][:S] if taken else numbers             # (the bases)
-        if ahead is not None or numbers:
-            held, at = _sent(ahead, numbers, q.device)
-            starts_at, bases_at = at if starts is not None else 0, at + 4 * len(starts or ()) if k_kind == 5 and ahead is not None else 0
-        positions_at, sequences, table_stride = (position if ahead is None else held).data_ptr(), S, table.stride(0)
-        T, position = most, 0
+            taken = _pages_of(ahead, None if ahead is None else [a + n for a, n in zip(ahead, counts)], most, table.shape[1], int(page))
+        else:
+            positions_at = position.data_ptr() if ahead is None else 0
+            numbers, ints = _packed(ahead, starts)
+            if numbers:
+                held = torch.empty(len(numbers), dtype=torch.int64, device=q.device)
+                at = held.data_ptr()
+                _send(numbers, at, q.device)
+                positions_at, starts_at = positions_at or at, at + 8 * ints if starts else 0
+        sequences, table_stride, T = S, table.stride(0), most
+        if ahead is not None:
+            position = 0
     elif starts is not None:
         raise ValueError("starts goes with a table of several sequences")
-    if torch.is_tensor(position) and (position.dtype != torch.int64 or position.numel() != 1 or not position.is_cuda):
+    if not sequences and torch.is_tensor(position) and (position.dtype != torch.int64 or position.numel() != 1 or not position.is_cuda):
         raise ValueError("a position read on the device is a one-element int64 tensor there")
     page, q_code = int(page), _DTYPES[q.dtype]
     if k_kind == 5:
         if not sequences:
-            taken = _pages_of(*((None, None) if torch.is_tensor(position) else ([int(position)], [int(position) + T])), T, width, page)
-        width = max(taken, default=0) if taken is not None else width
-        own, keys_at, values_at, table_at, at, slots = _expanded(positions_at, starts_at, bases_at, q, key_pages, value_pages, key_scales, value_scales, table,
-                                                                 position, T, None if taken is None else sum(taken), width, page, workspace)
+            taken = _pages_of(*((None, None) if torch.is_tensor(position) else ([int(position)], [int(position) + T])), T, table.shape[0], page)
+        width = max(taken, default=0) if taken is not None else table.shape[-1]
+        held, keys_at, values_at, table_at, at, starts_at, slots = _expanded(q, key_pages, value_pages, key_scales, value_scales, table, position, ahead, starts, T,
+                                                                             taken, width, page, workspace)
         key_scales = value_scales = None
         table_stride, k_kind, page_dtype = width if sequences else 0, 0, q_code
         if sequences:
@@ -1056,14 +1064,15 @@ def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scale
         keys_at, values_at, table_at, slots = key_pages.data_ptr(), value_pages.data_ptr(), table.data_ptr(), key_pages.numel() // (hkv * d)
         page_dtype = _page_dtype(kind, key_pages)
     device = q.device
-    if torch.is_tensor(position):
+    position_at = 0
+    if sequences:
+        position = 0
+    elif torch.is_tensor(position):
         position_at, position = at if kind == "int4" else position.data_ptr(), 0
-    else:
-        position_at, position = 0, int(position)
     q_token, q_head, _ = q.stride()
     out_token, out_head, _ = out.stride()
     p = _lib.block(_lib.PrefillParams, q.data_ptr(), out.data_ptr(), _ptr(lse), keys_at, values_at, _ptr(key_scales), _ptr(value_scales), table_at, position_at,
-                   _ptr(_status_word(device)), position, slots, q_token, q_head, out_token, out_head, T, hq, hkv, d, d, page, k_kind, page_dtype, q_code,
+                   _ptr(_status_word(device)), int(position), slots, q_token, q_head, out_token, out_head, T, hq, hkv, d, d, page, k_kind, page_dtype, q_code,
                    _PREFILL_ENGINES[engine], float(scale if scale is not None else d ** -0.5), float(multipliers[0]), float(multipliers[1]),
                    starts_at, positions_at, sequences, table_stride)
     _run("crit_b200_prefill", "crit_b200.prefill", device, p)

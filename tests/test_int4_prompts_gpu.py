@@ -46,7 +46,7 @@ def test_sequences_of_unequal_lengths_take_the_pages_they_have(hq, hkv, dim):
     took, out = _peak(lambda: _prefill(cache, q, firsts, starts=starts))
     assert took <= 2 * (own + 64 * cache.tables.shape[1]) + out.numel() * 2 + (1 << 20)       # (a power of two; and far below 8 of the longest)
     _check(cache, q, out, starts, firsts)
-    exact = torch.empty((own + 4 * 8 * cache.tables.shape[1] + 80) // 4, device="cuda")
+    exact = torch.empty((own + 4 * 8 * cache.tables.shape[1] + 8 * (8 + 9)) // 4, device="cuda")     # (the pages, their table and the lists)
     assert torch.equal(_prefill(cache, q, firsts, starts=starts, workspace=exact), out)
     device = torch.tensor(firsts, device="cuda")
     assert torch.equal(_prefill(cache, q, device, starts=starts), out)
