@@ -889,7 +889,7 @@ static int resident4(const void* fn, int threads, int smem, int* sms) {
 }
 
 // The launch of a geometry: kernel, heads a block takes, stages that the blocks' shares of an SM hold, blocks of an even launch.
-static int plan4(int q_heads, int kv_heads, int d, int columns, int n_rows, bool masks, bool fp16, bool even, Decode4Plan* out) {
+static int plan4(int q_heads, int kv_heads, int d, int columns, int n_rows, bool masks, bool even, Decode4Plan* out) {
     if (d != 64 && d != 128 && d != 256) return CRIT_B200_EUNSUPPORTED;
     const int rows = columns * (q_heads / kv_heads);
     const int nt = rows <= 8 ? 1 : (rows <= 16 || d == 256 ? 2 : 4);
@@ -905,7 +905,7 @@ static int plan4(int q_heads, int kv_heads, int d, int columns, int n_rows, bool
     u.stages = stages < 4 ? 4 : (stages > D4_MAX_STAGES ? D4_MAX_STAGES : stages);
     out->nt = nt, out->smem = 1024 + u.stages * u.stage_bytes;
     if (out->smem > 220 * 1024) return CRIT_B200_EUNSUPPORTED;
-    out->fn = decode4_pick(d, nt, masks, even && (nt > 1 || !fp16));
+    out->fn = decode4_pick(d, nt, masks, even);
     u.blocks = 0, out->sms = out->per_sm = 0;
     if (even) {
         out->per_sm = resident4((const void*)out->fn, 32 * u.heads, out->smem, &out->sms);
@@ -918,8 +918,7 @@ static int plan4(int q_heads, int kv_heads, int d, int columns, int n_rows, bool
 static int plan4(const crit_b200_attend_params& p, Decode4Plan* out) {
     const bool even = (p.flags & CRIT_B200_ATTEND_EVEN) != 0;
     if (even && (p.flags & CRIT_B200_ATTEND_PARTIALS)) return CRIT_B200_EUNSUPPORTED;
-    return plan4(p.q_heads, p.kv_heads, p.head_dim, p.columns, p.n_rows, p.parents || p.sliding > 0 || p.blocks,
-                 p.q_dtype == CRIT_B200_DTYPE_FP16, even, out);
+    return plan4(p.q_heads, p.kv_heads, p.head_dim, p.columns, p.n_rows, p.parents || p.sliding > 0 || p.blocks, even, out);
 }
 
 // Floats of an even launch's workspace: where the rows begin, and (dim + 2) a state row.
@@ -983,7 +982,7 @@ int launch_merge4(const crit_b200_attend_params& p, cudaStream_t s) {
 
 int plan_decode4(int q_heads, int kv_heads, int d, int columns, int32_t* out5) {
     Decode4Plan plan;
-    if (int e = plan4(q_heads, kv_heads, d, columns, 1, false, false, false, &plan)) return e;
+    if (int e = plan4(q_heads, kv_heads, d, columns, 1, false, false, &plan)) return e;
     int sms = 0;
     const int per_sm = resident4((const void*)plan.fn, 32 * plan.u.heads, plan.smem, &sms);
     out5[0] = 1024, out5[1] = plan.smem, out5[2] = 8 * plan.nt, out5[3] = per_sm, out5[4] = sms;
