@@ -8,7 +8,7 @@
 //
 // A warp takes a token's heads, or a part of them where there are too few tokens to fill the device: it makes the sines and
 // cosines once (32 lanes, two pairs each of a rotation of 128; the angle is a product in FP64, since a position of 2^20 times
-// a frequency loses 2^-4 of a radian in FP32, reduced to a part of a turn there and handed to sincospi in FP32), multiplies
+// a frequency loses 2^-4 of a radian in FP32, reduced to a part of a turn there and handed to sincospi in FP32, what FP32 leaves of it put back after), multiplies
 // the head weights into them, and walks the queries' rows, the keys' and (when it writes) the values'.  8, 16 or 32 lanes
 // share a row of up to 64, 128 or 256 elements: a lane holds four pairs, two vectors of four elements, so nothing crosses
 // lanes but the sum of squares, and a row is in flight while the one before it is worked on.  A row that goes to a page is
@@ -184,9 +184,11 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32, 4) norm_rope_kernel(const cri
             // at / (2 pi) less its whole turns: 1 / (2 pi) as a sum of two FP64 numbers, the product's rounding put back
             const double turns_of = at * 0.15915494309189535;
             const double rest = fma(at, 0.15915494309189535, -turns_of) + at * -9.839338337591243e-18;
+            const double halves = 2.0 * ((turns_of - rint(turns_of)) + rest);
+            const float near = (float)halves, beside = (float)(halves - (double)near) * 3.14159265f;      // what FP32 leaves of the angle, in radians
             float s, c;
-            sincospif((float)(2.0 * ((turns_of - rint(turns_of)) + rest)), &s, &c);
-            turn = make_float2(c * p.magnitude, s * p.magnitude);
+            sincospif(near, &s, &c);
+            turn = make_float2(fmaf(-s, beside, c) * p.magnitude, fmaf(c, beside, s) * p.magnitude);
         } else if (p.status) {
             atomicExch(p.status, CRIT_B200_STATUS_BOUNDS);   // an axis that positions has not: the pair becomes zeros
         }

@@ -110,3 +110,18 @@ def test_a_pools_step_gives_the_turned_keys_too(dtype):
                 pool.norm_rope_write(0, slots[:3], q, keys, values, positions, frequencies, q_weight=qw, key_weight=kw)
             assert pool.fresh_rows(0, 40) is None
     assert pk.status() == 0
+
+
+def test_cosines_and_sines_are_those_of_the_angle_in_64_bits():
+    """Pairs of (1, 0) come out as (cos, sin).  The angle is reduced in FP64 and its part beyond FP32 put back, so what is left is
+    sincospi's unit and two roundings: 2^-22 of each number (the reduction's own error is below 2^-33 of a turn here)."""
+    _, _, _, _, _, frequencies = inputs(1, 1, 1, 128, 128, torch.float32, 6)
+    positions = torch.cat([torch.arange(1, 2000), torch.randint(0, 1 << 20, (2000,), generator=torch.Generator().manual_seed(7))]).cuda()
+    for interleaved in (False, True):
+        q = torch.zeros(len(positions), 1, 128, device="cuda")
+        first, second = (slice(0, None, 2), slice(1, None, 2)) if interleaved else (slice(0, 64), slice(64, 128))
+        q[..., first] = 1.0
+        out = pk.norm_rope(q, None, positions, frequencies, interleaved=interleaved)[0][:, 0].double()
+        angle = positions.double()[:, None] * frequencies.double()
+        for got, want in ((out[:, first], angle.cos()), (out[:, second], angle.sin())):
+            assert bool(((got - want).abs() <= 2.0 ** -22 * want.abs() + 2.0 ** -30).all())
