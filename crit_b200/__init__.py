@@ -693,7 +693,10 @@ def attend(q, key_pages, value_pages, kind, tables, rows, starts, firsts, column
     pages of 128-wide heads, columns x group heads <= 32, chunk a multiple of 128; refused elsewhere).
     shards: a crit_b200.dist.ShardMerge: these pages hold one KV range of a context sharded over the ranks; every
     split state stays in the workspace, the fold of this rank's splits is stored into every rank's exchange buffer and
-    out / lse get the merge over all ranks (three launches: decode, fold + push, wait + merge)."""
+    out / lse get the merge over all ranks (three launches: decode, fold + push, wait + merge).
+    workspace: the states' (FP32; else the owner's): launches that may run at the same time, on two streams or as two graphs,
+    take one each (`owner`).  "int4" pages: nothing is read past the tables' width; of a row that ends there the columns past it
+    see the table's positions, a row that begins past it is reported (status) and, evenly, left out."""
     _refuse(fresh=fresh, derive=derive)
     # masks are served by the m16n8k16 kernels: of 4-bit pages under either engine, else "mma.sync"
     plain = (None, "mma.sync", "even") if kind == "int4" else (None, "mma.sync")
@@ -982,7 +985,8 @@ def prefill(q, key_pages, value_pages, kind, table, position, page, *, key_scale
     (equal counts, or `starts`: S + 1 ints, sequence s's tokens being rows starts[s]..starts[s+1]).  engine: None
     (tcgen05.mma tiles with TMEM accumulators for 16-bit pages of 128-wide heads, m16n8k16 tiles otherwise), "mma.sync"
     or "tcgen05" (refused where not served); "tcgen05:single" / "tcgen05:pair" also name the block shape (128 query rows
-    two blocks an SM / 256 rows over one ring of key and value tiles, which "tcgen05" picks by the launch's size).
+    two blocks an SM / 256 rows over one ring of key and value tiles, which "tcgen05" picks by the launch's size).  The
+    softmax's weights are rounded to q's type for the second product, their sum is not.
     "int4" pages are first made 16-bit ones of q's type (exact: no second rounding) in memory of the launch's own: the sequences'
     positions * kv_heads * dim * 4 bytes (with positions on the device those that the tables or the pool hold, whichever are
     fewer) and a few, of the current stream and given back when the call returns (a capture keeps its own), or `workspace` (FP32,

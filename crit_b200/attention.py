@@ -50,8 +50,8 @@ class DeviceAttention:
         need); chunk: positions per split (0: the kernels' rule).  kernels_mib: the most partials a launch takes from
         `scratch` (the engine's Scratch, crit_plugins.memory) when one is given.  prompt_reader: "prefill" or "decode".
         window_engine: "auto" (the kernels' choice, crit_b200.engine_for: E4M3 pages through tcgen05.mma where a kernel for
-        it serves the step, m16n8k16 tiles otherwise; a column's bits then depend on the window and the step it is read
-        in: exactness "repeatable"), "mma.sync" (the m16n8k16 kernel always: a column's bits are the same alone and in
+        it serves the step, 4-bit pages evenly where the partials are the kernels' own, m16n8k16 tiles otherwise; a column's
+        bits then depend on the window and the step it is read in: exactness "repeatable"), "mma.sync" (the m16n8k16 kernel always: a column's bits are the same alone and in
         any window or batch, "row-exact"), "tcgen05" (one kv head a unit, wherever that kernel serves a launch) or
         "tcgen05p" (whole page rows a unit, where that kernel serves the step).
         mode "torch", decode "flashinfer", flashinfer "auto", int8_qk and latent are the reference's other readers: not
@@ -77,7 +77,8 @@ class DeviceAttention:
     def facts(self):
         return {"reader": "crit_b200: a row's positions in contiguous splits of one chunk per pool, folded in split order; " +
                           ("a column's bits are the same alone and in any window" if self.window_engine == "mma.sync" else
-                           "E4M3 pages through tcgen05.mma where served: a column's bits depend on its window and its step"),
+                           "E4M3 pages through tcgen05.mma where served, 4-bit pages dealt out evenly: a column's bits depend on its "
+                           "window and its step"),
                 "prompt_reads": "through the prefill kernel" if self.prompt_reader == "prefill" else
                                 "in the decode's reduction (pieces of up to 64 columns)",
                 "split_kv_wide_windows": "16- or 32-row tiles; wider windows read their pages once per tile"}

@@ -5,7 +5,8 @@ from crit_b200.attention import DeviceAttention, PartitionedAttention
 
 def memory(context, options):
     """The split-K partials come from the engine's scratch (workspace_mib at most) or the kernels' own workspace:
-    nothing is allocated when the plugin is made."""
+    nothing is allocated when the plugin is made.  (A prompt chunk over 4-bit pages takes a 16-bit copy of its sequences' pages
+    from torch's allocator while it runs.)"""
     return {"device": 0, "host": 0}
 
 
