@@ -35,7 +35,7 @@
 // exact in FP16 with 3 bits to spare; bf16 weights would be 8 times coarser), while their sum is of the FP32 ones.  They are
 // 2^(x - ref + 11) with a reference that moves when a score passes it by 4 in the exponent: high in FP16's range, so that a weight
 // keeps its 11 bits down to 2^-25 of its row's largest, and what is left out below that is 2^-36 of it at the most.  (A reference
-// that moves at 1 would reach 2^-28, but moves so often that verify windows take 160 us instead of 143.  Scales on the weights
+// that moves at 1 would reach 2^-28, but moves so often that verify windows take 158 us instead of 143.  Scales on the weights
 // would take fewer instructions, 64 rows of 4,096 81 us, but round the product again, and lose it where a dominant position
 // meets small values: no better than 2^-20 of the largest at scales of 2^-3.)  Sums are FP32.
 //
@@ -46,13 +46,12 @@
 // names the pair), and merge4_kernel folds a row's consecutive slots.  No block idles while another has two splits to go.
 //
 // Measured (B200, CUDA events around graphs; HBM's floor at the measured copy bandwidth beside it): 64 rows of 4,096 positions,
-// 64 query heads on 8 of 128: 87 us (44), 3.3 TB/s; one row of 200,000, 24 on 4 of 256: 70 us (33); 32 verify windows of 6 columns, 40
-// on 8 of 128, FP16: 143 us (27); one row of 777: 11 us, two launches' latency.  Bound by instructions at the registers' occupancy:
-// of the 64 rows' launch about 340 a warp and tile (V 100, K 60, scales and softmax the rest) fill 60% of the issue slots with
-// 16 warps an SM, the integer pipe 56%, the tensor pipe a quarter; of the verify windows' 720 a tile with 8 warps an SM fill
-// 45%, each warp waiting for its own last result.  The same tiles streamed without the products take about 60 us.
-// Slower: a block's queries in shared memory for 3 blocks an SM (104 us against 85), 3 blocks of 256-wide heads (75 against 70),
-// the shifts of the codes as multiplications (87 against 81).
+// 64 query heads on 8 of 128: 88 us (44), 3.3 TB/s; one row of 200,000, 24 on 4 of 256: 71 us (33); 32 verify windows of 6 columns, 40
+// on 8 of 128, FP16: 143 us (27); one row of 777: 11 us, two launches' latency.  Cut into splits of 1,024: 98, 107, 220 and 43 us.
+// Bound by instructions at the registers' occupancy: of the 64 rows' launch about 410 a warp and tile (the values' codes 150, the
+// keys' 60, scales and softmax the rest) fill 65% of the issue slots with 16 warps an SM, the integer pipe 60%; of the verify
+// windows' 710 a tile with 8 warps an SM fill 46%, each warp waiting for its own last result.  The same tiles streamed without the
+// products take about 60 us.
 #include <mutex>
 #include <type_traits>
 
@@ -63,13 +62,14 @@ namespace crit_b200 {
 
 constexpr int D4_MAX_STAGES = 8;
 // Stages between the tile a warp works on and the one its turn refills.  A turn waits until every warp is done with the
-// tile whose stage it takes: 3 back instead of 2 the warps may stand further apart (64 sequences of 4,096, 32 heads on 8 of
-// 128: 80.6 us instead of 84.7; the other sizes 0 to 1%).
+// tile whose stage it takes: 3 back instead of 2 the warps may stand further apart (64 rows of 4,096: 87.7 us instead of 90.5, one
+// row of 200,000 70.7 instead of 72.2, verify windows 0.7% less).
 constexpr int D4_SLACK = 3;
 constexpr int D4_MAX_ROWS = 256;              // window rows an even launch lists
 
-// The most kv heads a block takes: the pieces asked of HBM are its heads' bytes of a position (8 against 4: 64 sequences of 4,096
-// 81 us against 85, verify windows of 6 143 against 147).  The blocks of so many heads an SM is to hold: a warp's accumulators
+// The most kv heads a block takes: the pieces asked of HBM are its heads' bytes of a position (8 against 4: 64 rows of 4,096
+// 88 us against 99, verify windows of 6 143 against 147).  The scales of a tile come for every kv head, whatever the block's share:
+// 6% of the bytes with 8 of 128 (each read once), 1.18 times the bytes with 32.  The blocks of so many heads an SM is to hold: a warp's accumulators
 // decide (the registers of 16 warps are 128 a thread, of 8 warps 255).
 constexpr int D4_HEADS = 8;
 constexpr __host__ __device__ int decode4_blocks(int d, int nt) { return nt == 1 && d <= 128 ? 2 : 1; }
@@ -968,7 +968,7 @@ int launch_merge4(const crit_b200_attend_params& p, cudaStream_t s) {
     Decode4Plan plan;
     if (int e = plan4(p, &plan)) return e;
     // Few rows share the blocks: a row may have a state in each, so 16 warps fold it; many rows have a few states each, a warp's
-    // work.  One row of 200,000: 67 us, with a warp 147; 64 rows of 4,096: 81 us, with 16 warps 115 (launch and fold together).
+    // work.  One row of 200,000: 71 us, with a warp 164; 64 rows of 4,096: 88 us, with 16 warps 123 (launch and fold together).
     const bool many = (int64_t)p.n_rows * (p.kv_heads / plan.u.heads) * plan.u.ctiles * 16 < plan.u.blocks;
     switch (p.head_dim) {
         case 64: launch_merge4_of<64>(p, plan, many, s); break;
