@@ -317,7 +317,8 @@ class DeviceAttention:
         """A PromptBatch: the bucket's tokens over the pool's prompt table, causal from batch.frontier_t, read on the
         device: window rows of up to 64 columns (reference: device_attention.py:577-641)."""
         import torch
-        key = (batch.bucket, str(q.device))
+        holds = pool.prompt_table.shape[1] * pool.page if pool.dtype == "int4" else None
+        key = (batch.bucket, str(q.device), holds)
         made = self._prompt_rows.get(key)
         if made is None:
             columns = min(PIECE_COLUMNS, batch.bucket)
@@ -326,8 +327,10 @@ class DeviceAttention:
             counts = torch.tensor([min(columns, batch.bucket - r * columns) for r in range(count)], dtype=torch.int32,
                                   device=q.device)
             made = self._prompt_rows[key] = (torch.zeros(count, dtype=torch.int32, device=q.device), starts, counts,
-                                             starts.long(), columns)
-        rows, starts, counts, offsets, columns = made
+                                             starts.long(), columns, torch.zeros_like(counts), None if holds is None else holds - starts)
+        rows, starts, counts, offsets, columns, none, room = made
+        if room is not None:             # (rows of padding that begin past the table would be reported: they have no columns)
+            counts = torch.clamp(room - batch.frontier_t, min=none, max=counts).to(torch.int32)
         meta = Windows(pool.prompt_table, rows, starts, counts, batch.frontier_t + offsets, columns)
         self._windows(layer, q, pool, meta, scale, out, found)
 

@@ -171,3 +171,37 @@ def test_arguments_that_a_launch_would_read_or_write_past():
         with pytest.raises(ValueError, match=match):
             chunk(**kw)
     assert pk.status() == 0
+
+
+def test_a_staged_chunk_whose_padding_passes_the_table():
+    """A bucket of 256 at the end of a table of 128 positions, captured: the chunk's tokens as they should be, nothing reported."""
+    pool = KVPool([0], 2, 64, 128, "cuda", "int4", page=16)
+    g = torch.Generator().manual_seed(321)
+    make = lambda n, h: torch.randn(n, h, 64, generator=g).bfloat16().cuda()
+    pool.open("a")
+    step = StepBatch.build([("a", 0, 90)], "cuda")
+    pool.write(0, pool.reserve(step), make(90, 2), make(90, 2))
+    pool.keep("a", 90)
+    chunk = SimpleNamespace(prompt=True, round=False, sequence="a", frontier=90, count=20, bucket=256, tokens_max=256, tokens=256,
+                            frontier_t=torch.tensor([90], device="cuda"))
+    q, keys, values, attention = make(256, 4), make(256, 2), make(256, 2), DeviceAttention()
+    pool.stage_prompt(chunk)
+    pool.write(0, pool.reserve(chunk), keys, values)
+    out = attention.forward(0, q, pool, chunk)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = attention.forward(0, q, pool, chunk)
+    for frontier, count in ((90, 20), (108, 20)):
+        if frontier > 90:
+            pool.commit_prompt(chunk)
+            chunk.frontier, chunk.count = frontier, count
+            chunk.frontier_t.fill_(frontier)
+            pool.stage_prompt(chunk)
+            pool.write(0, pool.reserve(chunk), keys, values)
+        graph.replay()
+        assert frontier > 90 or torch.equal(again[:count], out[:count])
+        cache = _as_cache(pool)
+        for c in (0, 7, count - 1):
+            want, _, room = attention4(cache, q[c], 0, frontier, c, count, c)
+            assert (np.abs(again[c].double().cpu().numpy() - want) <= bounds4(want, room, frontier + count, q.dtype)).all()
+        assert pk.status() == 0
