@@ -577,6 +577,8 @@ def gather(pages, kind, page, *, table=None, slots=None, count=None, scales=None
         raise ValueError(f"int4 rows are read through an int32 page table that holds the {count} positions, or at int64 slots")
     if count == 0:
         return out
+    if k_kind == 5 and out.data_ptr() % 16:            # (the kernel stores 16 bytes at once: made beside it)
+        return out.copy_(gather(pages, kind, page, table=table, slots=slots, count=count, scales=scales, dtype=out.dtype).view(out.shape))
     if not pages.is_contiguous():
         raise ValueError("pages are contiguous [slots][kv_heads][dim] storage")
     p = _lib.block(_lib.GatherParams, pages.data_ptr(), _ptr(scales), _ptr(table), _ptr(slots), out.data_ptr(), _ptr(_status_word(pages.device)), count,

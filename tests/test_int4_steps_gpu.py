@@ -205,3 +205,19 @@ def test_a_staged_chunk_whose_padding_passes_the_table():
             want, _, room = attention4(cache, q[c], 0, frontier, c, count, c)
             assert (np.abs(again[c].double().cpu().numpy() - want) <= bounds4(want, room, frontier + count, q.dtype)).all()
         assert pk.status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_rows_read_back_into_a_buffer_of_any_alignment(dtype):
+    cache = Cache4.filled(2, 64, 16, [50], seed=331)
+    want = pk.gather(cache.k, "int4", 16, table=cache.tables[0], count=50, scales=cache.ks, dtype=dtype)
+    slots = cache.slots(0, torch.arange(50)).view(5, 10)
+    for shift in range(0, 9):
+        buffer = torch.full((50 * 128 + 16,), -1, dtype=dtype, device="cuda")
+        out = buffer[shift:shift + 50 * 128].view(50, 2, 64)
+        got = pk.gather(cache.k, "int4", 16, table=cache.tables[0], count=50, scales=cache.ks, out=out)
+        assert got.data_ptr() == out.data_ptr() and torch.equal(out, want) and (buffer[:shift] == -1).all() and (buffer[shift + 50 * 128:] == -1).all()
+        out.zero_()
+        got = pk.gather(cache.k, "int4", 16, slots=slots, scales=cache.ks, out=out)
+        assert got.shape == (5, 10, 2, 64) and torch.equal(got.view_as(out), want) and torch.equal(out, want)
+    assert pk.status() == 0
